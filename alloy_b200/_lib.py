@@ -119,6 +119,15 @@ SIGNATURES = {
     "alloyb_kv_write": (_i, [_i, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64, _i, _p, _p]),
     "alloyb_attn_chunk": (_i, [_i, _p, _i64, _i64, _i64, _i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i,
                                _i64, _f, _p, _p]),
+    "alloyb_attn_span_workspace_bytes": (_sz, [_i] * 10),
+    "alloyb_attn_window": (_i, [_p, _i64, _i64, _i64, _i, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i,
+                                _i, _i, _f, _p, _sz, _p]),
+    "alloyb_attn_shared_prefix": (_i, [_p, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p,
+                                       _i, _i, _i, _i, _i, _i, _f, _p, _sz, _p]),
+    "alloyb_attn_scored": (_i, [_p, _i64, _i64, _i64, _i, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p, _p, _i, _i, _i, _i, _i,
+                                _i, _f, _p, _sz, _p]),
+    "alloyb_kv_evict": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
+    "alloyb_span_status": (_i, [C.POINTER(C.c_int32), _i]),
     "alloyb_moe_workspace_bytes": (_sz, [_i, _i, _i]),
     "alloyb_moe_routed": (_i, [_p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _sz, _p]),
     "alloyb_decoder_create": (_i, [C.POINTER(DecoderDesc), C.POINTER(_p)]),

@@ -1,0 +1,798 @@
+// Attention of query tokens over spans of an fp16 cache: a window with sinks, a shared prefix with an own rest, and the form that
+// keeps the attention weights.  out = sum_j softmax_j(scale q k_j) v_j over the keys j that a row sees; softmax in the exp2 frame with a
+// running maximum and sum, K and V read once.
+//
+// Few rows (one token, or as many as give 16 rows of a KV head; span_stream_kernel).  Bound: HBM, 4 D bytes a key for 4 D G n operations.
+// Every sequence's keys are cut into steps of 64, all sequences' steps laid end to end and dealt out evenly to as many CTAs as the GPU
+// holds at once, whatever the lengths: a CTA may finish one sequence and begin the next.  A warp takes 16 of a step's keys through a ring
+// of its own (cp.async, no barrier but its own), S and P V on mma.sync with the rows padded to 16.  A (sequence, KV head) that one CTA
+// covers is stored by it; the others' partial results go to a workspace and span_merge_kernel joins them.
+//
+// More rows (chunks, and all the batch's rows over a shared prefix; span_rows_kernel).  Bound: mma.sync.  A CTA owns 64 (token, head) rows,
+// a warp 16 of them, and tiles of 64 keys (32 at head_dim 256) that its warps share; the keys are split where the tiles alone leave SMs
+// empty.
+//
+// The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and the
+// merge launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
+//
+// New tokens' rows: keys from `pos` on are read from new_k / new_v directly, and written to the cache by whoever; nobody reads them there
+// in the same launch.
+#include "attn_span.cuh"
+
+namespace alloyb {
+namespace sp {
+
+// ---------------------------------------------------------------------------------------------------------------- few rows
+template <int D>
+struct StreamCfg {
+    static constexpr int SLOTS = D == 64 ? 4 : 3;
+    static constexpr int TILE = 16 * D * 2, SLOT = 2 * TILE;             // K, then V
+    static constexpr int RING = WARPS * SLOTS * SLOT, OUT = WARPS * 16 * D * 4;
+    static constexpr int Q = 16 * D * 2;
+    static constexpr int SMEM = (RING > OUT ? RING : OUT) + Q;
+};
+
+// A CTA takes at least this many steps: fewer would give more partial results than they save time.
+constexpr int MIN_STEPS = 2;
+
+__device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max((total + ctas - 1) / ctas, MIN_STEPS); }
+
+template <int D, bool SCORED, bool PREFIX>
+__global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P) {
+    using C = StreamCfg<D>;
+    pdl_launch_dependents();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int cum[MAX_BATCH + 1], seq_pos[MAX_BATCH];
+    __shared__ float back[16], sm_m[WARPS][16], sm_l[WARPS][16];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rows = P.n * P.G;
+    const uint32_t q_s = s32(smem), ring = q_s + C::Q + warp * (C::SLOTS * C::SLOT);
+    float* sm_o = reinterpret_cast<float*>(smem + C::Q);                 // [warp][16][D], in the rings' place between segments
+    pdl_wait();
+    if (warp == 0) {
+        int sum = 0;
+        if (lane == 0) cum[0] = 0;
+        for (int b0 = 0; b0 < P.B; b0 += 32) {
+            const int b = b0 + lane;
+            int x = 0;
+            if (b < P.B) {
+                const int pos = live_pos(P, b, blockIdx.x == 0);
+                seq_pos[b] = pos;
+                x = (seq_at(P, pos, 0, P.n).keys + STEP - 1) / STEP * P.KV_H;
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (b < P.B) cum[b + 1] = sum + x;
+            sum += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+    const int total = cum[P.B], per = steps_per_cta(total, gridDim.x);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= P.B; i += WARPS * 32) P.cum[i] = cum[i];
+    // new rows into the cache
+    if (P.nk) {
+        for (int i = blockIdx.x; i < P.B * P.KV_H; i += gridDim.x) {
+            const int b = i / P.KV_H, h = i - b * P.KV_H, pos = seq_pos[b];
+            if (pos < 0) continue;
+            for (int e = threadIdx.x; e < P.n * (D / 8); e += WARPS * 32) {
+                const int tok = e / (D / 8), c = (e - tok * (D / 8)) * 8;
+                const int64_t src = b * P.n_bs + h * P.n_hs + tok * P.n_ts + c, dst = (static_cast<int64_t>(i) * P.S + pos + tok) * D + c;
+                *reinterpret_cast<uint4*>(P.k + dst) = ld_after_wait(P.nk + src);
+                *reinterpret_cast<uint4*>(P.v + dst) = ld_after_wait(P.nv + src);
+            }
+        }
+    }
+
+    const int begin = min(total, static_cast<int>(blockIdx.x) * per), end = min(total, begin + per);
+    for (int s0 = begin; s0 < end;) {
+        int b = 0;
+        for (int hi = P.B; hi - b > 1;) {                                // the last sequence that begins at or before s0 and is not empty
+            const int mid = (b + hi) >> 1;
+            if (cum[mid] <= s0) b = mid;
+            else hi = mid;
+        }
+        const int seq_steps = (cum[b + 1] - cum[b]) / P.KV_H, kvh = (s0 - cum[b]) / seq_steps, item = b * P.KV_H + kvh;
+        const int step0 = s0 - cum[b] - kvh * seq_steps, steps = min(seq_steps - step0, end - s0);
+        const Seq sq = seq_at(P, seq_pos[b], 0, P.n);
+        const int64_t head = static_cast<int64_t>(item) * P.S * D;
+
+        auto request = [&](int i) {                                      // this warp's keys of the segment's i-th step
+            if (i < steps) {
+                constexpr int PIECES = D / 8;
+                const uint32_t dst = ring + i % C::SLOTS * C::SLOT;
+                const int place0 = (step0 + i) * STEP + warp * 16;
+#pragma unroll
+                for (int it = 0; it < PIECES / 2; ++it) {
+                    const int r = (it * 32 + lane) / PIECES, c = (it * 32 + lane) % PIECES, place = place0 + r;
+                    const bool live = place < sq.keys;
+                    const int j = live ? sq.row_of(place) : 0;
+                    int64_t at = head + static_cast<int64_t>(j) * D;
+                    const __half *k = P.k, *v = P.v;
+                    if (P.nk && live && j >= sq.pos) {
+                        at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
+                        k = P.nk;
+                        v = P.nv;
+                    }
+                    copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
+                    copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < C::SLOTS - 1; ++i) request(i);
+        // the rows of this (sequence, KV head); rows past the last are zero
+        for (int r = warp; r < 16; r += WARPS) {
+            const int tok = r / P.G, hg = r - tok * P.G;
+            const float f = load_q_row<D>(q_s, r, P.q, b * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, r < rows, lane);
+            if (lane == 0) back[r] = f * P.scale_log2;
+        }
+        __syncthreads();
+        const float scale[2] = {back[g], back[g + 8]};
+        const int row_pos[2] = {sq.pos + g / P.G, sq.pos + (g + 8) / P.G};
+
+        Rows<D> st;
+        st.clear();
+        for (int i = 0; i < steps; ++i) {
+            request(i + C::SLOTS - 1);
+            copy_wait<C::SLOTS - 1>();
+            __syncwarp();
+            const int place0 = (step0 + i) * STEP + warp * 16;
+            const uint32_t k_tile = ring + i % C::SLOTS * C::SLOT;
+            if (place0 < sq.keys) {
+                float s[2][4];
+                Rows<D>::template scores<1>(s, q_s, 0, k_tile, lane);
+                const bool whole = P.n == 1 && place0 + 16 <= sq.keys;   // one token sees every key of its spans
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int place = place0 + 8 * n + 2 * t + (e & 1);
+                        const bool seen = whole || (place < sq.keys && sees(P, row_pos[e >> 1], sq.row_of(place)));
+                        s[n][e] = seen ? s[n][e] * scale[e >> 1] : -INFINITY;
+                    }
+                if (SCORED) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int rr = 0; rr < 2; ++rr)
+                            if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < sq.keys)
+                                *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + g + 8 * rr) * P.pitch + place0 + 8 * n + 2 * t) =
+                                    make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
+                }
+                st.template take<1>(s, k_tile + C::TILE, lane);
+            }
+            __syncwarp();                                                // the slot has been read: the next request may fill it
+        }
+        st.sum_lanes();
+        copy_wait<0>();
+        __syncthreads();                                                 // every warp is done with its ring
+        if (t == 0) {
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                sm_m[warp][g + 8 * rr] = st.m[rr];
+                sm_l[warp][g + 8 * rr] = st.l[rr];
+            }
+        }
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr)
+            if (g + 8 * rr < rows) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *reinterpret_cast<float2*>(sm_o + (warp * 16 + g + 8 * rr) * D + 8 * i + 2 * t) = make_float2(st.o[i][2 * rr], st.o[i][2 * rr + 1]);
+            }
+        __syncthreads();
+        const bool whole = steps == seq_steps;
+        const int64_t slot = whole ? 2 * gridDim.x + item : 2 * blockIdx.x + (s0 > begin);
+        for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+            float top = sm_m[0][r];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w][r]);
+            float l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : ex2(sm_m[w][r] - top);
+                const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 16 + r) * D + d);
+                l = fmaf(f, sm_l[w][r], l);
+                acc.x = fmaf(f, x.x, acc.x);
+                acc.y = fmaf(f, x.y, acc.y);
+                acc.z = fmaf(f, x.z, acc.z);
+                acc.w = fmaf(f, x.w, acc.w);
+            }
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            if (d == 0) P.part_lse[slot * 16 + r] = l == 0.f ? -INFINITY : top + log2f(l) - P_BIAS_LOG2;
+            if (whole && !PREFIX) {
+                const int tok = r / P.G, hg = r - tok * P.G;
+                store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + d, acc.x, acc.y, acc.z, acc.w);
+            } else {
+                *reinterpret_cast<float4*>(P.part_o + (slot * 16 + r) * D + d) = acc;
+            }
+        }
+        __syncthreads();                                                 // the rings' memory is free again
+        s0 += steps;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- more rows
+template <int D>
+struct RowsCfg {
+    static constexpr int KT = D == 256 ? 32 : 64, STAGES = 2;
+    static constexpr int Q = 64 * D * 2, TILE = KT * D * 2;
+    static constexpr int SMEM = Q + STAGES * 2 * TILE;
+};
+
+// Grid (tiles * splits, KV_H, B).  PREFIX: rows of the whole batch over the shared prefix (grid z is 1), partial results only.
+template <int D, bool SCORED, bool PREFIX>
+__global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
+    using C = RowsCfg<D>;
+    constexpr int KT = C::KT;
+    pdl_launch_dependents();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float back[64];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int splits = PREFIX ? P.pre_splits : P.splits, tiles = gridDim.x / splits;
+    const int split = blockIdx.x % splits, tile = tiles - 1 - blockIdx.x / splits;      // the rows with the most keys go first
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    const int rows = P.n * P.G, all_rows = PREFIX ? rows * P.B : rows, row0 = tile * 64;
+    const uint32_t q_s = s32(smem), tiles_s = q_s + C::Q;
+    pdl_wait();
+    const int tok0 = row0 / P.G, tok1 = min(P.n, (row0 + 63) / P.G + 1);                // of a chunk: the tokens of these rows
+    Seq sq = {0, 0, 0, P.P};
+    if (!PREFIX) sq = seq_at(P, live_pos(P, b, tile == 0 && kvh == 0 && split == 0 && threadIdx.x == 0), tok0, tok1);
+    const int steps = (sq.keys + KT - 1) / KT, per = (steps + splits - 1) / splits;
+    const int step0 = min(steps, split * per), step1 = min(steps, step0 + per);
+    const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
+    const __half *ck = PREFIX ? P.pk : P.k, *cv = PREFIX ? P.pv : P.v;
+
+    auto request = [&](int step) {
+        if (step < step1) {
+            constexpr int PIECES = D / 8;
+            const uint32_t dst = tiles_s + (step - step0) % C::STAGES * (2 * C::TILE);
+#pragma unroll
+            for (int it = 0; it < KT * PIECES / (WARPS * 32); ++it) {
+                const int i = it * (WARPS * 32) + threadIdx.x, r = i / PIECES, c = i % PIECES, place = step * KT + r;
+                const bool live = place < sq.keys;
+                const int j = live ? sq.row_of(place) : 0;
+                int64_t at = head + static_cast<int64_t>(j) * D;
+                const __half *k = ck, *v = cv;
+                if (!PREFIX && P.nk && live && j >= sq.pos) {
+                    at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
+                    k = P.nk;
+                    v = P.nv;
+                }
+                copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
+                copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
+            }
+        }
+        copy_commit();
+    };
+    request(step0);
+    if (!PREFIX && P.nk && split == 0 && sq.pos >= 0) {
+        // the tokens whose first row is in this tile: their new rows into the cache
+        const int ta = (row0 + P.G - 1) / P.G, tb = min(P.n, (row0 + 63) / P.G + 1);
+        for (int e = threadIdx.x; e < (tb - ta) * (D / 8); e += WARPS * 32) {
+            const int tok = ta + e / (D / 8), c = (e % (D / 8)) * 8;
+            const int64_t src = b * P.n_bs + kvh * P.n_hs + tok * P.n_ts + c, dst = head + static_cast<int64_t>(sq.pos + tok) * D + c;
+            *reinterpret_cast<uint4*>(P.k + dst) = ld_after_wait(P.nk + src);
+            *reinterpret_cast<uint4*>(P.v + dst) = ld_after_wait(P.nv + src);
+        }
+    }
+#pragma unroll 4
+    for (int r = warp; r < 64; r += WARPS) {
+        const int R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
+        const float f = load_q_row<D>(q_s, r, P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, R < all_rows, lane);
+        if (lane == 0) back[r] = f * P.scale_log2;
+    }
+    __syncthreads();
+    const int r_own[2] = {row0 + warp * 16 + g, row0 + warp * 16 + g + 8};
+    const float scale[2] = {back[warp * 16 + g], back[warp * 16 + g + 8]};
+    const int row_pos[2] = {sq.pos + r_own[0] / P.G, sq.pos + r_own[1] / P.G};
+    const int first = sq.pos + (row0 + warp * 16) / P.G, last = sq.pos + (row0 + warp * 16 + 15) / P.G;   // the warp's earliest and latest row
+    const int item = b * P.KV_H + kvh;
+
+    Rows<D> st;
+    st.clear();
+    for (int step = step0; step < step1; ++step) {
+        request(step + 1);
+        copy_wait<1>();
+        __syncthreads();
+        const uint32_t k_tile = tiles_s + (step - step0) % C::STAGES * (2 * C::TILE);
+        float s[KT / 8][4];
+        Rows<D>::template scores<KT / 16>(s, q_s, warp * 16, k_tile, lane);
+        const int place0 = step * KT;
+        bool whole = place0 + KT <= sq.keys;
+        if (!PREFIX && whole) {
+            // every row of the warp sees every key: none lies behind the earliest row, and none before the latest row's window
+            const int j0 = sq.row_of(place0), j1 = sq.row_of(place0 + KT - 1);
+            whole = j1 <= first && (P.window <= 0 || (place0 >= sq.sink && j0 > last - P.window) || (place0 + KT <= sq.sink));
+        }
+        if (whole) {
+#pragma unroll
+            for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= scale[e >> 1];
+        } else {
+#pragma unroll
+            for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int place = place0 + 8 * n + 2 * t + (e & 1);
+                    const bool seen = place < sq.keys && (PREFIX || sees(P, row_pos[e >> 1], sq.row_of(place)));
+                    s[n][e] = seen ? s[n][e] * scale[e >> 1] : -INFINITY;
+                }
+        }
+        if (SCORED) {
+#pragma unroll
+            for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr)
+                    if (r_own[rr] < rows && place0 + 8 * n + 2 * t < sq.keys)
+                        *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + r_own[rr]) * P.pitch + place0 + 8 * n + 2 * t) =
+                            make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
+        }
+        st.template take<KT / 16>(s, k_tile + C::TILE, lane);
+        __syncthreads();                                                 // the tile has been read: its stage may be refilled
+    }
+    copy_wait<0>();
+    st.sum_lanes();
+    const bool direct = !PREFIX && splits == 1 && P.pre_o == nullptr;
+    const int64_t slot = ((static_cast<int64_t>(PREFIX ? 0 : b) * P.KV_H + kvh) * tiles + tile) * splits + split;
+    float* po = PREFIX ? P.pre_o : P.part_o;
+    float* pl = PREFIX ? P.pre_lse : P.part_lse;
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+        if (r_own[rr] >= all_rows) continue;
+        const int r = warp * 16 + g + 8 * rr;
+        const float inv = st.l[rr] == 0.f ? 0.f : 1.0f / st.l[rr];
+        if (t == 0 && (!direct || SCORED)) pl[slot * 64 + r] = st.l[rr] == 0.f ? -INFINITY : st.m[rr] + log2f(st.l[rr]) - P_BIAS_LOG2;
+        if (direct) {
+            const int tok = r_own[rr] / P.G, hg = r_own[rr] - tok * P.G;
+            const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const float x = st.o[i][2 * rr] * inv, y = st.o[i][2 * rr + 1] * inv;
+                if (P.q_dtype == ALLOYB_F16) *reinterpret_cast<__half2*>(static_cast<__half*>(P.out) + at + 8 * i + 2 * t) = __floats2half2_rn(x, y);
+                else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(P.out) + at + 8 * i + 2 * t) = __floats2bfloat162_rn(x, y);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<float2*>(po + (slot * 64 + r) * D + 8 * i + 2 * t) = make_float2(st.o[i][2 * rr] * inv, st.o[i][2 * rr + 1] * inv);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- joining
+constexpr int MERGE_WARPS = 8;
+constexpr int WEIGHT_KEYS = MERGE_WARPS * 32 * 4;                        // keys whose weights a CTA of the merge launch adds up
+
+// Where the partial results of row R of a (sequence, KV head) lie.
+struct Parts {
+    int own, pre;                                                        // how many of the row's own keys, of the prefix
+    int64_t own_at, own_step, own_first, pre_at;                         // indices (slot * rows of a slot + row) of part 0 / their distance
+    bool stored;                                                         // the output is there already
+    __device__ __forceinline__ int64_t own_index(int i) const { return i == 0 ? own_first : own_at + i * own_step; }
+};
+template <bool STREAM>
+__device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
+    Parts p;
+    const bool prefix = P.pre_o != nullptr;
+    const int b = item / P.KV_H, kvh = item - b * P.KV_H;
+    if (STREAM) {
+        const int c0 = P.cum[b], seq_steps = (P.cum[b + 1] - c0) / P.KV_H, total = P.cum[P.B], per = steps_per_cta(total, P.ctas);
+        const int first = c0 + kvh * seq_steps;
+        p.stored = false;
+        if (seq_steps == 0) {
+            p.own = 0;
+        } else {
+            const int a = first / per, z = (first + seq_steps - 1) / per;
+            p.own = z - a + 1;
+            p.own_first = (p.own == 1 ? 2 * static_cast<int64_t>(P.ctas) + item : 2 * static_cast<int64_t>(a) + (first > a * per)) * 16 + R;
+            p.own_at = 2 * static_cast<int64_t>(a) * 16 + R;
+            p.own_step = 2 * 16;
+            p.stored = p.own == 1 && !prefix;
+        }
+    } else {
+        p.own = P.splits;
+        p.own_first = p.own_at = (static_cast<int64_t>(item) * P.tiles + R / 64) * P.splits * 64 + R % 64;
+        p.own_step = 64;
+        p.stored = P.splits == 1 && !prefix;
+    }
+    p.pre = 0;
+    if (prefix) {
+        const int all = b * P.n * P.G + R, tiles = (P.B * P.n * P.G + 63) / 64;
+        p.pre = P.pre_splits;
+        p.pre_at = (static_cast<int64_t>(kvh) * tiles + all / 64) * P.pre_splits * 64 + all % 64;
+    }
+    return p;
+}
+
+// The row's log-sum over all its parts, by a warp.
+__device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int lane) {
+    float top = -INFINITY;
+    for (int i = lane; i < p.own; i += 32) top = fmaxf(top, __ldcg(P.part_lse + p.own_index(i)));
+    for (int i = lane; i < p.pre; i += 32) top = fmaxf(top, __ldcg(P.pre_lse + p.pre_at + i * 64));
+    top = warp_max(top);
+    float l = 0.f;
+    for (int i = lane; i < p.own; i += 32) {
+        const float x = __ldcg(P.part_lse + p.own_index(i));
+        l += x == -INFINITY ? 0.f : ex2(x - top);                        // (a NaN stays one)
+    }
+    for (int i = lane; i < p.pre; i += 32) {
+        const float x = __ldcg(P.pre_lse + p.pre_at + i * 64);
+        l += x == -INFINITY ? 0.f : ex2(x - top);
+    }
+    l = warp_sum(l);
+    return l == 0.f ? -INFINITY : top + log2f(l);
+}
+
+// Grid (rows + CTAs for the weights, sequences * KV heads).
+template <int D, bool STREAM, bool SCORED>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
+    pdl_launch_dependents();
+    __shared__ float sm_o[MERGE_WARPS][D];
+    __shared__ float sm_lse[64];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, item = blockIdx.y, rows = P.n * P.G;
+    const int b = item / P.KV_H, kvh = item - b * P.KV_H;
+    pdl_wait();
+    const int pos = live_pos(P, b, false);
+    if (static_cast<int>(blockIdx.x) < rows) {
+        const int R = blockIdx.x, tok = R / P.G, hg = R - tok * P.G;
+        const Parts p = parts_of<STREAM>(P, item, R);
+        if (p.stored) return;
+        const float lse = row_lse(P, p, lane);
+        float acc[D / 32];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+        constexpr int E = D / 32 < 4 ? D / 32 : 4, PER = D / 32 / E;     // elements of a lane's access, accesses
+        auto add = [&](const float* lses, const float* os, int64_t at) {
+            const float x = __ldcg(lses + at);
+            if (x == -INFINITY) return;                                  // (an empty part's rows are zeros, or were never written)
+            const float w = ex2(x - lse);
+#pragma unroll
+            for (int c = 0; c < PER; ++c) {
+                float v[E];
+                const float* src = os + at * D + (c * 32 + lane) * E;
+                if (E == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src));
+                else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(src));
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[c * E + e] = fmaf(w, v[e], acc[c * E + e]);
+            }
+        };
+        if (pos >= 0) {
+#pragma unroll 4
+            for (int i = warp; i < p.own; i += MERGE_WARPS) add(P.part_lse, P.part_o, p.own_index(i));
+#pragma unroll 4
+            for (int i = warp; i < p.pre; i += MERGE_WARPS) add(P.pre_lse, P.pre_o, p.pre_at + i * 64);
+        }
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+#pragma unroll
+            for (int e = 0; e < E; ++e) sm_o[warp][(c * 32 + lane) * E + e] = acc[c * E + e];
+        __syncthreads();
+        if (threadIdx.x < D / 4) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < MERGE_WARPS; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(&sm_o[w][threadIdx.x * 4]);
+                sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+            }
+            store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + threadIdx.x * 4, sum.x, sum.y, sum.z, sum.w);
+        }
+        return;
+    }
+    if (SCORED) {
+        // weights of WEIGHT_KEYS positions: the rows' probabilities, summed in the rows' order
+        const int first_key = (blockIdx.x - rows) * WEIGHT_KEYS, j0 = first_key + threadIdx.x * 4, len = pos + P.n;
+        if (pos < 0 || first_key >= len) return;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r0 = 0; r0 < rows; r0 += 64) {
+            __syncthreads();
+            for (int r = warp; r < 64 && r0 + r < rows; r += MERGE_WARPS) {
+                const float lse = row_lse(P, parts_of<STREAM>(P, item, r0 + r), lane);
+                if (lane == 0) sm_lse[r] = lse;
+            }
+            __syncthreads();
+            if (j0 < len) {
+                const float* src = P.scores + (static_cast<int64_t>(item) * rows + r0) * P.pitch + j0;
+                const int count = min(64, rows - r0);
+#pragma unroll 8
+                for (int r = 0; r < count; ++r) {
+                    // a key behind the row's last position has no score where its tile was not this row's
+                    const float4 s = __ldcg(reinterpret_cast<const float4*>(src + r * P.pitch));
+                    const int row_pos = pos + (r0 + r) / P.G;
+                    const float lse = sm_lse[r];
+                    const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (j0 + e <= row_pos) sum[e] += ex2(x[e] - lse);
+                }
+            }
+        }
+        float* w = P.weights + static_cast<int64_t>(item) * P.S;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = j0 + e;
+            if (j < pos) w[j] += sum[e];
+            else if (j < len) w[j] = sum[e];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+constexpr int SMS = 148;
+
+// How a call's work is laid out; a function of its sizes alone, so that the workspace's size is one too.
+struct Plan {
+    bool stream;                         // few rows: span_stream_kernel
+    int ctas, splits, tiles, pre_splits, pre_tiles;
+    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;         // byte offsets in the workspace
+    int64_t pitch;
+};
+
+static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+// CTAs that share a tile's keys: rounds of resident CTAs times a CTA's steps (and about three steps' time to begin and to end it).
+static int choose_splits(int64_t ctas, int64_t steps, int resident) {
+    int best = 1;
+    int64_t cost = INT64_MAX;
+    for (int s = 1; s <= 64 && s <= steps; ++s) {
+        const int64_t c = ((ctas * s + resident - 1) / resident) * ((steps + s - 1) / s + 3) * 8 + s;
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
+
+static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int sinks, int P, bool scored) {
+    Plan p = {};
+    const int64_t rows = static_cast<int64_t>(n) * (H / KV_H), items = static_cast<int64_t>(B) * KV_H;
+    const int64_t seen = window > 0 && static_cast<int64_t>(window) + sinks + n < S ? static_cast<int64_t>(window) + sinks + n : S;
+    p.stream = rows <= 16;
+    size_t lse_rows, o_rows;
+    if (p.stream) {
+        const int64_t steps = items * ((seen + STEP - 1) / STEP), most = (steps + MIN_STEPS - 1) / MIN_STEPS;
+        const int resident = SMS * (D == 64 ? 3 : (D == 128 ? 2 : 1));
+        p.ctas = static_cast<int>(most < resident ? most : resident);
+        lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
+        o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
+    } else {
+        const int kt = D == 256 ? 32 : 64;
+        p.tiles = static_cast<int>((rows + 63) / 64);
+        const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + 64 < S ? static_cast<int64_t>(window) + sinks + 64 : S;
+        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, 2 * SMS);
+        lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * 64;
+        o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
+    }
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at = align256(at + bytes);
+        return here;
+    };
+    p.cum = take((static_cast<size_t>(B) + 1) * 4);
+    p.part_lse = take(lse_rows * 4);
+    p.part_o = take(o_rows * D * 4);
+    if (P > 0) {
+        const int kt = D == 256 ? 32 : 64;
+        p.pre_tiles = static_cast<int>((rows * B + 63) / 64);
+        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, 2 * SMS);
+        const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * 64;
+        p.pre_lse = take(r * 4);
+        p.pre_o = take(r * D * 4);
+    }
+    if (scored) {
+        p.pitch = (static_cast<int64_t>(S) + 3) / 4 * 4;
+        p.scores = take(static_cast<size_t>(items) * rows * p.pitch * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+// A kernel with more dynamic shared memory than the default, once per device.
+template <typename K>
+static int allow_smem(K kern, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) {
+            set_cuda_error(e);
+            return ALLOYB_E_CUDA;
+        }
+        done[dev] = true;
+    }
+    return ALLOYB_OK;
+}
+template <typename K>
+static int launch(K kern, dim3 grid, int threads, int smem, bool (&done)[64], cudaStream_t st, const Params& P) {
+    const int rc = allow_smem(kern, smem, done);
+    if (rc != ALLOYB_OK) return rc;
+    const cudaError_t e = launch_pdl(kern, grid, dim3(threads), smem, st, P);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    return ALLOYB_OK;
+}
+
+template <int D, bool SCORED, bool PREFIX>
+static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
+    static bool ready[4][64] = {};
+    const int items = P.B * P.KV_H, rows = P.n * P.G;
+    int rc = ALLOYB_OK;
+    if (PREFIX)
+        rc = launch(span_rows_kernel<D, false, true>, dim3(plan.pre_tiles * plan.pre_splits, P.KV_H, 1), WARPS * 32, RowsCfg<D>::SMEM, ready[0], st, P);
+    if (rc != ALLOYB_OK) return rc;
+    if (plan.stream) rc = launch(span_stream_kernel<D, SCORED, PREFIX>, dim3(plan.ctas), WARPS * 32, StreamCfg<D>::SMEM, ready[1], st, P);
+    else rc = launch(span_rows_kernel<D, SCORED, false>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, RowsCfg<D>::SMEM, ready[2], st, P);
+    if (rc != ALLOYB_OK) return rc;
+    if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
+    const int more = SCORED ? (P.S + WEIGHT_KEYS - 1) / WEIGHT_KEYS : 0;
+    auto merge = plan.stream ? span_merge_kernel<D, true, SCORED> : span_merge_kernel<D, false, SCORED>;
+    const cudaError_t e = launch_pdl(merge, dim3(rows + more, items), dim3(MERGE_WARPS * 32), 0, st, P);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    return check_launch();
+}
+template <bool SCORED, bool PREFIX>
+static int run(const Plan& plan, const Params& P, int D, cudaStream_t st) {
+    switch (D) {
+        case 64: return run_d<64, SCORED, PREFIX>(plan, P, st);
+        case 128: return run_d<128, SCORED, PREFIX>(plan, P, st);
+        default: return run_d<256, SCORED, PREFIX>(plan, P, st);
+    }
+}
+
+static int sizes_ok(int B, int H, int KV_H, int D, int n, int S) {
+    if (B <= 0 || H <= 0 || KV_H <= 0 || H % KV_H || S <= 0 || n < 0 || n > S) return ALLOYB_E_SHAPE;
+    if (D != 64 && D != 128 && D != 256) return ALLOYB_E_SHAPE;
+    if (B > MAX_BATCH || static_cast<int64_t>(B) * KV_H > 65535 || static_cast<int64_t>(n) * (H / KV_H) * B > (1 << 28)) return ALLOYB_E_LIMIT;
+    return ALLOYB_OK;
+}
+
+// The arguments that the three entries share, checked and laid out.  new_k null: the cache holds the rows already.
+static int fill(Params& P, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_ts, int q_dtype, void* k, void* v, const void* nk, const void* nv,
+                int64_t n_bs, int64_t n_hs, int64_t n_ts, const int32_t* pos, int pos_count, void* out, int B, int H, int KV_H, int D, int n, int S,
+                float scale) {
+    if (!q || !k || !v || !pos || !out || (nk != nullptr) != (nv != nullptr)) return ALLOYB_E_NULL;
+    const int rc = sizes_ok(B, H, KV_H, D, n, S);
+    if (rc != ALLOYB_OK) return rc;
+    if (pos_count != 1 && pos_count != B) return ALLOYB_E_SHAPE;
+    if (q_dtype != ALLOYB_F16 && q_dtype != ALLOYB_BF16) return ALLOYB_E_DTYPE;
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(nk) | reinterpret_cast<uintptr_t>(nv)) % 16 ||
+        reinterpret_cast<uintptr_t>(out) % 8 || reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(pos) % 4)
+        return ALLOYB_E_ALIGN;
+    if (nk && ((n_bs | n_hs | n_ts) % 8)) return ALLOYB_E_ALIGN;
+    P = Params{};
+    P.q = q; P.q_bs = q_bs; P.q_hs = q_hs; P.q_ts = q_ts; P.q_dtype = q_dtype;
+    P.q_vec = ((reinterpret_cast<uintptr_t>(q) | (q_bs * 2) | (q_hs * 2) | (q_ts * 2)) & 15) == 0;
+    P.k = static_cast<__half*>(k); P.v = static_cast<__half*>(v); P.S = S;
+    P.nk = static_cast<const __half*>(nk); P.nv = static_cast<const __half*>(nv);
+    P.n_bs = n_bs; P.n_hs = n_hs; P.n_ts = n_ts;
+    P.pos = pos; P.pos_count = pos_count; P.out = out;
+    P.B = B; P.H = H; P.KV_H = KV_H; P.G = H / KV_H; P.n = n;
+    P.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * 1.4426950408889634f;
+    return ALLOYB_OK;
+}
+static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_bytes) {
+    if (!workspace) return ALLOYB_E_NULL;
+    if (reinterpret_cast<uintptr_t>(workspace) % 256) return ALLOYB_E_ALIGN;
+    if (workspace_bytes < plan.bytes) return ALLOYB_E_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    P.cum = reinterpret_cast<int*>(ws + plan.cum);
+    P.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
+    P.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+    P.ctas = plan.ctas; P.splits = plan.splits; P.tiles = plan.tiles; P.pre_splits = plan.pre_splits;
+    if (plan.pre_splits) {
+        P.pre_lse = reinterpret_cast<float*>(ws + plan.pre_lse);
+        P.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
+    }
+    if (plan.pitch) {
+        P.scores = reinterpret_cast<float*>(ws + plan.scores);
+        P.pitch = plan.pitch;
+    }
+    return ALLOYB_OK;
+}
+
+}  // namespace sp
+
+// defined in kv_evict.cu
+cudaError_t kv_evict_status(int* status, int clear);
+
+}  // namespace alloyb
+
+using namespace alloyb;
+
+extern "C" size_t alloyb_attn_span_workspace_bytes(int B, int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks, int prefix_len,
+                                                   int scored) {
+    if (sp::sizes_ok(B, H, KV_H, D, n_tokens, S_max) != ALLOYB_OK || window < 0 || sinks < 0 || prefix_len < 0) return 0;
+    return sp::plan_of(B, H, KV_H, D, n_tokens, S_max, window, sinks, prefix_len, scored != 0).bytes;
+}
+
+extern "C" int alloyb_attn_window(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype, void* k, void* v,
+                                  const void* new_k, const void* new_v, int64_t new_batch_stride, int64_t new_head_stride, int64_t new_tok_stride,
+                                  const int32_t* pos, int pos_count, void* out, int B, int H, int KV_H, int D, int n_tokens, int S_max, int window,
+                                  int sinks, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    sp::Params P;
+    int rc = sp::fill(P, q, q_batch_stride, q_head_stride, q_tok_stride, q_dtype, k, v, new_k, new_v, new_batch_stride, new_head_stride, new_tok_stride,
+                      pos, pos_count, out, B, H, KV_H, D, n_tokens, S_max, scale);
+    if (rc != ALLOYB_OK) return rc;
+    if (window < 1 || sinks < 0) return ALLOYB_E_SHAPE;
+    P.window = window;
+    P.sinks = sinks;
+    const sp::Plan plan = sp::plan_of(B, H, KV_H, D, n_tokens, S_max, window, sinks, 0, false);
+    rc = sp::place(P, plan, workspace, workspace_bytes);
+    if (rc != ALLOYB_OK || n_tokens == 0) return rc;
+    return sp::run<false, false>(plan, P, D, as_stream(stream));
+}
+
+extern "C" int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype,
+                                         const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride, int prefix_len, void* k, void* v,
+                                         const void* new_k, const void* new_v, int64_t new_batch_stride, int64_t new_head_stride, int64_t new_tok_stride,
+                                         const int32_t* pos, int pos_count, void* out, int B, int H, int KV_H, int D, int n_tokens, int S_max,
+                                         float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    sp::Params P;
+    int rc = sp::fill(P, q, q_batch_stride, q_head_stride, q_tok_stride, q_dtype, k, v, new_k, new_v, new_batch_stride, new_head_stride, new_tok_stride,
+                      pos, pos_count, out, B, H, KV_H, D, n_tokens, S_max, scale);
+    if (rc != ALLOYB_OK) return rc;
+    if (prefix_len < 0) return ALLOYB_E_SHAPE;
+    if (prefix_len > 0) {
+        if (!prefix_k || !prefix_v) return ALLOYB_E_NULL;
+        if ((reinterpret_cast<uintptr_t>(prefix_k) | reinterpret_cast<uintptr_t>(prefix_v)) % 16 || prefix_head_stride % 8) return ALLOYB_E_ALIGN;
+    }
+    P.pk = static_cast<const __half*>(prefix_k);
+    P.pv = static_cast<const __half*>(prefix_v);
+    P.p_hs = prefix_head_stride;
+    P.P = prefix_len;
+    const sp::Plan plan = sp::plan_of(B, H, KV_H, D, n_tokens, S_max, 0, 0, prefix_len, false);
+    rc = sp::place(P, plan, workspace, workspace_bytes);
+    if (rc != ALLOYB_OK || n_tokens == 0) return rc;
+    return prefix_len > 0 ? sp::run<false, true>(plan, P, D, as_stream(stream)) : sp::run<false, false>(plan, P, D, as_stream(stream));
+}
+
+extern "C" int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype, void* k, void* v,
+                                  const void* new_k, const void* new_v, int64_t new_batch_stride, int64_t new_head_stride, int64_t new_tok_stride,
+                                  const int32_t* pos, int pos_count, float* weights, void* out, int B, int H, int KV_H, int D, int n_tokens, int S_max,
+                                  float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    sp::Params P;
+    int rc = sp::fill(P, q, q_batch_stride, q_head_stride, q_tok_stride, q_dtype, k, v, new_k, new_v, new_batch_stride, new_head_stride, new_tok_stride,
+                      pos, pos_count, out, B, H, KV_H, D, n_tokens, S_max, scale);
+    if (rc != ALLOYB_OK) return rc;
+    if (!weights) return ALLOYB_E_NULL;
+    if (reinterpret_cast<uintptr_t>(weights) % 4) return ALLOYB_E_ALIGN;
+    P.weights = weights;
+    const sp::Plan plan = sp::plan_of(B, H, KV_H, D, n_tokens, S_max, 0, 0, 0, true);
+    rc = sp::place(P, plan, workspace, workspace_bytes);
+    if (rc != ALLOYB_OK || n_tokens == 0) return rc;
+    return sp::run<true, false>(plan, P, D, as_stream(stream));
+}
+
+extern "C" int alloyb_span_status(int32_t* status_out, int clear) {
+    if (!status_out) return ALLOYB_E_NULL;
+    int positions = 0, lengths = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&positions, sp::g_span_status, sizeof(int));
+    if (e == cudaSuccess && clear && positions) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(sp::g_span_status, &zero, sizeof(int));
+    }
+    if (e == cudaSuccess) e = kv_evict_status(&lengths, clear);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    *status_out = positions | lengths << 1;
+    return ALLOYB_OK;
+}

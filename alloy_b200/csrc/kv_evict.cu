@@ -1,0 +1,289 @@
+// Eviction from an fp16 cache by accumulated attention weight: of every (sequence, KV head)'s rows the first `sinks`, the last `recent` and,
+// of those between, the ones of the largest weight stay (ties: the lower position), in their order, at the front of a cache -- another one
+// or the same.
+//
+// Two launches.  evict_select_kernel, a CTA per (sequence, KV head): the weight that the last row to stay has is found digit by digit
+// (a histogram of eleven, eleven and ten bits of the weights in an order-preserving integer form), then the positions above it, and as many
+// of those equal to it as are wanted, are written in order.  evict_copy_kernel moves the rows.  Bound: HBM, two rows read and written a
+// kept position.
+//
+// In place a row only moves towards the front: a CTA owns a slice of columns of one (sequence, KV head) and walks the positions in order,
+// all of a batch read before any of it is written, so no row is overwritten before it is read.
+#include "common.cuh"
+
+namespace alloyb {
+namespace ev {
+
+static __device__ int g_evict_status = 0;    // sticky: 1 once a length was out of range
+constexpr int THREADS = 1024, WARPS = THREADS / 32;
+constexpr int BINS = 2048;
+
+struct Params {
+    const __half *k, *v;                     // (B, KV_H, S, D)
+    const float* w;                          // (B, KV_H, S)
+    const int32_t* len;
+    int len_count;
+    __half *k_out, *v_out;                   // (B, KV_H, S_out, D)
+    float* w_out;
+    int32_t *kept, *new_len;                 // (B, KV_H, keep), (B,)
+    int B, KV_H, S, S_out, keep, sinks, recent;
+};
+
+__device__ __forceinline__ int length_of(const Params& P, int b, bool tell) {
+    const int n = P.len[P.len_count == 1 ? 0 : b];
+    if (n > P.S || n < 0) {
+        if (tell) atomicOr(&g_evict_status, 1);
+        return 0;
+    }
+    return n;
+}
+// Larger weight, larger integer; the zeros are equal, a NaN is below everything.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    if (x != x) return 0u;
+    const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
+    pdl_launch_dependents();
+    __shared__ int hist[BINS], warp_above[WARPS], warp_equal[WARPS], found[3];
+    const int item = blockIdx.x, b = item / P.KV_H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    const int len = length_of(P, b, threadIdx.x == 0 && item == b * P.KV_H);
+    int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
+    if (threadIdx.x == 0 && item == b * P.KV_H) P.new_len[b] = min(len, P.keep);
+    if (len <= P.keep) {
+        for (int i = threadIdx.x; i < P.keep; i += THREADS) kept[i] = i < len ? i : -1;
+        return;
+    }
+    // len > keep >= sinks + recent: the three parts do not meet
+    const int first = P.sinks, last = len - P.recent, count = last - first, want = P.keep - P.sinks - P.recent;
+    for (int i = threadIdx.x; i < P.sinks; i += THREADS) kept[i] = i;
+    for (int i = threadIdx.x; i < P.recent; i += THREADS) kept[P.keep - P.recent + i] = last + i;
+    if (want == 0) return;
+    const float* w = P.w + static_cast<int64_t>(item) * P.S + first;
+    // the integer form of the want-th largest: `prefix` holds the digits found, `left` how many are wanted of those that share them
+    uint32_t prefix = 0u;
+    int left = want;
+    constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
+#pragma unroll
+    for (int digit = 0; digit < 3; ++digit) {
+        for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
+        __syncthreads();
+        const uint32_t mask = digit == 0 ? 0u : ~0u << (SHIFT[digit] + BITS[digit]);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count; i += THREADS) {
+            const uint32_t u = order_of(__ldcg(w + i));
+            if ((u & mask) == prefix) atomicAdd(&hist[(u >> SHIFT[digit]) & ((1u << BITS[digit]) - 1u)], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // from the top: the bin in which the count reaches `left`; a lane adds up BINS / 32 bins
+            constexpr int PER = BINS / 32;
+            int sum = 0;
+            for (int i = 0; i < PER; ++i) sum += hist[BINS - 1 - lane * PER - i];
+            int before = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += y;
+            }
+            before -= sum;
+            if (before < left && before + sum >= left) {
+                int bin = BINS - 1 - lane * PER;
+                while (before + hist[bin] < left) before += hist[bin--];
+                found[0] = bin;
+                found[1] = left - before;
+            }
+        }
+        __syncthreads();
+        prefix |= static_cast<uint32_t>(found[0]) << SHIFT[digit];
+        left = found[1];
+    }
+    // positions above the limit, and the first `left` of those equal to it: a warp owns a run of positions
+    const int run = (count + WARPS * 32 - 1) / (WARPS * 32) * 32, r0 = min(count, warp * run), r1 = min(count, r0 + run);
+    int above = 0, equal = 0;
+    for (int i0 = r0; i0 < r1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t u = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+        above += __popc(__ballot_sync(0xffffffffu, i < r1 && u > prefix));
+        equal += __popc(__ballot_sync(0xffffffffu, i < r1 && u == prefix));
+    }
+    if (lane == 0) {
+        warp_above[warp] = above;
+        warp_equal[warp] = equal;
+    }
+    __syncthreads();
+    above = equal = 0;
+    for (int k = 0; k < warp; ++k) {
+        above += warp_above[k];
+        equal += warp_equal[k];
+    }
+    for (int i0 = r0; i0 < r1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t u = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+        const uint32_t is_above = __ballot_sync(0xffffffffu, i < r1 && u > prefix), is_equal = __ballot_sync(0xffffffffu, i < r1 && u == prefix);
+        const uint32_t below = (1u << lane) - 1u;
+        const int a = above + __popc(is_above & below), e = equal + __popc(is_equal & below);
+        if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + i;
+        above += __popc(is_above);
+        equal += __popc(is_equal);
+    }
+}
+
+// Another cache: every position on its own.  A warp takes UNROLL rounds of 32 pieces of 16 bytes, K's and V's of a position side by side.
+constexpr int COPY_THREADS = 256, UNROLL = 8;
+template <int D>
+struct CopyCfg {
+    static constexpr int PIECES = 2 * D / 8, ROWS = COPY_THREADS * UNROLL / PIECES;      // positions of a CTA
+};
+template <int D>
+__global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const Params P) {
+    using C = CopyCfg<D>;
+    pdl_launch_dependents();
+    const int item = blockIdx.y, row0 = blockIdx.x * C::ROWS;
+    pdl_wait();
+    const int n = min(length_of(P, item / P.KV_H, false), P.keep);
+    if (row0 >= n) return;
+    const int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
+    const int64_t src = static_cast<int64_t>(item) * P.S, dst = static_cast<int64_t>(item) * P.S_out;
+    uint4 x[UNROLL];
+    int at[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int row = row0 + (u * COPY_THREADS + threadIdx.x) / C::PIECES;
+        at[u] = row < n ? __ldcg(kept + row) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int p = (u * COPY_THREADS + threadIdx.x) % C::PIECES;
+        const __half* from = p < D / 8 ? P.k : P.v;
+        if (at[u] >= 0) x[u] = __ldcg(reinterpret_cast<const uint4*>(from + (src + at[u]) * D) + p % (D / 8));
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const int i = u * COPY_THREADS + threadIdx.x, row = row0 + i / C::PIECES, p = i % C::PIECES;
+        __half* to = p < D / 8 ? P.k_out : P.v_out;
+        if (at[u] >= 0) __stcg(reinterpret_cast<uint4*>(to + (dst + row) * D) + p % (D / 8), x[u]);
+    }
+    for (int i = threadIdx.x; i < C::ROWS && row0 + i < n; i += COPY_THREADS)
+        P.w_out[dst + row0 + i] = __ldcg(P.w + src + __ldcg(kept + row0 + i));
+}
+
+// The same cache: grid (slices of 32 bytes of K's and of V's columns, and one for the weights; sequences * KV heads).
+template <int D>
+__global__ void __launch_bounds__(COPY_THREADS) evict_move_kernel(const Params P) {
+    constexpr int SLICES = D / 16, HALF = COPY_THREADS / 2;
+    pdl_launch_dependents();
+    const int item = blockIdx.y, slice = blockIdx.x;
+    pdl_wait();
+    const int n = min(length_of(P, item / P.KV_H, false), P.keep);
+    const int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
+    const int64_t src = static_cast<int64_t>(item) * P.S, dst = static_cast<int64_t>(item) * P.S_out;
+    if (slice == 2 * SLICES) {
+        for (int i0 = 0; i0 < n; i0 += COPY_THREADS * UNROLL) {
+            float x[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int i = i0 + u * COPY_THREADS + threadIdx.x;
+                if (i < n) x[u] = __ldcg(P.w + src + __ldcg(kept + i));
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int i = i0 + u * COPY_THREADS + threadIdx.x;
+                if (i < n) __stcg(P.w_out + dst + i, x[u]);
+            }
+        }
+        return;
+    }
+    const __half* from = slice < SLICES ? P.k : P.v;
+    __half* to = slice < SLICES ? P.k_out : P.v_out;
+    const int col = slice % SLICES * 16 + (threadIdx.x & 1) * 8;
+    for (int i0 = 0; i0 < n; i0 += HALF * UNROLL) {
+        uint4 x[UNROLL];
+        int at[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = i0 + u * HALF + (threadIdx.x >> 1);
+            at[u] = i < n ? __ldcg(kept + i) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (at[u] >= 0) x[u] = __ldcg(reinterpret_cast<const uint4*>(from + (src + at[u]) * D + col));
+        __syncthreads();                                     // this batch is read before any of it is written
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (at[u] >= 0) __stcg(reinterpret_cast<uint4*>(to + (dst + i0 + u * HALF + (threadIdx.x >> 1)) * D + col), x[u]);
+    }
+}
+
+template <int D>
+static cudaError_t copy(const Params& P, bool in_place, cudaStream_t st) {
+    const int items = P.B * P.KV_H;
+    if (in_place) return launch_pdl(evict_move_kernel<D>, dim3(2 * (D / 16) + 1, items), dim3(COPY_THREADS), 0, st, P);
+    return launch_pdl(evict_copy_kernel<D>, dim3((P.keep + CopyCfg<D>::ROWS - 1) / CopyCfg<D>::ROWS, items), dim3(COPY_THREADS), 0, st, P);
+}
+
+}  // namespace ev
+
+cudaError_t kv_evict_status(int* status, int clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, ev::g_evict_status, sizeof(int));
+    if (e == cudaSuccess && clear && *status) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(ev::g_evict_status, &zero, sizeof(int));
+    }
+    return e;
+}
+
+}  // namespace alloyb
+
+using namespace alloyb;
+
+extern "C" int alloyb_kv_evict(const void* k, const void* v, const float* weights, const int32_t* lengths, int lengths_count, void* k_out, void* v_out,
+                               float* weights_out, int32_t* kept, int32_t* new_lengths, int B, int KV_H, int D, int S, int S_out, int keep, int sinks,
+                               int recent, void* stream) {
+    if (!k || !v || !weights || !lengths || !k_out || !v_out || !weights_out || !kept || !new_lengths) return ALLOYB_E_NULL;
+    if (B <= 0 || KV_H <= 0 || S <= 0 || S_out <= 0 || keep <= 0 || keep > S_out || sinks < 0 || recent < 0) return ALLOYB_E_SHAPE;
+    if (static_cast<int64_t>(sinks) + recent > keep) return ALLOYB_E_SHAPE;
+    if (D != 64 && D != 128 && D != 256) return ALLOYB_E_SHAPE;
+    if (lengths_count != 1 && lengths_count != B) return ALLOYB_E_SHAPE;
+    const int64_t items = static_cast<int64_t>(B) * KV_H;
+    if (items > 65535) return ALLOYB_E_LIMIT;
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
+        return ALLOYB_E_ALIGN;
+    // every output either is its input or lies apart from all three
+    const uintptr_t in[3] = {reinterpret_cast<uintptr_t>(k), reinterpret_cast<uintptr_t>(v), reinterpret_cast<uintptr_t>(weights)};
+    const uintptr_t out[3] = {reinterpret_cast<uintptr_t>(k_out), reinterpret_cast<uintptr_t>(v_out), reinterpret_cast<uintptr_t>(weights_out)};
+    const int64_t row[3] = {D * 2, D * 2, 4};
+    bool in_place = false;
+    for (int o = 0; o < 3; ++o)
+        for (int i = 0; i < 3; ++i) {
+            if (o == i && out[o] == in[i] && S_out == S) {
+                in_place = true;
+                continue;
+            }
+            const uintptr_t out_end = out[o] + items * S_out * row[o], in_end = in[i] + items * S * row[i];
+            if (out[o] < in_end && in[i] < out_end) return ALLOYB_E_SHAPE;
+        }
+    ev::Params P;
+    P.k = static_cast<const __half*>(k); P.v = static_cast<const __half*>(v); P.w = weights;
+    P.len = lengths; P.len_count = lengths_count;
+    P.k_out = static_cast<__half*>(k_out); P.v_out = static_cast<__half*>(v_out); P.w_out = weights_out;
+    P.kept = kept; P.new_len = new_lengths;
+    P.B = B; P.KV_H = KV_H; P.S = S; P.S_out = S_out; P.keep = keep; P.sinks = sinks; P.recent = recent;
+    cudaStream_t st = as_stream(stream);
+    cudaError_t e = launch_pdl(ev::evict_select_kernel, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), 0, st, P);
+    if (e == cudaSuccess) {
+        switch (D) {
+            case 64: e = ev::copy<64>(P, in_place, st); break;
+            case 128: e = ev::copy<128>(P, in_place, st); break;
+            default: e = ev::copy<256>(P, in_place, st); break;
+        }
+    }
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    return check_launch();
+}

@@ -17,14 +17,19 @@ Calls follow what the stream wrote before them, weights included, with the excep
 program that rewrites such packed rows on the stream puts one more operation between the
 write and the call.
 
-Two ops have no reference schema: ``attention_cache_q8_paged`` (decode
-attention over the 16-token-paged pool of 34-byte q8_0 blocks) and
-``linear_residual`` (row-parallel projection with the residual add fused).
+These ops have no reference schema: ``attention_cache_q8_paged`` (decode
+attention over the 16-token-paged pool of 34-byte q8_0 blocks),
+``linear_residual`` (row-parallel projection with the residual add fused), and
+what keeps long contexts affordable over fp16 caches: ``attention_cache_window``
+(sliding window and first rows that stay visible), ``attention_shared_prefix``
+(a batch behind one prefix, read once), ``attention_cache_scored`` (attention
+that keeps its weights) and ``kv_evict`` (the rows of the largest weights stay).
 """
 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from collections.abc import Sequence
 
@@ -93,6 +98,24 @@ lib.define(
 lib.define(
     "linear_residual(Tensor activations, Tensor weight, Tensor? scales, Tensor residual, "
     "str format) -> Tensor"
+)
+
+# Long contexts in a bounded cache (no reference schema; fp16 caches).
+lib.define(
+    "attention_cache_window(Tensor q, Tensor new_k, Tensor new_v, Tensor cache_pos, Tensor(a!) k_cache, "
+    "Tensor(b!) v_cache, int window, int sinks=0, float scale=-1.0, bool write_kv=True) -> Tensor"
+)
+lib.define(
+    "attention_shared_prefix(Tensor q, Tensor new_k, Tensor new_v, Tensor cache_pos, Tensor prefix_k, Tensor prefix_v, "
+    "Tensor(a!) k_cache, Tensor(b!) v_cache, float scale=-1.0, bool write_kv=True) -> Tensor"
+)
+lib.define(
+    "attention_cache_scored(Tensor q, Tensor new_k, Tensor new_v, Tensor cache_pos, Tensor(a!) k_cache, "
+    "Tensor(b!) v_cache, Tensor(c!) weights, float scale=-1.0, bool write_kv=True) -> Tensor"
+)
+lib.define(
+    "kv_evict(Tensor k_cache, Tensor v_cache, Tensor weights, Tensor lengths, Tensor(a!) k_out, Tensor(b!) v_out, "
+    "Tensor(c!) weights_out, int keep, int sinks=0, int recent=0) -> (Tensor, Tensor)"
 )
 
 _FORMATS = {"q4_k": _lib.Q4_K, "q6_k": _lib.Q6_K, "q8_0": _lib.Q8_0}
@@ -716,6 +739,190 @@ def _attention_cache_q8_paged(q, new_k, new_v, seq_pos, page_table, kv_pool, sca
                              _norm_scale(scale, q.shape[-1]), write_kv)
 
 
+# ------------------------------------------------------------------------------- long contexts in a bounded cache
+
+
+def span_status(clear: bool = True) -> int:
+    """Sticky status of the ops below on the current device (bit 0: a position, bit 1: a length was out of range since it was
+    last cleared).  Synchronises the device."""
+    out = C.c_int32(0)
+    check(_lib.load().alloyb_span_status(C.byref(out), 1 if clear else 0), "alloyb_span_status")
+    return int(out.value)
+
+
+@functools.lru_cache(maxsize=1024)
+def _span_workspace_bytes(b, h, kv_h, d, s, s_max, window, sinks, prefix, scored) -> int:
+    return _lib.load().alloyb_attn_span_workspace_bytes(b, h, kv_h, d, s, s_max, window, sinks, prefix, scored)
+
+
+def _on_device(fn):
+    """Run an op on its first tensor's device (the kernels launch on the current one)."""
+    @functools.wraps(fn)
+    def run(t, *args, **kwargs):
+        if t.device.index == _current_device():
+            return fn(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(t, *args, **kwargs)
+    return run
+
+
+def _together(*tensors: torch.Tensor) -> None:
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev:
+            raise ValueError(f"all tensors must be on {dev}, got one on {t.device}")
+
+
+def _strides3(t: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of the first three dimensions (0 where there is nothing to step over)."""
+    return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape[:3]))
+
+
+def _span_pos(pos: torch.Tensor, b: int) -> torch.Tensor:
+    if pos.numel() != 1 and pos.numel() != b:
+        raise ValueError(f"positions must hold one element or one per sequence ({b}), got {pos.numel()}")
+    return _pos_i32(pos.reshape(-1))
+
+
+def _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv):
+    """What the attention ops over spans of an fp16 cache share: checks, and the leading arguments of their C entries."""
+    if q.ndim != 4:
+        raise ValueError(f"attention expects 4D Q (B, H, S, D), got {q.ndim}D")
+    b, h, s, d = q.shape
+    if q.dtype != torch.float16 and q.dtype != torch.bfloat16:
+        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if d not in (64, 128, 256):
+        raise NotImplementedError(f"built for head_dim 64, 128 and 256, got {d}")
+    if new_k.ndim != 4 or new_v.ndim != 4:
+        raise ValueError("new_k / new_v must be 4D (B, KV_H, S, D)")
+    kv_h = new_k.shape[1]
+    if kv_h <= 0 or h <= 0 or h % kv_h:
+        raise ValueError(f"{h} query heads do not group over {kv_h} KV heads")
+    for name, t in (("new_k", new_k), ("new_v", new_v)):
+        if t.dtype != torch.float16:
+            raise TypeError(f"{name} must be float16, got {t.dtype}")
+        if t.shape != (b, kv_h, s, d):
+            raise ValueError(f"{name} must be {(b, kv_h, s, d)}, got {tuple(t.shape)}")
+    for name, t in (("k cache", k_cache), ("v cache", v_cache)):
+        if t.dtype != torch.float16:
+            raise TypeError(f"{name} must be float16, got {t.dtype}")
+        if t.ndim != 4 or t.shape[0] < b or t.shape[1] != kv_h or t.shape[3] != d or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous (>= {b}, {kv_h}, S, {d}), got {tuple(t.shape)}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("K and V caches must have the same shape")
+    if s > k_cache.shape[2]:
+        raise ValueError(f"{s} tokens do not fit a cache of {k_cache.shape[2]} rows")
+    pos = _span_pos(cache_pos, b)
+    _together(q, new_k, new_v, pos, k_cache, v_cache)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if write_kv:
+        ns = _strides3(new_k)
+        if (new_k.stride(3) != 1 or new_v.stride(3) != 1 or ns != _strides3(new_v) or (ns[0] | ns[1] | ns[2]) % 8
+                or (new_k.data_ptr() | new_v.data_ptr()) % 16):
+            new_k, new_v = (t.clone(memory_format=torch.contiguous_format) for t in (new_k, new_v))
+            ns = _strides3(new_k)
+        rows = (new_k.data_ptr(), new_v.data_ptr(), *ns)
+    else:
+        rows = (None, None, 0, 0, 0)
+    out = torch.empty((b, s, h, d), dtype=q.dtype, device=q.device)
+    head = (q.data_ptr(), *_strides3(q), _DTYPES[q.dtype])
+    tail = (*rows, pos.data_ptr(), pos.numel())
+    return out, (b, h, kv_h, d, s, k_cache.shape[2]), head, tail, (q, new_k, new_v, pos)
+
+
+@torch.library.impl(lib, "attention_cache_window", "CUDA")
+@_on_device
+def _attention_cache_window(q, new_k, new_v, cache_pos, k_cache, v_cache, window, sinks=0, scale=-1.0, write_kv=True):
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
+    if out.numel():
+        window, sinks = min(window, size[5]), min(sinks, size[5])
+        ws = torch.empty(_span_workspace_bytes(*size, window, sinks, 0, 0), dtype=torch.uint8, device=out.device)
+        check(_lib.load().alloyb_attn_window(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, window, sinks,
+                                             scale, ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_window")
+    return out.transpose(1, 2)
+
+
+@torch.library.impl(lib, "attention_shared_prefix", "CUDA")
+@_on_device
+def _attention_shared_prefix(q, new_k, new_v, cache_pos, prefix_k, prefix_v, k_cache, v_cache, scale=-1.0, write_kv=True):
+    out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
+    _, _, kv_h, d, _, _ = size
+    for name, t in (("prefix_k", prefix_k), ("prefix_v", prefix_v)):
+        if t.dtype != torch.float16:
+            raise TypeError(f"{name} must be float16, got {t.dtype}")
+        if t.ndim != 3 or t.shape[0] != kv_h or t.shape[2] != d:
+            raise ValueError(f"{name} must be ({kv_h}, P, {d}), got {tuple(t.shape)}")
+    if prefix_k.shape != prefix_v.shape:
+        raise ValueError("prefix_k and prefix_v must have the same shape")
+    _together(q, prefix_k, prefix_v)
+    p = prefix_k.shape[1]
+
+    def dense_rows(t):
+        return t.stride(2) == 1 and (p <= 1 or t.stride(1) == d) and (kv_h == 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0
+
+    if not (dense_rows(prefix_k) and dense_rows(prefix_v) and prefix_k.stride(0) == prefix_v.stride(0)):
+        prefix_k, prefix_v = (t.clone(memory_format=torch.contiguous_format) for t in (prefix_k, prefix_v))
+    if out.numel():
+        ws = torch.empty(_span_workspace_bytes(*size, 0, 0, p, 0), dtype=torch.uint8, device=out.device)
+        check(_lib.load().alloyb_attn_shared_prefix(*head, prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(0) if kv_h > 1 else 0, p,
+                                                    k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, scale,
+                                                    ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_shared_prefix")
+    return out.transpose(1, 2)
+
+
+def _check_weights(name, weights, cache):
+    if weights.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32, got {weights.dtype}")
+    if weights.shape != cache.shape[:3] or not weights.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {tuple(cache.shape[:3])}, got {tuple(weights.shape)}")
+
+
+@torch.library.impl(lib, "attention_cache_scored", "CUDA")
+@_on_device
+def _attention_cache_scored(q, new_k, new_v, cache_pos, k_cache, v_cache, weights, scale=-1.0, write_kv=True):
+    out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
+    _check_weights("weights", weights, k_cache)
+    _together(q, weights)
+    if out.numel():
+        ws = torch.empty(_span_workspace_bytes(*size, 0, 0, 0, 1), dtype=torch.uint8, device=out.device)
+        check(_lib.load().alloyb_attn_scored(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, weights.data_ptr(), out.data_ptr(), *size,
+                                             scale, ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_scored")
+    return out.transpose(1, 2)
+
+
+@torch.library.impl(lib, "kv_evict", "CUDA")
+@_on_device
+def _kv_evict(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out, keep, sinks=0, recent=0):
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_out", k_out), ("v_out", v_out)):
+        if t.dtype != torch.float16:
+            raise TypeError(f"{name} must be float16, got {t.dtype}")
+        if t.ndim != 4 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous (B, KV_H, S, D), got {tuple(t.shape)}")
+    b, kv_h, s, d = k_cache.shape
+    if d not in (64, 128, 256):
+        raise NotImplementedError(f"built for head_dim 64, 128 and 256, got {d}")
+    s_out = k_out.shape[2]
+    if v_cache.shape != k_cache.shape or k_out.shape != (b, kv_h, s_out, d) or v_out.shape != k_out.shape:
+        raise ValueError("K and V must have the same shape, and the outputs theirs but for the number of rows")
+    _check_weights("weights", weights, k_cache)
+    _check_weights("weights_out", weights_out, k_out)
+    if keep < 1 or keep > s_out or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"need sinks + recent <= keep <= rows of the outputs, got {sinks} + {recent}, {keep}, {s_out}")
+    lengths = _span_pos(lengths, b)
+    _together(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out)
+    kept = torch.empty((b, kv_h, keep), dtype=torch.int32, device=k_cache.device)
+    new_lengths = torch.empty((b,), dtype=torch.int32, device=k_cache.device)
+    if k_cache.numel():
+        check(_lib.load().alloyb_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lengths.data_ptr(), lengths.numel(),
+                                          k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), kept.data_ptr(),
+                                          new_lengths.data_ptr(), b, kv_h, d, s, s_out, keep, sinks, recent, _stream()),
+              "alloyb_kv_evict")
+    return kept, new_lengths
+
+
 # ------------------------------------------------------------------------------- Meta kernels
 # Same shape functions as the reference's Meta registrations
 # (packages/alloy-torch/src/alloy_torch/custom_ops.py:285-300, :666-673, :750-785).
@@ -781,6 +988,19 @@ torch.library.impl(lib, "attention_cache_q8", "Meta")(
 torch.library.impl(lib, "attention_cache_q8_paged", "Meta")(
     lambda q, new_k, new_v, seq_pos, page_table, kv_pool, scale=-1.0, write_kv=True:
     torch.empty_like(q))
+
+
+def _span_meta(q, *args, **kwargs):
+    b, h, s, d = q.shape
+    return torch.empty((b, s, h, d), dtype=q.dtype, device=q.device).transpose(1, 2)
+
+
+for _name in ("attention_cache_window", "attention_shared_prefix", "attention_cache_scored"):
+    torch.library.impl(lib, _name, "Meta")(_span_meta)
+torch.library.impl(lib, "kv_evict", "Meta")(
+    lambda k_cache, v_cache, weights, lengths, k_out, v_out, weights_out, keep, sinks=0, recent=0:
+    (torch.empty(tuple(k_cache.shape[:2]) + (keep,), dtype=torch.int32, device=k_cache.device),
+     torch.empty((k_cache.shape[0],), dtype=torch.int32, device=k_cache.device)))
 
 
 # ------------------------------------------------------------------------------- glue

@@ -337,6 +337,62 @@ int alloyb_attn_decode_static(int layout, const void* q, int64_t q_batch_stride,
  * Synchronises the stream.  No counterpart in the reference. */
 int alloyb_attn_static_status(int32_t* status_out, void* stream);
 
+/* ------------------------------------------------------------------ long contexts in a bounded cache (new)
+ * Attention of n_tokens query tokens per sequence over spans of an fp16 cache, and the eviction of its rows.  No counterpart
+ * in the reference, whose sliding windows are ring caches (torch/custom_ops.py:136-150).
+ *
+ * Common to the three attention entries.  k, v: the cache, (B, KV_H, S_max, D) fp16 dense, 16-byte aligned; D is 64, 128
+ * or 256, H any multiple of KV_H.  q: (B, H, n_tokens, D) with strides in elements, f16 or bf16; out: (B, n_tokens, H, D) dense in
+ * q's type, 8-byte aligned.  pos: int32 device (pos_count,), the cache row of each sequence's first token, 1 = shared by all; token
+ * i sits in row pos + i and sees rows up to its own.  A negative pos means a sequence without tokens in this call: its
+ * output is zeros, its cache is left alone.  So is one whose rows do not fit (pos + n_tokens > S_max), which also sets bit 0 of
+ * alloyb_span_status.  new_k / new_v (both or neither): the tokens' rows, fp16 (B, KV_H, n_tokens, D) with strides in elements
+ * (multiples of 8, 16-byte aligned); they are stored at rows pos + i.  NULL: the cache holds them already.
+ * scale <= 0 selects 1/sqrt(D).  Scores, softmax and sums are fp32, the probabilities enter P V as fp16; bf16 queries keep all
+ * their bits.  What rows hold that no token of a sequence sees does not matter.  At most 1024 sequences, B * KV_H <= 65535.
+ * workspace: alloyb_attn_span_workspace_bytes(the same sizes) bytes, 256-byte aligned, undefined before and
+ * after: it needs no clearing and must not be shared by calls that may overlap.  window 0 = none; prefix_len and scored
+ * as in the call.  0 for sizes that the calls refuse. */
+size_t alloyb_attn_span_workspace_bytes(int B, int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks,
+                                        int prefix_len, int scored);
+/* A token in row p sees the rows j <= p with j > p - window (window >= 1) and the first `sinks` rows (j < sinks). */
+int alloyb_attn_window(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype,
+                       void* k, void* v, const void* new_k, const void* new_v, int64_t new_batch_stride,
+                       int64_t new_head_stride, int64_t new_tok_stride, const int32_t* pos, int pos_count, void* out, int B,
+                       int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks, float scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Every token sees all prefix_len rows of prefix_k / prefix_v -- fp16 (KV_H, prefix_len, D), rows dense, heads
+ * prefix_head_stride elements apart (a multiple of 8), 16-byte aligned -- and its own sequence's rows up to its own.  The prefix is read
+ * once for all sequences.  prefix_len may be 0. */
+int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride,
+                              int q_dtype, const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride,
+                              int prefix_len, void* k, void* v, const void* new_k, const void* new_v,
+                              int64_t new_batch_stride, int64_t new_head_stride, int64_t new_tok_stride, const int32_t* pos,
+                              int pos_count, void* out, int B, int H, int KV_H, int D, int n_tokens, int S_max, float scale,
+                              void* workspace, size_t workspace_bytes, void* stream);
+/* Causal attention over the cache that keeps its weights: weights[b, kvh, j] (fp32, (B, KV_H, S_max) dense) grows by the sum over the
+ * KV head's query heads and the call's tokens of the probability that each gives row j.  The entries of the tokens' own rows are
+ * set instead: what stood there belonged to a row that is gone.  Entries behind them are left alone.  The sums are taken in a fixed
+ * order. */
+int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype,
+                       void* k, void* v, const void* new_k, const void* new_v, int64_t new_batch_stride,
+                       int64_t new_head_stride, int64_t new_tok_stride, const int32_t* pos, int pos_count, float* weights,
+                       void* out, int B, int H, int KV_H, int D, int n_tokens, int S_max, float scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Of each (sequence, KV head)'s rows [0, lengths[b]) keeps min(lengths[b], keep): the first `sinks`, the last `recent`, and of
+ * those between the ones of the largest weight (ties: the lowest row; NaN below everything; sinks + recent <= keep).  They go, in
+ * their order, to rows [0, min(lengths[b], keep)) of k_out / v_out / weights_out -- (B, KV_H, S_out, D) and
+ * (B, KV_H, S_out) dense, keep <= S_out; rows behind them are left alone.  Each output may be its input itself (S_out == S); otherwise
+ * it must not overlap an input.  kept: int32 (B, KV_H, keep), the rows they came from, -1 behind the last; new_lengths: int32
+ * (B,).  lengths: int32 device (lengths_count,), 1 = shared.  A length outside [0, S] counts as 0 and sets bit 1 of
+ * alloyb_span_status. */
+int alloyb_kv_evict(const void* k, const void* v, const float* weights, const int32_t* lengths, int lengths_count,
+                    void* k_out, void* v_out, float* weights_out, int32_t* kept, int32_t* new_lengths, int B, int KV_H,
+                    int D, int S, int S_out, int keep, int sinks, int recent, void* stream);
+/* Sticky status of these calls on the current device (bit 0: a position, bit 1: a length was out of range); clear != 0 resets
+ * it.  Synchronises the device. */
+int alloyb_span_status(int32_t* status_out, int clear);
+
 /* ------------------------------------------------------------------ one-launch decode step
  * The whole decode step of a Llama-shape model for ONE token (batch 1, fp16 activations, Q4_K /
  * Q6_K weights, head_dim 128, at most 8 query heads per KV head) as a single persistent launch:
