@@ -37,17 +37,149 @@ constexpr int MIN_STEPS = 2;
 
 __device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max((total + ctas - 1) / ctas, MIN_STEPS); }
 
+// What the warps of a CTA leave for its epilogue.
+struct StreamShared {
+    float back[16], m[WARPS][16], l[WARPS][16];
+};
+
+// `steps` steps of one (sequence, KV head) from step0 on: maxima, sums and outputs of the four warps into shared memory (outputs at sm_o,
+// [warp][16][D], where the rings were).  put(row, place, two scores) takes the scores.  A barrier is behind the last store.
+template <int D, bool SCORED, typename Put>
+__device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, uint8_t* smem, int b, int kvh, const Seq& sq, int step0, int steps, const Put& put) {
+    using C = StreamCfg<D>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rows = P.n * P.G;
+    const uint32_t q_s = s32(smem), ring = q_s + C::Q + warp * (C::SLOTS * C::SLOT);
+    float* sm_o = reinterpret_cast<float*>(smem + C::Q);
+    const int64_t head = (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
+
+    auto request = [&](int i) {                                      // this warp's keys of the segment's i-th step
+        if (i < steps) {
+            constexpr int PIECES = D / 8;
+            const uint32_t dst = ring + i % C::SLOTS * C::SLOT;
+            const int place0 = (step0 + i) * STEP + warp * 16;
+#pragma unroll
+            for (int it = 0; it < PIECES / 2; ++it) {
+                const int r = (it * 32 + lane) / PIECES, c = (it * 32 + lane) % PIECES, place = place0 + r;
+                const bool live = place < sq.keys;
+                const int j = live ? sq.row_of(place) : 0;
+                int64_t at = head + static_cast<int64_t>(j) * D;
+                const __half *k = P.k, *v = P.v;
+                if (P.nk && live && j >= sq.pos) {
+                    at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
+                    k = P.nk;
+                    v = P.nv;
+                }
+                copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
+                copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
+            }
+        }
+        copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::SLOTS - 1; ++i) request(i);
+    // the rows of this (sequence, KV head); rows past the last are zero
+    for (int r = warp; r < 16; r += WARPS) {
+        const int tok = r / P.G, hg = r - tok * P.G;
+        const float f = load_q_row<D>(q_s, r, P.q, b * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, r < rows, lane);
+        if (lane == 0) sh.back[r] = f * P.scale_log2;
+    }
+    __syncthreads();
+    const float scale[2] = {sh.back[g], sh.back[g + 8]};
+    const int row_pos[2] = {sq.pos + g / P.G, sq.pos + (g + 8) / P.G};
+
+    Rows<D> st;
+    st.clear();
+    for (int i = 0; i < steps; ++i) {
+        request(i + C::SLOTS - 1);
+        copy_wait<C::SLOTS - 1>();
+        __syncwarp();
+        const int place0 = (step0 + i) * STEP + warp * 16;
+        const uint32_t k_tile = ring + i % C::SLOTS * C::SLOT;
+        if (place0 < sq.keys) {
+            float s[2][4];
+            Rows<D>::template scores<1>(s, q_s, 0, k_tile, lane);
+            const bool whole = P.n == 1 && place0 + 16 <= sq.keys;   // one token sees every key of its spans
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int place = place0 + 8 * n + 2 * t + (e & 1);
+                    const bool seen = whole || (place < sq.keys && sees(P, row_pos[e >> 1], sq.row_of(place)));
+                    s[n][e] = seen ? s[n][e] * scale[e >> 1] : -INFINITY;
+                }
+            if (SCORED) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int rr = 0; rr < 2; ++rr)
+                        if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < sq.keys)
+                            put(g + 8 * rr, place0 + 8 * n + 2 * t, make_float2(s[n][2 * rr], s[n][2 * rr + 1]));
+            }
+            st.template take<1>(s, k_tile + C::TILE, lane);
+        }
+        __syncwarp();                                                // the slot has been read: the next request may fill it
+    }
+    st.sum_lanes();
+    copy_wait<0>();
+    __syncthreads();                                                 // every warp is done with its ring
+    if (t == 0) {
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            sh.m[warp][g + 8 * rr] = st.m[rr];
+            sh.l[warp][g + 8 * rr] = st.l[rr];
+        }
+    }
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr)
+        if (g + 8 * rr < rows) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<float2*>(sm_o + (warp * 16 + g + 8 * rr) * D + 8 * i + 2 * t) = make_float2(st.o[i][2 * rr], st.o[i][2 * rr + 1]);
+        }
+    __syncthreads();
+}
+// The four warps' results of row r, dims d .. d + 3, joined: outputs relative to `top`, `l` the sum (times 2^P_BIAS_LOG2, both).
+template <int D>
+__device__ __forceinline__ float4 join_warps(const StreamShared& sh, const float* sm_o, int r, int d, float& top, float& l) {
+    top = sh.m[0][r];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sh.m[w][r]);
+    l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        const float f = sh.m[w][r] == -INFINITY && sh.l[w][r] == 0.f ? 0.f : ex2(sh.m[w][r] - top);
+        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 16 + r) * D + d);
+        l = fmaf(f, sh.l[w][r], l);
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+    }
+    return acc;
+}
+// The new rows of one (sequence, KV head) into the cache.
+template <int D>
+__device__ __forceinline__ void append_rows(const Params& P, int b, int kvh, int pos) {
+    for (int e = threadIdx.x; e < P.n * (D / 8); e += WARPS * 32) {
+        const int tok = e / (D / 8), c = (e - tok * (D / 8)) * 8;
+        const int64_t src = b * P.n_bs + kvh * P.n_hs + tok * P.n_ts + c, dst = ((static_cast<int64_t>(b) * P.KV_H + kvh) * P.S + pos + tok) * D + c;
+        *reinterpret_cast<uint4*>(P.k + dst) = ld_after_wait(P.nk + src);
+        *reinterpret_cast<uint4*>(P.v + dst) = ld_after_wait(P.nv + src);
+    }
+}
+
 template <int D, bool SCORED, bool PREFIX>
 __global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P) {
     using C = StreamCfg<D>;
     pdl_launch_dependents();
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int cum[MAX_BATCH + 1], seq_pos[MAX_BATCH];
-    __shared__ float back[16], sm_m[WARPS][16], sm_l[WARPS][16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    __shared__ StreamShared sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows = P.n * P.G;
-    const uint32_t q_s = s32(smem), ring = q_s + C::Q + warp * (C::SLOTS * C::SLOT);
-    float* sm_o = reinterpret_cast<float*>(smem + C::Q);                 // [warp][16][D], in the rings' place between segments
+    const float* sm_o = reinterpret_cast<const float*>(smem + C::Q);
     pdl_wait();
     if (warp == 0) {
         int sum = 0;
@@ -73,20 +205,12 @@ __global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P)
     const int total = cum[P.B], per = steps_per_cta(total, gridDim.x);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= P.B; i += WARPS * 32) P.cum[i] = cum[i];
-    // new rows into the cache
     if (P.nk) {
         for (int i = blockIdx.x; i < P.B * P.KV_H; i += gridDim.x) {
-            const int b = i / P.KV_H, h = i - b * P.KV_H, pos = seq_pos[b];
-            if (pos < 0) continue;
-            for (int e = threadIdx.x; e < P.n * (D / 8); e += WARPS * 32) {
-                const int tok = e / (D / 8), c = (e - tok * (D / 8)) * 8;
-                const int64_t src = b * P.n_bs + h * P.n_hs + tok * P.n_ts + c, dst = (static_cast<int64_t>(i) * P.S + pos + tok) * D + c;
-                *reinterpret_cast<uint4*>(P.k + dst) = ld_after_wait(P.nk + src);
-                *reinterpret_cast<uint4*>(P.v + dst) = ld_after_wait(P.nv + src);
-            }
+            const int b = i / P.KV_H;
+            if (seq_pos[b] >= 0) append_rows<D>(P, b, i - b * P.KV_H, seq_pos[b]);
         }
     }
-
     const int begin = min(total, static_cast<int>(blockIdx.x) * per), end = min(total, begin + per);
     for (int s0 = begin; s0 < end;) {
         int b = 0;
@@ -97,114 +221,15 @@ __global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P)
         }
         const int seq_steps = (cum[b + 1] - cum[b]) / P.KV_H, kvh = (s0 - cum[b]) / seq_steps, item = b * P.KV_H + kvh;
         const int step0 = s0 - cum[b] - kvh * seq_steps, steps = min(seq_steps - step0, end - s0);
-        const Seq sq = seq_at(P, seq_pos[b], 0, P.n);
-        const int64_t head = static_cast<int64_t>(item) * P.S * D;
-
-        auto request = [&](int i) {                                      // this warp's keys of the segment's i-th step
-            if (i < steps) {
-                constexpr int PIECES = D / 8;
-                const uint32_t dst = ring + i % C::SLOTS * C::SLOT;
-                const int place0 = (step0 + i) * STEP + warp * 16;
-#pragma unroll
-                for (int it = 0; it < PIECES / 2; ++it) {
-                    const int r = (it * 32 + lane) / PIECES, c = (it * 32 + lane) % PIECES, place = place0 + r;
-                    const bool live = place < sq.keys;
-                    const int j = live ? sq.row_of(place) : 0;
-                    int64_t at = head + static_cast<int64_t>(j) * D;
-                    const __half *k = P.k, *v = P.v;
-                    if (P.nk && live && j >= sq.pos) {
-                        at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
-                        k = P.nk;
-                        v = P.nv;
-                    }
-                    copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
-                    copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
-                }
-            }
-            copy_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < C::SLOTS - 1; ++i) request(i);
-        // the rows of this (sequence, KV head); rows past the last are zero
-        for (int r = warp; r < 16; r += WARPS) {
-            const int tok = r / P.G, hg = r - tok * P.G;
-            const float f = load_q_row<D>(q_s, r, P.q, b * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, r < rows, lane);
-            if (lane == 0) back[r] = f * P.scale_log2;
-        }
-        __syncthreads();
-        const float scale[2] = {back[g], back[g + 8]};
-        const int row_pos[2] = {sq.pos + g / P.G, sq.pos + (g + 8) / P.G};
-
-        Rows<D> st;
-        st.clear();
-        for (int i = 0; i < steps; ++i) {
-            request(i + C::SLOTS - 1);
-            copy_wait<C::SLOTS - 1>();
-            __syncwarp();
-            const int place0 = (step0 + i) * STEP + warp * 16;
-            const uint32_t k_tile = ring + i % C::SLOTS * C::SLOT;
-            if (place0 < sq.keys) {
-                float s[2][4];
-                Rows<D>::template scores<1>(s, q_s, 0, k_tile, lane);
-                const bool whole = P.n == 1 && place0 + 16 <= sq.keys;   // one token sees every key of its spans
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int place = place0 + 8 * n + 2 * t + (e & 1);
-                        const bool seen = whole || (place < sq.keys && sees(P, row_pos[e >> 1], sq.row_of(place)));
-                        s[n][e] = seen ? s[n][e] * scale[e >> 1] : -INFINITY;
-                    }
-                if (SCORED) {
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int rr = 0; rr < 2; ++rr)
-                            if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < sq.keys)
-                                *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + g + 8 * rr) * P.pitch + place0 + 8 * n + 2 * t) =
-                                    make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
-                }
-                st.template take<1>(s, k_tile + C::TILE, lane);
-            }
-            __syncwarp();                                                // the slot has been read: the next request may fill it
-        }
-        st.sum_lanes();
-        copy_wait<0>();
-        __syncthreads();                                                 // every warp is done with its ring
-        if (t == 0) {
-#pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-                sm_m[warp][g + 8 * rr] = st.m[rr];
-                sm_l[warp][g + 8 * rr] = st.l[rr];
-            }
-        }
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr)
-            if (g + 8 * rr < rows) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<float2*>(sm_o + (warp * 16 + g + 8 * rr) * D + 8 * i + 2 * t) = make_float2(st.o[i][2 * rr], st.o[i][2 * rr + 1]);
-            }
-        __syncthreads();
+        span_segment<D, SCORED>(P, sh, smem, b, kvh, seq_at(P, seq_pos[b], 0, P.n), step0, steps, [&](int r, int place, float2 s) {
+            *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + r) * P.pitch + place) = s;
+        });
         const bool whole = steps == seq_steps;
         const int64_t slot = whole ? 2 * gridDim.x + item : 2 * blockIdx.x + (s0 > begin);
         for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
             const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-            float top = sm_m[0][r];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm_m[w][r]);
-            float l = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = sm_m[w][r] == -INFINITY && sm_l[w][r] == 0.f ? 0.f : ex2(sm_m[w][r] - top);
-                const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * 16 + r) * D + d);
-                l = fmaf(f, sm_l[w][r], l);
-                acc.x = fmaf(f, x.x, acc.x);
-                acc.y = fmaf(f, x.y, acc.y);
-                acc.z = fmaf(f, x.z, acc.z);
-                acc.w = fmaf(f, x.w, acc.w);
-            }
+            float top, l;
+            float4 acc = join_warps<D>(sh, sm_o, r, d, top, l);
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             if (d == 0) P.part_lse[slot * 16 + r] = l == 0.f ? -INFINITY : top + log2f(l) - P_BIAS_LOG2;
@@ -218,6 +243,97 @@ __global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P)
         __syncthreads();                                                 // the rings' memory is free again
         s0 += steps;
     }
+}
+
+// Few (sequence, KV head)s of few keys: a cluster of CTAs each, joined through distributed shared memory, all in one launch.  The scored
+// form keeps its scores in shared memory ([row][the CTA's keys]) and needs nothing of the workspace.
+__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(s32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float peer_f32(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_f32x4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Grid (CTAs of a cluster, B * KV_H); P.splits CTAs a cluster, P.tiles steps at most a CTA.
+template <int D, bool SCORED>
+__global__ void __launch_bounds__(WARPS * 32) span_cluster_kernel(const Params P) {
+    using C = StreamCfg<D>;
+    pdl_launch_dependents();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ StreamShared sh;
+    __shared__ float cta_m[16], cta_l[16], lse[16];
+    const int item = blockIdx.y, b = item / P.KV_H, kvh = item - b * P.KV_H, rank = blockIdx.x, ranks = P.splits;
+    const int rows = P.n * P.G;
+    float* sm_o = reinterpret_cast<float*>(smem + C::Q);
+    float* sm_s = reinterpret_cast<float*>(smem + C::SMEM);              // scored: [row][tiles * STEP]
+    pdl_wait();
+    const int pos = live_pos(P, b, rank == 0 && kvh == 0 && threadIdx.x == 0);
+    if (P.nk && rank == ranks - 1 && pos >= 0) append_rows<D>(P, b, kvh, pos);
+    const Seq sq = seq_at(P, pos, 0, P.n);
+    const int total = (sq.keys + STEP - 1) / STEP, per = (total + ranks - 1) / ranks;
+    const int step0 = min(total, rank * per), steps = min(total, step0 + per) - step0;
+    span_segment<D, SCORED>(P, sh, smem, b, kvh, sq, step0, steps, [&](int r, int place, float2 s) {
+        *reinterpret_cast<float2*>(sm_s + r * (P.tiles * STEP) + place - step0 * STEP) = s;
+    });
+    for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        float top, l;
+        const float4 acc = join_warps<D>(sh, sm_o, r, d, top, l);
+        *reinterpret_cast<float4*>(sm_o + r * D + d) = acc;              // (warp 0's place: nobody else reads it)
+        if (d == 0) {
+            cta_m[r] = top;
+            cta_l[r] = l;
+        }
+    }
+    cluster_barrier();
+    for (int i = rank + threadIdx.x * ranks; i < rows * (D / 4); i += WARPS * 32 * ranks) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        float top = -INFINITY, l = 0.f;
+        for (int k = 0; k < ranks; ++k) top = fmaxf(top, peer_f32(cta_m + r, k));
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < ranks; ++k) {
+            const float m = peer_f32(cta_m + r, k), lk = peer_f32(cta_l + r, k), f = m == -INFINITY && lk == 0.f ? 0.f : ex2(m - top);
+            const float4 x = peer_f32x4(sm_o + r * D + d, k);
+            l = fmaf(f, lk, l);
+            acc = make_float4(fmaf(f, x.x, acc.x), fmaf(f, x.y, acc.y), fmaf(f, x.z, acc.z), fmaf(f, x.w, acc.w));
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int tok = r / P.G, hg = r - tok * P.G;
+        store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    if (SCORED) {
+        if (threadIdx.x < rows) {
+            float top = -INFINITY, l = 0.f;
+            for (int k = 0; k < ranks; ++k) top = fmaxf(top, peer_f32(cta_m + threadIdx.x, k));
+            for (int k = 0; k < ranks; ++k) {
+                const float m = peer_f32(cta_m + threadIdx.x, k), lk = peer_f32(cta_l + threadIdx.x, k);
+                l += m == -INFINITY && lk == 0.f ? 0.f : lk * ex2(m - top);
+            }
+            lse[threadIdx.x] = top + log2f(l) - P_BIAS_LOG2;
+        }
+        __syncthreads();
+        float* w = P.weights + static_cast<int64_t>(item) * P.S;
+        for (int i = threadIdx.x; i < steps * STEP && step0 * STEP + i < sq.keys; i += WARPS * 32) {
+            const int j = step0 * STEP + i;
+            float sum = 0.f;
+            for (int r = 0; r < rows; ++r) sum += ex2(sm_s[r * (P.tiles * STEP) + i] - lse[r]);
+            if (j < pos) sum += w[j];
+            w[j] = sum;
+        }
+    }
+    cluster_barrier();                                                   // nobody's shared memory goes away while a peer still reads it
 }
 
 // ---------------------------------------------------------------------------------------------------------------- more rows
@@ -529,9 +645,14 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
+constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
+// Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
+constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
+
 // How a call's work is laid out; a function of its sizes alone, so that the workspace's size is one too.
 struct Plan {
     bool stream;                         // few rows: span_stream_kernel
+    int cluster, cluster_steps;          // few rows, few steps: span_cluster_kernel with this many CTAs, of this many steps at most
     int ctas, splits, tiles, pre_splits, pre_tiles;
     size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;         // byte offsets in the workspace
     int64_t pitch;
@@ -559,6 +680,17 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     const int64_t seen = window > 0 && static_cast<int64_t>(window) + sinks + n < S ? static_cast<int64_t>(window) + sinks + n : S;
     p.stream = rows <= 16;
     size_t lse_rows, o_rows;
+    if (p.stream && P == 0) {
+        const int64_t most = (seen + STEP - 1) / STEP;
+        int ranks = 1;
+        while (ranks < CLUSTER_MAX && ranks < most) ranks *= 2;
+        const int64_t per = (most + ranks - 1) / ranks;
+        if (items * ranks <= CLUSTER_CTAS && per <= CLUSTER_STEPS && (!scored || rows * per <= cluster_scores(D))) {
+            p.cluster = ranks;
+            p.cluster_steps = static_cast<int>(per);
+            return p;
+        }
+    }
     if (p.stream) {
         const int64_t steps = items * ((seen + STEP - 1) / STEP), most = (steps + MIN_STEPS - 1) / MIN_STEPS;
         const int resident = SMS * (D == 64 ? 3 : (D == 128 ? 2 : 1));
@@ -625,11 +757,54 @@ static int launch(K kern, dim3 grid, int threads, int smem, bool (&done)[64], cu
     return ALLOYB_OK;
 }
 
+template <int D, bool SCORED>
+static int launch_cluster(const Plan& plan, const Params& P, cudaStream_t st) {
+    static bool ready[64] = {}, wide[64] = {};
+    auto kern = span_cluster_kernel<D, SCORED>;
+    const int rows = P.n * P.G, extra = SCORED ? rows * plan.cluster_steps * STEP * 4 : 0;
+    int rc = allow_smem(kern, StreamCfg<D>::SMEM + (SCORED ? cluster_scores(D) * STEP * 4 : 0), ready);
+    if (rc != ALLOYB_OK) return rc;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (plan.cluster > 8 && !wide[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) {
+            set_cuda_error(e);
+            return ALLOYB_E_CUDA;
+        }
+        wide[dev] = true;
+    }
+    Params p = P;
+    p.splits = plan.cluster;
+    p.tiles = plan.cluster_steps;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.cluster, P.B * P.KV_H);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = StreamCfg<D>::SMEM + extra;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = plan.cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    return check_launch();
+}
+
 template <int D, bool SCORED, bool PREFIX>
 static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
     static bool ready[4][64] = {};
     const int items = P.B * P.KV_H, rows = P.n * P.G;
     int rc = ALLOYB_OK;
+    if (!PREFIX && plan.cluster) return launch_cluster<D, SCORED>(plan, P, st);
     if (PREFIX)
         rc = launch(span_rows_kernel<D, false, true>, dim3(plan.pre_tiles * plan.pre_splits, P.KV_H, 1), WARPS * 32, RowsCfg<D>::SMEM, ready[0], st, P);
     if (rc != ALLOYB_OK) return rc;
@@ -687,6 +862,7 @@ static int fill(Params& P, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_
     return ALLOYB_OK;
 }
 static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_bytes) {
+    if (plan.bytes == 0) return ALLOYB_OK;                               // one launch that needs none
     if (!workspace) return ALLOYB_E_NULL;
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return ALLOYB_E_ALIGN;
     if (workspace_bytes < plan.bytes) return ALLOYB_E_WORKSPACE;

@@ -758,16 +758,15 @@ def _span_workspace_bytes(b, h, kv_h, d, s, s_max, window, sinks, prefix, scored
 def _on_device(fn):
     """Run an op on its first tensor's device (the kernels launch on the current one)."""
     @functools.wraps(fn)
-    def run(t, *args, **kwargs):
+    def run(t, *args):
         if t.device.index == _current_device():
-            return fn(t, *args, **kwargs)
+            return fn(t, *args)
         with torch.cuda.device(t.device):
-            return fn(t, *args, **kwargs)
+            return fn(t, *args)
     return run
 
 
-def _together(*tensors: torch.Tensor) -> None:
-    dev = tensors[0].device
+def _together(dev: torch.device, *tensors: torch.Tensor) -> None:
     for t in tensors:
         if t.device != dev:
             raise ValueError(f"all tensors must be on {dev}, got one on {t.device}")
@@ -775,17 +774,22 @@ def _together(*tensors: torch.Tensor) -> None:
 
 def _strides3(t: torch.Tensor) -> tuple[int, int, int]:
     """Strides of the first three dimensions (0 where there is nothing to step over)."""
-    return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape[:3]))
+    a, b, c, _ = t.stride()
+    na, nb, nc, _ = t.shape
+    return a if na > 1 else 0, b if nb > 1 else 0, c if nc > 1 else 0
 
 
 def _span_pos(pos: torch.Tensor, b: int) -> torch.Tensor:
-    if pos.numel() != 1 and pos.numel() != b:
-        raise ValueError(f"positions must hold one element or one per sequence ({b}), got {pos.numel()}")
-    return _pos_i32(pos.reshape(-1))
+    n = pos.numel()
+    if n != 1 and n != b:
+        raise ValueError(f"positions must hold one element or one per sequence ({b}), got {n}")
+    if pos.dtype != torch.int32:
+        pos = pos.to(torch.int32)
+    return pos if pos.is_contiguous() else pos.contiguous()
 
 
-def _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv):
-    """What the attention ops over spans of an fp16 cache share: checks, and the leading arguments of their C entries."""
+def _span_refuse(q, new_k, new_v, k_cache, v_cache) -> None:
+    """Says what is wrong with the arguments of an attention op over spans of an fp16 cache."""
     if q.ndim != 4:
         raise ValueError(f"attention expects 4D Q (B, H, S, D), got {q.ndim}D")
     b, h, s, d = q.shape
@@ -812,23 +816,53 @@ def _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv):
         raise ValueError("K and V caches must have the same shape")
     if s > k_cache.shape[2]:
         raise ValueError(f"{s} tokens do not fit a cache of {k_cache.shape[2]} rows")
+
+
+def _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv):
+    """What the attention ops over spans of an fp16 cache share: checks, the output, and the leading arguments of their C entries.
+    (One decode step's call costs the host about as much as the device: the checks are one expression, taken apart only on failure.)"""
+    f16 = torch.float16
+    dtype = q.dtype
+    row_shape, cache_shape = new_k.shape, k_cache.shape
+    if not (q.ndim == 4 and len(row_shape) == 4 and len(cache_shape) == 4):
+        _span_refuse(q, new_k, new_v, k_cache, v_cache)
+        raise ValueError("K and V caches must be (B, KV_H, S, D)")
+    b, h, s, d = q.shape
+    kv_h = row_shape[1]
+    s_max = cache_shape[2]
+    if not ((dtype == f16 or dtype == torch.bfloat16) and (d == 128 or d == 64 or d == 256) and kv_h > 0 and h > 0 and h % kv_h == 0
+            and new_k.dtype == f16 and new_v.dtype == f16 and k_cache.dtype == f16 and v_cache.dtype == f16
+            and row_shape == (b, kv_h, s, d) and new_v.shape == row_shape and cache_shape[0] >= b and cache_shape[1] == kv_h
+            and cache_shape[3] == d and v_cache.shape == cache_shape and k_cache.is_contiguous() and v_cache.is_contiguous() and s <= s_max):
+        _span_refuse(q, new_k, new_v, k_cache, v_cache)
     pos = _span_pos(cache_pos, b)
-    _together(q, new_k, new_v, pos, k_cache, v_cache)
+    dev = q.device
+    _together(dev, new_k, new_v, pos, k_cache, v_cache)
     if q.stride(3) != 1:
         q = q.contiguous()
     if write_kv:
-        ns = _strides3(new_k)
-        if (new_k.stride(3) != 1 or new_v.stride(3) != 1 or ns != _strides3(new_v) or (ns[0] | ns[1] | ns[2]) % 8
-                or (new_k.data_ptr() | new_v.data_ptr()) % 16):
+        n0, n1, n2 = ns = _strides3(new_k)
+        k_at, v_at = new_k.data_ptr(), new_v.data_ptr()
+        if new_k.stride(3) != 1 or new_v.stride(3) != 1 or ns != _strides3(new_v) or (n0 | n1 | n2) % 8 or (k_at | v_at) % 16:
             new_k, new_v = (t.clone(memory_format=torch.contiguous_format) for t in (new_k, new_v))
-            ns = _strides3(new_k)
-        rows = (new_k.data_ptr(), new_v.data_ptr(), *ns)
+            k_at, v_at = new_k.data_ptr(), new_v.data_ptr()
+            n0, n1, n2 = _strides3(new_k)
     else:
-        rows = (None, None, 0, 0, 0)
-    out = torch.empty((b, s, h, d), dtype=q.dtype, device=q.device)
-    head = (q.data_ptr(), *_strides3(q), _DTYPES[q.dtype])
-    tail = (*rows, pos.data_ptr(), pos.numel())
-    return out, (b, h, kv_h, d, s, k_cache.shape[2]), head, tail, (q, new_k, new_v, pos)
+        k_at = v_at = None
+        n0 = n1 = n2 = 0
+    out = q.new_empty((b, s, h, d))
+    return (out, (b, h, kv_h, d, s, s_max), (q.data_ptr(), *_strides3(q), _DTYPES[dtype]),
+            (k_at, v_at, n0, n1, n2, pos.data_ptr(), pos.numel()), (q, new_k, new_v, pos))
+
+
+def _span_workspace(out, *size):
+    """(address, bytes, the tensor that keeps it) of a call's workspace.  Every call has its own: calls on several streams, and graphs
+    that replay at the same time, share nothing."""
+    n = _span_workspace_bytes(*size)
+    if n == 0:
+        return None, 0, None
+    ws = torch.empty(n, dtype=torch.uint8, device=out.device)
+    return ws.data_ptr(), n, ws
 
 
 @torch.library.impl(lib, "attention_cache_window", "CUDA")
@@ -839,9 +873,11 @@ def _attention_cache_window(q, new_k, new_v, cache_pos, k_cache, v_cache, window
     out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
     if out.numel():
         window, sinks = min(window, size[5]), min(sinks, size[5])
-        ws = torch.empty(_span_workspace_bytes(*size, window, sinks, 0, 0), dtype=torch.uint8, device=out.device)
-        check(_lib.load().alloyb_attn_window(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, window, sinks,
-                                             scale, ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_window")
+        ws, n, _ws = _span_workspace(out, *size, window, sinks, 0, 0)
+        rc = _lib.load().alloyb_attn_window(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, window, sinks, scale, ws, n,
+                                            _stream())
+        if rc:
+            check(rc, "alloyb_attn_window")
     return out.transpose(1, 2)
 
 
@@ -857,7 +893,7 @@ def _attention_shared_prefix(q, new_k, new_v, cache_pos, prefix_k, prefix_v, k_c
             raise ValueError(f"{name} must be ({kv_h}, P, {d}), got {tuple(t.shape)}")
     if prefix_k.shape != prefix_v.shape:
         raise ValueError("prefix_k and prefix_v must have the same shape")
-    _together(q, prefix_k, prefix_v)
+    _together(q.device, prefix_k, prefix_v)
     p = prefix_k.shape[1]
 
     def dense_rows(t):
@@ -866,10 +902,11 @@ def _attention_shared_prefix(q, new_k, new_v, cache_pos, prefix_k, prefix_v, k_c
     if not (dense_rows(prefix_k) and dense_rows(prefix_v) and prefix_k.stride(0) == prefix_v.stride(0)):
         prefix_k, prefix_v = (t.clone(memory_format=torch.contiguous_format) for t in (prefix_k, prefix_v))
     if out.numel():
-        ws = torch.empty(_span_workspace_bytes(*size, 0, 0, p, 0), dtype=torch.uint8, device=out.device)
-        check(_lib.load().alloyb_attn_shared_prefix(*head, prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(0) if kv_h > 1 else 0, p,
-                                                    k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, scale,
-                                                    ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_shared_prefix")
+        ws, n, _ws = _span_workspace(out, *size, 0, 0, p, 0)
+        rc = _lib.load().alloyb_attn_shared_prefix(*head, prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(0) if kv_h > 1 else 0, p,
+                                                   k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, scale, ws, n, _stream())
+        if rc:
+            check(rc, "alloyb_attn_shared_prefix")
     return out.transpose(1, 2)
 
 
@@ -885,11 +922,13 @@ def _check_weights(name, weights, cache):
 def _attention_cache_scored(q, new_k, new_v, cache_pos, k_cache, v_cache, weights, scale=-1.0, write_kv=True):
     out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
     _check_weights("weights", weights, k_cache)
-    _together(q, weights)
+    _together(q.device, weights)
     if out.numel():
-        ws = torch.empty(_span_workspace_bytes(*size, 0, 0, 0, 1), dtype=torch.uint8, device=out.device)
-        check(_lib.load().alloyb_attn_scored(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, weights.data_ptr(), out.data_ptr(), *size,
-                                             scale, ws.data_ptr(), ws.numel(), _stream()), "alloyb_attn_scored")
+        ws, n, _ws = _span_workspace(out, *size, 0, 0, 0, 1)
+        rc = _lib.load().alloyb_attn_scored(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, weights.data_ptr(), out.data_ptr(), *size, scale, ws,
+                                            n, _stream())
+        if rc:
+            check(rc, "alloyb_attn_scored")
     return out.transpose(1, 2)
 
 
@@ -912,7 +951,7 @@ def _kv_evict(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out, kee
     if keep < 1 or keep > s_out or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"need sinks + recent <= keep <= rows of the outputs, got {sinks} + {recent}, {keep}, {s_out}")
     lengths = _span_pos(lengths, b)
-    _together(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out)
+    _together(k_cache.device, v_cache, weights, lengths, k_out, v_out, weights_out)
     kept = torch.empty((b, kv_h, keep), dtype=torch.int32, device=k_cache.device)
     new_lengths = torch.empty((b,), dtype=torch.int32, device=k_cache.device)
     if k_cache.numel():

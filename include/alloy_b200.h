@@ -352,7 +352,7 @@ int alloyb_attn_static_status(int32_t* status_out, void* stream);
  * their bits.  What rows hold that no token of a sequence sees does not matter.  At most 1024 sequences, B * KV_H <= 65535.
  * workspace: alloyb_attn_span_workspace_bytes(the same sizes) bytes, 256-byte aligned, undefined before and
  * after: it needs no clearing and must not be shared by calls that may overlap.  window 0 = none; prefix_len and scored
- * as in the call.  0 for sizes that the calls refuse. */
+ * as in the call.  0 where the call needs none (workspace may be NULL then), and for sizes that the calls refuse. */
 size_t alloyb_attn_span_workspace_bytes(int B, int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks,
                                         int prefix_len, int scored);
 /* A token in row p sees the rows j <= p with j > p - window (window >= 1) and the first `sinks` rows (j < sinks). */

@@ -13,6 +13,8 @@ from tests import _span_ref as R
 OK = 1 << 20
 E_SHAPE, E_ALIGN, E_DTYPE, E_NULL, E_WORKSPACE, E_LIMIT = -1, -2, -3, -4, -6, -8
 
+LONG = dict(s=1 << 20, w=1 << 19)      # sizes that need a workspace
+
 
 def window(q=OK, qd=_lib.F16, k=OK, v=OK, nk=OK, nv=OK, ns=64, pos=OK, pos_n=1, out=OK, b=2, h=4, kv=2, d=64, n=1, s=128, w=8, sinks=0, ws=OK,
            ws_bytes=1 << 40):
@@ -21,11 +23,11 @@ def window(q=OK, qd=_lib.F16, k=OK, v=OK, nk=OK, nv=OK, ns=64, pos=OK, pos_n=1, 
 
 
 @pytest.mark.parametrize("change,code", [
-    (dict(q=None), E_NULL), (dict(k=None), E_NULL), (dict(nk=None), E_NULL), (dict(pos=None), E_NULL), (dict(out=None), E_NULL), (dict(ws=None), E_NULL),
+    (dict(q=None), E_NULL), (dict(k=None), E_NULL), (dict(nk=None), E_NULL), (dict(pos=None), E_NULL), (dict(out=None), E_NULL), (dict(ws=None, **LONG), E_NULL),
     (dict(b=0), E_SHAPE), (dict(h=5), E_SHAPE), (dict(kv=0), E_SHAPE), (dict(d=96), E_SHAPE), (dict(n=129), E_SHAPE), (dict(n=-1), E_SHAPE),
     (dict(s=0), E_SHAPE), (dict(w=0), E_SHAPE), (dict(sinks=-1), E_SHAPE), (dict(pos_n=3), E_SHAPE), (dict(qd=_lib.F32), E_DTYPE),
     (dict(k=OK + 8), E_ALIGN), (dict(v=OK + 2), E_ALIGN), (dict(nk=OK + 8), E_ALIGN), (dict(ns=60), E_ALIGN), (dict(out=OK + 2), E_ALIGN),
-    (dict(ws=OK + 16), E_ALIGN), (dict(ws_bytes=0), E_WORKSPACE), (dict(b=1025, pos_n=1), E_LIMIT), (dict(b=1000, kv=66, h=66), E_LIMIT),
+    (dict(ws=OK + 16, **LONG), E_ALIGN), (dict(ws_bytes=0, **LONG), E_WORKSPACE), (dict(b=1025, pos_n=1), E_LIMIT), (dict(b=1000, kv=66, h=66), E_LIMIT),
 ])
 def test_window_refusals(change, code):
     assert window(**change) == code
@@ -65,11 +67,13 @@ def test_prefix_scored_and_evict_refusals():
 def test_workspace_is_arithmetic_and_covers_what_the_calls_ask():
     size = _lib.load().alloyb_attn_span_workspace_bytes
     assert size(0, 4, 2, 64, 1, 128, 8, 0, 0, 0) == 0 and size(1, 4, 2, 64, 1, 128, -1, 0, 0, 0) == 0
-    plain, with_prefix, with_scores = size(2, 8, 2, 128, 1, 4096, 0, 0, 0, 0), size(2, 8, 2, 128, 1, 4096, 0, 0, 999, 0), size(2, 8, 2, 128, 1, 4096, 0, 0, 0, 1)
-    assert plain % 256 == 0 and with_prefix > plain and with_scores >= plain + 2 * 8 * 4096 * 4
+    long = (2, 8, 2, 128, 1, 1 << 17)
+    plain, with_prefix, with_scores = size(*long, 0, 0, 0, 0), size(*long, 0, 0, 999, 0), size(*long, 0, 0, 0, 1)
+    assert 0 < plain and plain % 256 == 0 and with_prefix > plain and with_scores >= plain + 2 * 8 * (1 << 17) * 4
+    assert size(1, 8, 2, 128, 1, 128, 64, 4, 0, 0) == 0                         # few keys: one launch that needs none
     assert size(64, 64, 8, 128, 1, 1 << 20, 4096, 4, 0, 0) < 64 << 20           # a window's does not grow with the cache
-    for args in ((2, 4, 2, 64, 1, 128, 8, 0), (2, 4, 2, 64, 40, 128, 8, 0)):
-        assert window(n=args[4], ws_bytes=size(*args, 0, 0) - 1) == E_WORKSPACE
+    for n in (1, 40):
+        assert window(n=n, ws_bytes=size(2, 4, 2, 64, n, LONG["s"], LONG["w"], 0, 0, 0) - 1, **LONG) == E_WORKSPACE
 
 
 def test_meta_shapes():
