@@ -20,6 +20,11 @@
 #include "attn_span.cuh"
 
 namespace alloyb {
+
+// defined in attn_span_tc.cu
+int launch_span_tc(const sp::Params& P, int D, bool prefix, dim3 grid, cudaStream_t st);
+cudaError_t span_tc_status(int* status, int clear);
+
 namespace sp {
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
@@ -517,15 +522,15 @@ __device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
         }
     } else {
         p.own = P.splits;
-        p.own_first = p.own_at = (static_cast<int64_t>(item) * P.tiles + R / 64) * P.splits * 64 + R % 64;
-        p.own_step = 64;
+        p.own_first = p.own_at = (static_cast<int64_t>(item) * P.tiles + R / P.tile_rows) * P.splits * P.tile_rows + R % P.tile_rows;
+        p.own_step = P.tile_rows;
         p.stored = P.splits == 1 && !prefix;
     }
     p.pre = 0;
     if (prefix) {
-        const int all = b * P.n * P.G + R, tiles = (P.B * P.n * P.G + 63) / 64;
+        const int all = b * P.n * P.G + R, tr = P.pre_tile_rows, tiles = (P.B * P.n * P.G + tr - 1) / tr;
         p.pre = P.pre_splits;
-        p.pre_at = (static_cast<int64_t>(kvh) * tiles + all / 64) * P.pre_splits * 64 + all % 64;
+        p.pre_at = (static_cast<int64_t>(kvh) * tiles + all / tr) * P.pre_splits * tr + all % tr;
     }
     return p;
 }
@@ -534,7 +539,7 @@ __device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
 __device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int lane) {
     float top = -INFINITY;
     for (int i = lane; i < p.own; i += 32) top = fmaxf(top, __ldcg(P.part_lse + p.own_index(i)));
-    for (int i = lane; i < p.pre; i += 32) top = fmaxf(top, __ldcg(P.pre_lse + p.pre_at + i * 64));
+    for (int i = lane; i < p.pre; i += 32) top = fmaxf(top, __ldcg(P.pre_lse + p.pre_at + i * P.pre_tile_rows));
     top = warp_max(top);
     float l = 0.f;
     for (int i = lane; i < p.own; i += 32) {
@@ -542,7 +547,7 @@ __device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int la
         l += x == -INFINITY ? 0.f : ex2(x - top);                        // (a NaN stays one)
     }
     for (int i = lane; i < p.pre; i += 32) {
-        const float x = __ldcg(P.pre_lse + p.pre_at + i * 64);
+        const float x = __ldcg(P.pre_lse + p.pre_at + i * P.pre_tile_rows);
         l += x == -INFINITY ? 0.f : ex2(x - top);
     }
     l = warp_sum(l);
@@ -586,7 +591,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
 #pragma unroll 4
             for (int i = warp; i < p.own; i += MERGE_WARPS) add(P.part_lse, P.part_o, p.own_index(i));
 #pragma unroll 4
-            for (int i = warp; i < p.pre; i += MERGE_WARPS) add(P.pre_lse, P.pre_o, p.pre_at + i * 64);
+            for (int i = warp; i < p.pre; i += MERGE_WARPS) add(P.pre_lse, P.pre_o, p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows);
         }
 #pragma unroll
         for (int c = 0; c < PER; ++c)
@@ -645,6 +650,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
+constexpr int TC_ROWS = 192;             // rows of a KV head from which they go to the 5th-generation tensor cores
 constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
 // Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
 constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
@@ -653,6 +659,7 @@ constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
 struct Plan {
     bool stream;                         // few rows: span_stream_kernel
     int cluster, cluster_steps;          // few rows, few steps: span_cluster_kernel with this many CTAs, of this many steps at most
+    bool tc, pre_tc;                     // more rows, the own keys / the prefix: span_tc_kernel, not span_rows_kernel
     int ctas, splits, tiles, pre_splits, pre_tiles;
     size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;         // byte offsets in the workspace
     int64_t pitch;
@@ -698,11 +705,12 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
     } else {
-        const int kt = D == 256 ? 32 : 64;
-        p.tiles = static_cast<int>((rows + 63) / 64);
-        const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + 64 < S ? static_cast<int64_t>(window) + sinks + 64 : S;
-        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, 2 * SMS);
-        lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * 64;
+        p.tc = !scored && D <= 128 && rows >= TC_ROWS;
+        const int kt = p.tc ? 128 : (D == 256 ? 32 : 64), tr = p.tc ? 256 : 64;
+        p.tiles = static_cast<int>((rows + tr - 1) / tr);
+        const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + tr < S ? static_cast<int64_t>(window) + sinks + tr : S;
+        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, p.tc ? SMS : 2 * SMS);
+        lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * tr;
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
     size_t at = 0;
@@ -715,10 +723,11 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     p.part_lse = take(lse_rows * 4);
     p.part_o = take(o_rows * D * 4);
     if (P > 0) {
-        const int kt = D == 256 ? 32 : 64;
-        p.pre_tiles = static_cast<int>((rows * B + 63) / 64);
-        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, 2 * SMS);
-        const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * 64;
+        p.pre_tc = D <= 128 && rows * B >= TC_ROWS;
+        const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
+        p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
+        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, p.pre_tc ? SMS : 2 * SMS);
+        const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * tr;
         p.pre_lse = take(r * 4);
         p.pre_o = take(r * D * 4);
     }
@@ -805,10 +814,13 @@ static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
     const int items = P.B * P.KV_H, rows = P.n * P.G;
     int rc = ALLOYB_OK;
     if (!PREFIX && plan.cluster) return launch_cluster<D, SCORED>(plan, P, st);
-    if (PREFIX)
-        rc = launch(span_rows_kernel<D, false, true>, dim3(plan.pre_tiles * plan.pre_splits, P.KV_H, 1), WARPS * 32, RowsCfg<D>::SMEM, ready[0], st, P);
+    if (PREFIX) {
+        const dim3 grid(plan.pre_tiles * plan.pre_splits, P.KV_H, 1);
+        rc = plan.pre_tc ? launch_span_tc(P, D, true, grid, st) : launch(span_rows_kernel<D, false, true>, grid, WARPS * 32, RowsCfg<D>::SMEM, ready[0], st, P);
+    }
     if (rc != ALLOYB_OK) return rc;
-    if (plan.stream) rc = launch(span_stream_kernel<D, SCORED, PREFIX>, dim3(plan.ctas), WARPS * 32, StreamCfg<D>::SMEM, ready[1], st, P);
+    if (plan.tc) rc = launch_span_tc(P, D, false, dim3(plan.tiles * plan.splits, P.KV_H, P.B), st);
+    else if (plan.stream) rc = launch(span_stream_kernel<D, SCORED, PREFIX>, dim3(plan.ctas), WARPS * 32, StreamCfg<D>::SMEM, ready[1], st, P);
     else rc = launch(span_rows_kernel<D, SCORED, false>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, RowsCfg<D>::SMEM, ready[2], st, P);
     if (rc != ALLOYB_OK) return rc;
     if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
@@ -871,6 +883,8 @@ static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_
     P.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
     P.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     P.ctas = plan.ctas; P.splits = plan.splits; P.tiles = plan.tiles; P.pre_splits = plan.pre_splits;
+    P.tile_rows = plan.tc ? 256 : 64;
+    P.pre_tile_rows = plan.pre_tc ? 256 : 64;
     if (plan.pre_splits) {
         P.pre_lse = reinterpret_cast<float*>(ws + plan.pre_lse);
         P.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);
@@ -957,18 +971,19 @@ extern "C" int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t
 
 extern "C" int alloyb_span_status(int32_t* status_out, int clear) {
     if (!status_out) return ALLOYB_E_NULL;
-    int positions = 0, lengths = 0;
+    int positions = 0, more = 0, lengths = 0;
     cudaError_t e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&positions, sp::g_span_status, sizeof(int));
     if (e == cudaSuccess && clear && positions) {
         const int zero = 0;
         e = cudaMemcpyToSymbol(sp::g_span_status, &zero, sizeof(int));
     }
+    if (e == cudaSuccess) e = span_tc_status(&more, clear);
     if (e == cudaSuccess) e = kv_evict_status(&lengths, clear);
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return ALLOYB_E_CUDA;
     }
-    *status_out = positions | lengths << 1;
+    *status_out = positions | more | lengths << 1;
     return ALLOYB_OK;
 }

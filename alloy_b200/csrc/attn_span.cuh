@@ -38,10 +38,10 @@ struct Params {
     float* part_lse;                     // [slot][row], log2
     int* cum;                            // B + 1: steps of the sequences before (written by the stream kernel for the merge)
     int ctas;                            // of the stream kernel
-    int splits, tiles;                   // of the row-tile kernel: CTAs per tile, tiles per (sequence, KV head)
-    float* pre_o;                        // the prefix's partials, [tile, KV head][split][64][D]
+    int splits, tiles, tile_rows;        // of the row-tile kernels: CTAs per tile, tiles per (sequence, KV head), rows of a tile
+    float* pre_o;                        // the prefix's partials, [KV head][tile][split][row][D]
     float* pre_lse;
-    int pre_splits;
+    int pre_splits, pre_tile_rows;
     float* scores;                       // [sequence, KV head][row][pitch], log2 frame, for the weights
     int64_t pitch;
     float* weights;                      // (B, KV_H, S)
@@ -118,8 +118,9 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t i, float a,
 
 // One query row into shared memory as fp16, by a warp (row null: zeros).  bf16 rows are brought under 2^15 by a power of two, so that fp16
 // holds every element of at least 2^-29 of the row's largest exactly; returns the factor that puts the row's scores back.
-template <int D>
-__device__ __forceinline__ float load_q_row(uint32_t dst, int r, const void* q, int64_t at, int dtype, bool vec, bool live, int lane) {
+// place(d): the shared address of element d, d a multiple of D / 32.
+template <int D, typename Place>
+__device__ __forceinline__ float load_q_row_to(const Place& place, const void* q, int64_t at, int dtype, bool vec, bool live, int lane) {
     constexpr int E = D / 32;                                // elements of a lane
     uint16_t h[E];
 #pragma unroll
@@ -155,8 +156,7 @@ __device__ __forceinline__ float load_q_row(uint32_t dst, int r, const void* q, 
 #pragma unroll
         for (int e = 0; e < E; ++e) h[e] = __half_as_ushort(__float2half_rn(x[e]));
     }
-    const int d = lane * E;
-    const uint32_t to = dst + piece_at<D>(r, d >> 3) + (d & 7) * 2;
+    const uint32_t to = place(lane * E);
     if (E == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<uint32_t*>(h)) : "memory");
     if (E == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(reinterpret_cast<uint32_t*>(h)[0]), "r"(reinterpret_cast<uint32_t*>(h)[1]) : "memory");
     if (E == 8)
@@ -164,6 +164,11 @@ __device__ __forceinline__ float load_q_row(uint32_t dst, int r, const void* q, 
                      "r"(reinterpret_cast<uint32_t*>(h)[2]), "r"(reinterpret_cast<uint32_t*>(h)[3])
                      : "memory");
     return back;
+}
+
+template <int D>
+__device__ __forceinline__ float load_q_row(uint32_t dst, int r, const void* q, int64_t at, int dtype, bool vec, bool live, int lane) {
+    return load_q_row_to<D>([&](int d) { return dst + piece_at<D>(r, d >> 3) + (d & 7) * 2; }, q, at, dtype, vec, live, lane);
 }
 
 // A warp's sixteen rows against NK * 16 keys of a tile: running maximum m, sum l (this lane's columns only; times 64) and output o of rows

@@ -1,0 +1,461 @@
+// Attention of many query rows over spans of an fp16 cache on the 5th-generation tensor cores (head_dim 64 and 128): the chunks of a
+// prompt under a window, and a large batch's rows over a shared prefix.  attn_span.cu has the rest, and joins partial results.
+//
+// What bounds it: a tile of 256 rows x 128 keys takes 2048 clocks of the tensor pipe at head_dim 128 (S and P V), and its 32768
+// exponentials 2048 clocks of the SM's sixteen a clock.  So a CTA works on two groups of 128 rows in turns: while one group's scores
+// are in its softmax warps, the tensor pipe has the other's.
+//
+// * Q (two groups), K and V tiles of 128 keys in shared memory, 128-byte swizzle; K and V in two stages by cp.async from wherever a key's
+//   row lies (first rows, window, the new tokens' own rows); places past the last key are zero-filled.  K is a K-major operand, V an MN-major
+//   one, so neither is transposed.
+// * Scores and output accumulators in tensor memory.  A thread owns a row and keeps its 128 scores in registers between the maximum and
+//   the exponentials; P (fp16, rounded once) overwrites the scores and is read from there as the A operand.
+// * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
+// Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
+#include "attn_span.cuh"
+
+namespace alloyb {
+namespace st5 {
+
+using sp::Params;
+using sp::Seq;
+
+constexpr int ROWS = 256, KT = 128, STAGES = 2;
+constexpr int THREADS = 12 * 32;             // warp 1 MMA, warps 0, 2, 3 copies, warps 4-7 and 8-11 the groups' softmax
+constexpr int COPIERS = 96;
+constexpr int HALF = 128 * 128;              // bytes of 128 rows x 64 halves
+constexpr uint32_t SPIN = 1u << 22;
+
+static __device__ int g_tc_error = 0;        // sticky: a bounded wait of this file's kernel ran out
+
+template <int D>
+struct Cfg {
+    static constexpr int TILE = D / 64 * HALF;
+    static constexpr int SMEM = 1024 + 2 * TILE + 2 * STAGES * TILE + 256;
+    static constexpr int COLS = 256;         // tensor-memory columns of a group: 128 of scores, D of outputs
+};
+struct Bars {
+    uint64_t k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
+    uint64_t s_full[2], p_full[2], o_full;
+    uint32_t tmem_base;
+};
+
+using sp::ex2;
+using sp::pack_h2;
+using sp::s32;
+
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(b)), "r"(n)); }
+__device__ __forceinline__ void bar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(b)) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(s32(b)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool bar_wait_slow(uint64_t* b, uint32_t parity) {
+    for (uint32_t i = 0; i < SPIN; ++i) {
+        if (bar_try(b, parity)) return true;
+        if (i > 32) __nanosleep(64);
+    }
+    atomicExch(&g_tc_error, 1);
+    return false;
+}
+__device__ __forceinline__ void bar_wait(bool& ok, uint64_t* b, uint32_t parity) {
+    if (ok && !bar_try(b, parity)) ok = bar_wait_slow(b, parity);
+}
+// Shared-memory operand in the 128-byte swizzle, rows of 128 bytes, groups of eight rows 1024 bytes apart.  K-major: the leading offset is
+// unused; MN-major: it leads to the next 64 elements.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t leading) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | static_cast<uint64_t>((leading >> 4) & 0x3fffu) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+// kind::f16, fp16 operands, fp32 accumulators, M = 128; b_mn: B is MN-major
+__device__ __forceinline__ constexpr uint32_t umma_idesc(int n, bool b_mn) {
+    return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n) >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(b)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+          "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+          "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+                   "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Two fp32 values in one 64-bit register and the two-wide instructions on them.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unf2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// Byte offset of 16-byte piece c of a row in a tile: halves of 64 elements, each in the 128-byte swizzle.
+__device__ __forceinline__ uint32_t piece_at(int row, int c) { return (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4); }
+
+// Grid (tiles * splits, KV_H, B); PREFIX: rows of the whole batch over the shared prefix, grid z 1, partial results only.
+template <int D, bool PREFIX>
+__global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const Params P) {
+    using C = Cfg<D>;
+    constexpr int TILE = C::TILE, PIECES = D / 8;
+    pdl_launch_dependents();
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ float back[ROWS];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t q_s = s32(smem), k_s = q_s + 2 * TILE, v_s = k_s + STAGES * TILE;
+    Bars* bars = reinterpret_cast<Bars*>(smem + 2 * TILE + 2 * STAGES * TILE);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int splits = PREFIX ? P.pre_splits : P.splits, tiles = gridDim.x / splits;
+    const int split = blockIdx.x % splits, tile = tiles - 1 - blockIdx.x / splits;      // the rows with the most keys go first
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    const int rows = P.n * P.G, all_rows = PREFIX ? rows * P.B : rows, row0 = tile * ROWS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            bar_init(&bars->k_full[s], 3);
+            bar_init(&bars->v_full[s], 3);
+            bar_init(&bars->k_empty[s], 1);
+            bar_init(&bars->v_empty[s], 1);
+        }
+        for (int g = 0; g < 2; ++g) {
+            bar_init(&bars->s_full[g], 1);
+            bar_init(&bars->p_full[g], 4);
+        }
+        bar_init(&bars->o_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&bars->tmem_base)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    pdl_wait();
+    const int tok0 = row0 / P.G, tok1 = min(P.n, (row0 + ROWS - 1) / P.G + 1);
+    Seq sq = {0, 0, 0, P.P};
+    if (!PREFIX) sq = sp::seq_at(P, sp::live_pos(P, b, tile == 0 && kvh == 0 && split == 0 && threadIdx.x == 0), tok0, tok1);
+    const int steps = (sq.keys + KT - 1) / KT, per = (steps + splits - 1) / splits;
+    const int step0 = min(steps, split * per), n_tiles = min(steps, step0 + per) - step0;
+    const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
+
+    // ---- Q rows; dead rows are zero
+    for (int r = warp; r < ROWS; r += THREADS / 32) {
+        const int R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
+        const bool live = R < all_rows;
+        const float f = sp::load_q_row_to<D>([&](int d) { return q_s + (r >> 7) * TILE + piece_at(r & 127, d >> 3) + (d & 7) * 2; }, P.q,
+                                             rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, live, lane);
+        if (lane == 0) back[r] = f * P.scale_log2;
+    }
+    fence_async();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    bool ok = true;
+
+    if (warp < 4) {
+        if (warp == 1) {
+            // ------------------------------------------------ MMA issue (one lane)
+            if (lane == 0 && n_tiles > 0) {
+                auto scores = [&](int g, int s) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
+                        umma_ss(tmem + g * C::COLS, umma_desc(q_s + g * TILE + off, 16), umma_desc(k_s + s * TILE + off, 16), umma_idesc(KT, false), kk > 0);
+                    }
+                    umma_commit(&bars->s_full[g]);
+                };
+                bar_wait(ok, &bars->k_full[0], 0);
+                fence_after();
+                if (ok) {
+                    scores(0, 0);
+                    scores(1, 0);
+                    umma_commit(&bars->k_empty[0]);
+                }
+                for (int j = 0; j < n_tiles && ok; ++j) {
+                    const int s = j % STAGES, s1 = (j + 1) % STAGES;
+                    for (int g = 0; g < 2 && ok; ++g) {
+                        bar_wait(ok, &bars->p_full[g], j & 1);
+                        if (g == 0) bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
+                        fence_after();
+                        if (!ok) break;
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; ++kk)
+                            umma_ts(tmem + g * C::COLS + 128, tmem + g * C::COLS + kk * 8, umma_desc(v_s + s * TILE + kk * 2048, HALF), umma_idesc(D, true),
+                                    j > 0 || kk > 0);
+                        if (g == 1) umma_commit(&bars->v_empty[s]);
+                        if (j + 1 < n_tiles) {
+                            if (g == 0) {
+                                bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
+                                fence_after();
+                            }
+                            if (ok) scores(g, s1);
+                            if (ok && g == 1) umma_commit(&bars->k_empty[s1]);
+                        }
+                    }
+                }
+                if (ok) umma_commit(&bars->o_full);
+            }
+            __syncwarp();
+        } else {
+            // ------------------------------------------------ K and V tiles: 96 threads, cp.async
+            const int ct = (warp == 0 ? 0 : warp - 1) * 32 + lane, c = ct % PIECES, r0 = ct / PIECES;
+            const __half *ck = PREFIX ? P.pk : P.k, *cv = PREFIX ? P.pv : P.v;
+            // copy n: K of tile n / 2 (even), V (odd)
+            auto request = [&](int n) {
+                const int j = n >> 1, s = j % STAGES;
+                const bool is_v = n & 1;
+                if (j >= STAGES) bar_wait(ok, is_v ? &bars->v_empty[s] : &bars->k_empty[s], ((j / STAGES) - 1) & 1);
+                const __half *src = (is_v ? cv : ck) + head, *fresh = is_v ? P.nv : P.nk;
+                const uint32_t dst = (is_v ? v_s : k_s) + s * TILE;
+                const int place0 = (step0 + j) * KT;
+                if (ok) {
+                    const int first = PREFIX ? place0 : sq.lo + place0 - sq.sink;       // row of the tile's first place, where it lies in one piece
+                    const bool plain = place0 + KT <= sq.keys && (PREFIX || (place0 >= sq.sink && (!P.nk || first + KT <= sq.pos)));
+                    if (plain) {
+                        const __half* from = src + (static_cast<int64_t>(first) + r0) * D + c * 8;
+                        constexpr int STRIDE = COPIERS / PIECES;
+#pragma unroll 8
+                        for (int r = r0; r < KT; r += STRIDE, from += STRIDE * D) sp::copy16(dst + piece_at(r, c), from, true);
+                    } else {
+                        for (int r = r0; r < KT; r += COPIERS / PIECES) {
+                            const bool live = place0 + r < sq.keys;
+                            const int row = !live ? 0 : (PREFIX ? place0 + r : sq.row_of(place0 + r));
+                            const __half* from = src + static_cast<int64_t>(row) * D;
+                            if (!PREFIX && live && P.nk && row >= sq.pos) from = fresh + b * P.n_bs + kvh * P.n_hs + (row - sq.pos) * P.n_ts;
+                            sp::copy16(dst + piece_at(r, c), from + c * 8, live);
+                        }
+                    }
+                }
+                sp::copy_commit();
+            };
+            auto publish = [&](int n) {                               // copy n has landed: hand it to the tensor pipe's proxy
+                fence_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(n & 1 ? &bars->v_full[(n >> 1) % STAGES] : &bars->k_full[(n >> 1) % STAGES]);
+            };
+            const int n_copies = 2 * n_tiles;
+            for (int n = 0; n < n_copies; ++n) {
+                request(n);
+                if (n >= 2) {
+                    sp::copy_wait<2>();
+                    publish(n - 2);
+                }
+            }
+            sp::copy_wait<0>();
+            for (int n = n_copies >= 2 ? n_copies - 2 : 0; n < n_copies; ++n) publish(n);
+            if (!PREFIX && P.nk && split == 0 && sq.pos >= 0) {
+                // the tokens whose first row is in this tile: their new rows into the cache
+                const int ta = (row0 + P.G - 1) / P.G, tb = min(P.n, (row0 + ROWS - 1) / P.G + 1);
+                for (int tok = ta + r0; tok < tb; tok += COPIERS / PIECES) {
+                    const int64_t from = b * P.n_bs + kvh * P.n_hs + tok * P.n_ts + c * 8, to = head + static_cast<int64_t>(sq.pos + tok) * D + c * 8;
+                    *reinterpret_cast<uint4*>(P.k + to) = ld_after_wait(P.nk + from);
+                    *reinterpret_cast<uint4*>(P.v + to) = ld_after_wait(P.nv + from);
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ softmax: a thread per row
+        const int g = (warp - 4) >> 2, r = g * 128 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * C::COLS;
+        const int R = row0 + r, pos = sq.pos + R / P.G;                       // (of a chunk) last row of the cache that this one may see
+        const int first = sq.pos + (R - lane) / P.G, last = sq.pos + (R - lane + 31) / P.G;
+        const float scale = back[r];
+        float m_run = -INFINITY, l_run = 0.f;                                 // (l times 64, like the accumulators)
+        for (int j = 0; j < n_tiles; ++j) {
+            const int place0 = (step0 + j) * KT;
+            bar_wait(ok, &bars->s_full[g], j & 1);
+            fence_after();
+            float s[KT];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(lanes + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+            wait_ld();
+            bool whole = place0 + KT <= sq.keys;                              // (uniform in the warp)
+            if (!PREFIX && whole) {
+                const int j0 = sq.row_of(place0), j1 = sq.row_of(place0 + KT - 1);
+                whole = j1 <= first && (P.window <= 0 || (place0 >= sq.sink && j0 > last - P.window) || place0 + KT <= sq.sink);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < KT; ++e) {
+                    const int place = place0 + e;
+                    if (!(place < sq.keys && (PREFIX || sp::sees(P, pos, sq.row_of(place))))) s[e] = -INFINITY;
+                }
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < KT; e += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(mx4[k], fmaxf(s[e + k], s[e + 4 + k]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+            const bool grow = mx > m_run + sp::RESCALE_LOG2;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float alpha = grow ? ex2(m_run - mx) : 1.0f;
+                if (grow) m_run = mx;
+                l_run *= alpha;
+                if (j > 0) {                                                  // (these scores came behind the last P V: it is complete)
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        float o[16];
+                        uint32_t w[16];
+                        tmem_ld16(lanes + 128 + c * 16, o);
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
+                        tmem_st16(lanes + 128 + c * 16, w);
+                    }
+                    wait_st();
+                }
+            }
+            const float sub = m_run == -INFINITY ? 0.f : sp::P_BIAS_LOG2 - m_run;
+            const uint64_t scale2 = f2(scale, scale), sub2 = f2(sub, sub);
+            uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x0, x1;
+                    unf2(f2_fma(f2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, sub2), x0, x1);
+                    const float p0 = ex2(x0), p1 = ex2(x1);
+                    sum[e & 1] = f2_add(sum[e & 1], f2(p0, p1));
+                    p[e] = pack_h2(p0, p1);
+                }
+                tmem_st16(lanes + c * 16, p);
+            }
+            float a0, a1, b0, b1;
+            unf2(sum[0], a0, a1);
+            unf2(sum[1], b0, b1);
+            l_run += (a0 + a1) + (b0 + b1);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->p_full[g]);
+        }
+        // ---- normalise and store
+        if (n_tiles > 0) {
+            bar_wait(ok, &bars->o_full, 0);
+            fence_after();
+        }
+        const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+        const bool row_live = ok && R < all_rows, direct = !PREFIX && splits == 1 && P.pre_o == nullptr;
+        const int tok = R / P.G, hg = R - tok * P.G;
+        const int64_t slot = ((static_cast<int64_t>(PREFIX ? 0 : b) * P.KV_H + kvh) * tiles + tile) * splits + split;
+        if (row_live && !direct)
+            (PREFIX ? P.pre_lse : P.part_lse)[slot * ROWS + r] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run) - sp::P_BIAS_LOG2;
+        float* po = (PREFIX ? P.pre_o : P.part_o) + (slot * ROWS + r) * D;
+        const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (n_tiles > 0) {
+                tmem_ld32(lanes + 128 + c * 32, o);
+                wait_ld();
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            }
+            if (row_live) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 x = make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+                    if (direct) sp::store4(P.out, P.q_dtype, at + c * 32 + q * 4, x.x, x.y, x.z, x.w);
+                    else *reinterpret_cast<float4*>(po + c * 32 + q * 4) = x;
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+template <int D, bool PREFIX>
+static int launch(dim3 grid, cudaStream_t st, const Params& P) {
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    cudaError_t e = cudaSuccess;
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(span_tc_kernel<D, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+        if (e == cudaSuccess) ready[dev] = true;
+    }
+    if (e == cudaSuccess) e = launch_pdl(span_tc_kernel<D, PREFIX>, grid, dim3(THREADS), Cfg<D>::SMEM, st, P);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return ALLOYB_E_CUDA;
+    }
+    return ALLOYB_OK;
+}
+
+}  // namespace st5
+
+// Launches of span_tc_kernel for attn_span.cu, which has checked the sizes (D 64 or 128) and laid the workspace out.
+int launch_span_tc(const sp::Params& P, int D, bool prefix, dim3 grid, cudaStream_t st) {
+    if (D == 64) return prefix ? st5::launch<64, true>(grid, st, P) : st5::launch<64, false>(grid, st, P);
+    return prefix ? st5::launch<128, true>(grid, st, P) : st5::launch<128, false>(grid, st, P);
+}
+
+cudaError_t span_tc_status(int* status, int clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, sp::g_span_status, sizeof(int));
+    if (e == cudaSuccess && clear && *status) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(sp::g_span_status, &zero, sizeof(int));
+    }
+    return e;
+}
+
+int span_tc_device_error(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, st5::g_tc_error, sizeof(int)) != cudaSuccess) return 0;
+    if (clear && v) {
+        const int z = 0;
+        cudaMemcpyToSymbol(st5::g_tc_error, &z, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace alloyb

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import alloy_b200  # noqa: F401
-from alloy_b200 import ops
+from alloy_b200 import _lib, ops
 from tests import _span_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -81,6 +81,7 @@ class Case:
 
 def check(out, ref, mag, dtype, what=""):
     got = out.double().cpu()
+    assert _lib.load().alloyb_device_error(1) == 0
     over = (got - ref).abs() - R.out_bound(ref, mag, dtype)
     assert torch.isfinite(got).all() and float(over.max()) <= 0, f"{what}: {float((got - ref).abs().max()):.3e} off, {float(over.max()):.3e} over"
 
@@ -102,6 +103,9 @@ SHAPES = [
     (1, 12, 4, 256, 70, 300, [100], 64, 70, torch.float16, "dense", False),
     (2, 8, 8, 128, 65, 900, [830, 400], 4000, 0, torch.float16, "model", True),    # a window past the cache: plain causal attention
     (1, 40, 2, 128, 9, 333, [300], 50, 20, torch.float16, "model", True),          # twenty heads a group
+    (2, 8, 1, 128, 33, 3000, [2900, 1300], 2000, 129, torch.bfloat16, "packed", True),
+    (1, 24, 1, 64, 300, 900, [599], 128, 1, torch.float16, "dense", True),
+    (2, 4, 1, 128, 200, 400, [0, 200], 1, 0, torch.float16, "model", False),
 ]
 
 
@@ -167,6 +171,10 @@ def test_bf16_queries_beyond_fp16():
     (2, 16, 2, 256, 1, 300, [250, 3], 77, torch.float16, "model", True),
     (2, 8, 1, 256, 5, 64, [50, 3], 700, torch.bfloat16, "model", True),            # 40 rows of a sequence
     (5, 14, 2, 64, 11, 64, [50, 3, 0, -1, 53], 64, torch.float16, "model", True),
+    (70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], 300, torch.float16, "model", True),      # 280 rows a KV head: tensor memory
+    (33, 16, 2, 64, 2, 24, [i % 23 - 1 for i in range(33)], 1025, torch.bfloat16, "packed", True),
+    (24, 8, 1, 128, 1, 16, [3], 1, torch.float16, "model", True),
+    (2, 8, 1, 128, 60, 80, [20, -1], 130, torch.float16, "model", True),                         # the own keys there too
 ])
 def test_shared_prefix(b, h, kv_h, d, n, s, pos, p, dtype, layout, write):
     c = Case(b, h, kv_h, d, n, s, pos, dtype, layout=layout, prefix=max(p, 1))
