@@ -940,6 +940,7 @@ extern "C" int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, 
     if (prefix_len < 0) return ALLOYB_E_SHAPE;
     if (prefix_len > 0) {
         if (!prefix_k || !prefix_v) return ALLOYB_E_NULL;
+        if (KV_H > 1 && prefix_head_stride < static_cast<int64_t>(prefix_len) * D) return ALLOYB_E_SHAPE;
         if ((reinterpret_cast<uintptr_t>(prefix_k) | reinterpret_cast<uintptr_t>(prefix_v)) % 16 || prefix_head_stride % 8) return ALLOYB_E_ALIGN;
     }
     P.pk = static_cast<const __half*>(prefix_k);

@@ -5,13 +5,16 @@
 // exponentials 2048 clocks of the SM's sixteen a clock.  So a CTA works on two groups of 128 rows in turns: while one group's scores
 // are in its softmax warps, the tensor pipe has the other's.
 //
-// * Q (two groups), K and V tiles of 128 keys in shared memory, 128-byte swizzle; K and V in two stages by cp.async from wherever a key's
-//   row lies (first rows, window, the new tokens' own rows); places past the last key are zero-filled.  K is a K-major operand, V an MN-major
-//   one, so neither is transposed.
+// * Q (two groups), K and V tiles of 128 keys in shared memory, 128-byte swizzle, K and V in two stages by TMA.  Tiles that are not 128 rows
+//   in one piece (the first rows, the end of a sequence) come in by cp.async, places past the last key zero-filled: what a cache holds there
+//   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.  (All tiles by cp.async, and the new
+//   tokens' rows from their own tensors: 314 us for 2048 tokens behind 6000 under a window of 4096, 32/8 heads, head_dim 128.)
 // * Scores and output accumulators in tensor memory.  A thread owns a row and keeps its 128 scores in registers between the maximum and
 //   the exponentials; P (fp16, rounded once) overwrites the scores and is read from there as the A operand.
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
+#include <cuda.h>
+
 #include "attn_span.cuh"
 
 namespace alloyb {
@@ -33,6 +36,10 @@ struct Cfg {
     static constexpr int TILE = D / 64 * HALF;
     static constexpr int SMEM = 1024 + 2 * TILE + 2 * STAGES * TILE + 256;
     static constexpr int COLS = 256;         // tensor-memory columns of a group: 128 of scores, D of outputs
+};
+struct alignas(64) Args {
+    CUtensorMap k, v;                        // (D, rows, heads), boxes of 64 elements x 128 rows, 128-byte swizzle
+    Params p;
 };
 struct Bars {
     uint64_t k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
@@ -135,12 +142,26 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+                 "r"(s32(bar)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Byte offset of 16-byte piece c of a row in a tile: halves of 64 elements, each in the 128-byte swizzle.
 __device__ __forceinline__ uint32_t piece_at(int row, int c) { return (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4); }
 
 // Grid (tiles * splits, KV_H, B); PREFIX: rows of the whole batch over the shared prefix, grid z 1, partial results only.
 template <int D, bool PREFIX>
-__global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const Params P) {
+__global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_constant__ Args A) {
+    const Params& P = A.p;
     using C = Cfg<D>;
     constexpr int TILE = C::TILE, PIECES = D / 8;
     pdl_launch_dependents();
@@ -241,59 +262,39 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const Params P) {
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------ K and V tiles: 96 threads, cp.async
+            // ------------------------------------------------ K and V tiles
             const int ct = (warp == 0 ? 0 : warp - 1) * 32 + lane, c = ct % PIECES, r0 = ct / PIECES;
-            const __half *ck = PREFIX ? P.pk : P.k, *cv = PREFIX ? P.pv : P.v;
-            // copy n: K of tile n / 2 (even), V (odd)
-            auto request = [&](int n) {
+            const int z = PREFIX ? kvh : b * P.KV_H + kvh;
+            for (int n = 0; n < 2 * n_tiles; ++n) {                   // K of tile n / 2 (even), V (odd)
                 const int j = n >> 1, s = j % STAGES;
                 const bool is_v = n & 1;
+                uint64_t* full = is_v ? &bars->v_full[s] : &bars->k_full[s];
                 if (j >= STAGES) bar_wait(ok, is_v ? &bars->v_empty[s] : &bars->k_empty[s], ((j / STAGES) - 1) & 1);
-                const __half *src = (is_v ? cv : ck) + head, *fresh = is_v ? P.nv : P.nk;
                 const uint32_t dst = (is_v ? v_s : k_s) + s * TILE;
                 const int place0 = (step0 + j) * KT;
-                if (ok) {
-                    const int first = PREFIX ? place0 : sq.lo + place0 - sq.sink;       // row of the tile's first place, where it lies in one piece
-                    const bool plain = place0 + KT <= sq.keys && (PREFIX || (place0 >= sq.sink && (!P.nk || first + KT <= sq.pos)));
-                    if (plain) {
-                        const __half* from = src + (static_cast<int64_t>(first) + r0) * D + c * 8;
-                        constexpr int STRIDE = COPIERS / PIECES;
-#pragma unroll 8
-                        for (int r = r0; r < KT; r += STRIDE, from += STRIDE * D) sp::copy16(dst + piece_at(r, c), from, true);
-                    } else {
-                        for (int r = r0; r < KT; r += COPIERS / PIECES) {
-                            const bool live = place0 + r < sq.keys;
-                            const int row = !live ? 0 : (PREFIX ? place0 + r : sq.row_of(place0 + r));
-                            const __half* from = src + static_cast<int64_t>(row) * D;
-                            if (!PREFIX && live && P.nk && row >= sq.pos) from = fresh + b * P.n_bs + kvh * P.n_hs + (row - sq.pos) * P.n_ts;
-                            sp::copy16(dst + piece_at(r, c), from + c * 8, live);
+                // (rows past the prefix's last are outside the map: TMA fills them with zeros)
+                if (PREFIX || (place0 >= sq.sink && place0 + KT <= sq.keys)) {
+                    if (lane == 0) {
+                        if (warp == 0 && ok) {
+                            bar_expect(full, TILE);
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h) tma_3d(dst + h * HALF, is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z, full);
+                        } else {
+                            bar_arrive(full);
                         }
                     }
-                }
-                sp::copy_commit();
-            };
-            auto publish = [&](int n) {                               // copy n has landed: hand it to the tensor pipe's proxy
-                fence_async();
-                __syncwarp();
-                if (lane == 0) bar_arrive(n & 1 ? &bars->v_full[(n >> 1) % STAGES] : &bars->k_full[(n >> 1) % STAGES]);
-            };
-            const int n_copies = 2 * n_tiles;
-            for (int n = 0; n < n_copies; ++n) {
-                request(n);
-                if (n >= 2) {
-                    sp::copy_wait<2>();
-                    publish(n - 2);
-                }
-            }
-            sp::copy_wait<0>();
-            for (int n = n_copies >= 2 ? n_copies - 2 : 0; n < n_copies; ++n) publish(n);
-            if (!PREFIX && P.nk && split == 0 && sq.pos >= 0) {
-                // the tokens whose first row is in this tile: their new rows into the cache
-                const int ta = (row0 + P.G - 1) / P.G, tb = min(P.n, (row0 + ROWS - 1) / P.G + 1);
-                for (int tok = ta + r0; tok < tb; tok += COPIERS / PIECES) {
-                    const int64_t from = b * P.n_bs + kvh * P.n_hs + tok * P.n_ts + c * 8, to = head + static_cast<int64_t>(sq.pos + tok) * D + c * 8;
-                    *reinterpret_cast<uint4*>(P.k + to) = ld_after_wait(P.nk + from);
-                    *reinterpret_cast<uint4*>(P.v + to) = ld_after_wait(P.nv + from);
+                } else {
+                    const __half* src = (is_v ? P.v : P.k) + head + c * 8;
+                    if (ok)
+                        for (int r = r0; r < KT; r += COPIERS / PIECES) {
+                            const bool live = place0 + r < sq.keys;
+                            sp::copy16(dst + piece_at(r, c), src + static_cast<int64_t>(live ? sq.row_of(place0 + r) : 0) * D, live);
+                        }
+                    sp::copy_commit();
+                    sp::copy_wait<0>();
+                    fence_async();                                    // to the tensor pipe's proxy
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(full);
                 }
             }
         }
@@ -329,8 +330,8 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const Params P) {
 #pragma unroll
             for (int e = 0; e < KT; e += 8)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx4[k] = fmaxf(mx4[k], fmaxf(s[e + k], s[e + 4 + k]));
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+                for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], s[e + k], s[e + 4 + k]);
+            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
             const bool grow = mx > m_run + sp::RESCALE_LOG2;
             if (__any_sync(0xffffffffu, grow)) {
                 const float alpha = grow ? ex2(m_run - mx) : 1.0f;
@@ -413,17 +414,60 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const Params P) {
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
+// The new tokens' rows into the cache, ahead of a kernel that reads them there.
+template <int D>
+__global__ void __launch_bounds__(256) span_append_kernel(const Params P) {
+    pdl_launch_dependents();
+    const int i = blockIdx.x * 256 + threadIdx.x, tok = i / (D / 8), c = i % (D / 8) * 8, kvh = blockIdx.y, b = blockIdx.z;
+    pdl_wait();
+    if (tok >= P.n) return;
+    const int pos = sp::live_pos(P, b, false);
+    if (pos < 0) return;
+    const int64_t from = b * P.n_bs + kvh * P.n_hs + tok * P.n_ts + c, to = ((static_cast<int64_t>(b) * P.KV_H + kvh) * P.S + pos + tok) * D + c;
+    *reinterpret_cast<uint4*>(P.k + to) = ld_after_wait(P.nk + from);
+    *reinterpret_cast<uint4*>(P.v + to) = ld_after_wait(P.nv + from);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+static bool map_rows(CUtensorMap* m, const __half* base, int D, int64_t rows, int64_t heads, int64_t head_stride) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads)};
+    const cuuint64_t pitch[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(head_stride) * 2};
+    const cuuint32_t box[3] = {64, KT, 1}, step[3] = {1, 1, 1};
+    return encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool PREFIX>
 static int launch(dim3 grid, cudaStream_t st, const Params& P) {
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    cudaError_t e = cudaSuccess;
-    if (!ready[dev]) {
+    cudaError_t e = encode_fn() ? cudaSuccess : cudaErrorNotSupported;
+    if (e == cudaSuccess && !ready[dev]) {
         e = cudaFuncSetAttribute(span_tc_kernel<D, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
         if (e == cudaSuccess) ready[dev] = true;
     }
-    if (e == cudaSuccess) e = launch_pdl(span_tc_kernel<D, PREFIX>, grid, dim3(THREADS), Cfg<D>::SMEM, st, P);
+    Args a;
+    a.p = P;
+    if (e == cudaSuccess) {
+        const bool mapped = PREFIX ? map_rows(&a.k, P.pk, D, P.P, P.KV_H, P.KV_H > 1 ? P.p_hs : static_cast<int64_t>(P.P) * D) &&
+                                         map_rows(&a.v, P.pv, D, P.P, P.KV_H, P.KV_H > 1 ? P.p_hs : static_cast<int64_t>(P.P) * D)
+                                   : map_rows(&a.k, P.k, D, P.S, static_cast<int64_t>(P.B) * P.KV_H, static_cast<int64_t>(P.S) * D) &&
+                                         map_rows(&a.v, P.v, D, P.S, static_cast<int64_t>(P.B) * P.KV_H, static_cast<int64_t>(P.S) * D);
+        if (!mapped) e = cudaErrorInvalidValue;
+    }
+    if (e == cudaSuccess && !PREFIX && P.nk) e = launch_pdl(span_append_kernel<D>, dim3((P.n * (D / 8) + 255) / 256, P.KV_H, P.B), dim3(256), 0, st, P);
+    if (e == cudaSuccess) e = launch_pdl(span_tc_kernel<D, PREFIX>, grid, dim3(THREADS), Cfg<D>::SMEM, st, a);
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return ALLOYB_E_CUDA;

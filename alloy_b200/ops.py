@@ -897,7 +897,7 @@ def _attention_shared_prefix(q, new_k, new_v, cache_pos, prefix_k, prefix_v, k_c
     p = prefix_k.shape[1]
 
     def dense_rows(t):
-        return t.stride(2) == 1 and (p <= 1 or t.stride(1) == d) and (kv_h == 1 or t.stride(0) % 8 == 0) and t.data_ptr() % 16 == 0
+        return t.stride(2) == 1 and (p <= 1 or t.stride(1) == d) and (kv_h == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= p * d)) and t.data_ptr() % 16 == 0
 
     if not (dense_rows(prefix_k) and dense_rows(prefix_v) and prefix_k.stride(0) == prefix_v.stride(0)):
         prefix_k, prefix_v = (t.clone(memory_format=torch.contiguous_format) for t in (prefix_k, prefix_v))

@@ -362,7 +362,7 @@ int alloyb_attn_window(const void* q, int64_t q_batch_stride, int64_t q_head_str
                        int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks, float scale, void* workspace,
                        size_t workspace_bytes, void* stream);
 /* Every token sees all prefix_len rows of prefix_k / prefix_v -- fp16 (KV_H, prefix_len, D), rows dense, heads
- * prefix_head_stride elements apart (a multiple of 8), 16-byte aligned -- and its own sequence's rows up to its own.  The prefix is read
+ * prefix_head_stride elements apart (a multiple of 8, at least prefix_len * D), 16-byte aligned -- and its own sequence's rows up to its own.  The prefix is read
  * once for all sequences.  prefix_len may be 0. */
 int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride,
                               int q_dtype, const void* prefix_k, const void* prefix_v, int64_t prefix_head_stride,

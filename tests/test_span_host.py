@@ -40,11 +40,11 @@ def test_no_tokens_is_no_launch():
 def test_prefix_scored_and_evict_refusals():
     lib = _lib.load()
 
-    def prefix(pk=OK, phs=64, p=16):
+    def prefix(pk=OK, phs=1024, p=16):
         return lib.alloyb_attn_shared_prefix(OK, 64, 64, 64, _lib.F16, pk, OK, phs, p, OK, OK, None, None, 0, 0, 0, OK, 1, OK, 2, 4, 2, 64, 0, 128, -1.0, OK,
                                              1 << 40, None)
     assert prefix() == 0 and prefix(None, p=0) == 0
-    assert prefix(None) == E_NULL and prefix(OK + 8) == E_ALIGN and prefix(phs=68) == E_ALIGN and prefix(p=-1) == E_SHAPE
+    assert prefix(None) == E_NULL and prefix(OK + 8) == E_ALIGN and prefix(phs=1028) == E_ALIGN and prefix(phs=1016) == E_SHAPE and prefix(p=-1) == E_SHAPE
 
     def scored(w):
         return lib.alloyb_attn_scored(OK, 64, 64, 64, _lib.F16, OK, OK, None, None, 0, 0, 0, OK, 1, w, OK, 2, 4, 2, 64, 0, 128, -1.0, OK, 1 << 40, None)
