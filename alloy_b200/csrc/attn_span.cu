@@ -84,9 +84,16 @@ __device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, 
 #pragma unroll
     for (int i = 0; i < C::SLOTS - 1; ++i) request(i);
     // the rows of this (sequence, KV head); rows past the last are zero
-    for (int r = warp; r < 16; r += WARPS) {
-        const int tok = r / P.G, hg = r - tok * P.G;
-        const float f = load_q_row<D>(q_s, r, P.q, b * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, r < rows, lane);
+    QRow<D> qr[16 / WARPS];
+#pragma unroll
+    for (int i = 0; i < 16 / WARPS; ++i) {
+        const int r = warp + i * WARPS, tok = r / P.G, hg = r - tok * P.G;
+        qr[i].read(P.q, b * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, r < rows, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / WARPS; ++i) {
+        const int r = warp + i * WARPS;
+        const float f = qr[i].put([&](int d) { return q_s + piece_at<D>(r, d >> 3) + (d & 7) * 2; }, P.q_dtype, lane);
         if (lane == 0) sh.back[r] = f * P.scale_log2;
     }
     __syncthreads();
@@ -405,11 +412,20 @@ __global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
             *reinterpret_cast<uint4*>(P.v + dst) = ld_after_wait(P.nv + src);
         }
     }
-#pragma unroll 4
-    for (int r = warp; r < 64; r += WARPS) {
-        const int R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
-        const float f = load_q_row<D>(q_s, r, P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, R < all_rows, lane);
-        if (lane == 0) back[r] = f * P.scale_log2;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 64 / WARPS; i0 += 8) {
+        QRow<D> qr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int R = row0 + warp + (i0 + i) * WARPS, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
+            qr[i].read(P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, R < all_rows, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = warp + (i0 + i) * WARPS;
+            const float f = qr[i].put([&](int d) { return q_s + piece_at<D>(r, d >> 3) + (d & 7) * 2; }, P.q_dtype, lane);
+            if (lane == 0) back[r] = f * P.scale_log2;
+        }
     }
     __syncthreads();
     const int r_own[2] = {row0 + warp * 16 + g, row0 + warp * 16 + g + 8};
@@ -650,7 +666,9 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
-constexpr int TC_ROWS = 192;             // rows of a KV head from which they go to the 5th-generation tensor cores
+// Rows of a KV head, and operations of a call, from which they go to the 5th-generation tensor cores.
+constexpr int TC_ROWS = 192;
+constexpr int64_t TC_WORK = 4000000000ll;
 constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
 // Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
 constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
@@ -705,7 +723,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
     } else {
-        p.tc = !scored && D <= 128 && rows >= TC_ROWS;
+        p.tc = !scored && D <= 128 && rows >= TC_ROWS && 4 * D * rows * items * seen >= TC_WORK;
         const int kt = p.tc ? 128 : (D == 256 ? 32 : 64), tr = p.tc ? 256 : 64;
         p.tiles = static_cast<int>((rows + tr - 1) / tr);
         const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + tr < S ? static_cast<int64_t>(window) + sinks + tr : S;
@@ -723,7 +741,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     p.part_lse = take(lse_rows * 4);
     p.part_o = take(o_rows * D * 4);
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_ROWS;
+        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_WORK;
         const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
         p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, p.pre_tc ? SMS : 2 * SMS);

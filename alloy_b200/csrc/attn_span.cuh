@@ -73,6 +73,9 @@ __device__ __forceinline__ bool sees(const Params& P, int row_pos, int j) {
     return j <= row_pos && (P.window <= 0 || j > row_pos - P.window || j < P.sinks);
 }
 
+// The lowest n bits (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
 __device__ __forceinline__ uint32_t s32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -116,60 +119,67 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t i, float a,
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = w;
 }
 
-// One query row into shared memory as fp16, by a warp (row null: zeros).  bf16 rows are brought under 2^15 by a power of two, so that fp16
-// holds every element of at least 2^-29 of the row's largest exactly; returns the factor that puts the row's scores back.
-// place(d): the shared address of element d, d a multiple of D / 32.
-template <int D, typename Place>
-__device__ __forceinline__ float load_q_row_to(const Place& place, const void* q, int64_t at, int dtype, bool vec, bool live, int lane) {
-    constexpr int E = D / 32;                                // elements of a lane
-    uint16_t h[E];
+// A query row on its way into shared memory as fp16, a warp's lanes D / 32 elements each.  Reading and placing are apart so that a warp
+// asks for several rows before it waits for the first.
+template <int D>
+struct QRow {
+    static constexpr int E = D / 32;
+    uint32_t w[E / 2];
+    __device__ __forceinline__ void read(const void* q, int64_t at, bool vec, bool live, int lane) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = 0;
-    if (live) {
+        for (int e = 0; e < E / 2; ++e) w[e] = 0u;
+        if (!live) return;                                   // rows past the last are zeros
         const uint16_t* src = static_cast<const uint16_t*>(q) + at + lane * E;
         if (vec) {
-            if (E == 2) *reinterpret_cast<uint32_t*>(h) = __ldcg(reinterpret_cast<const uint32_t*>(src));
-            if (E == 4) *reinterpret_cast<uint2*>(h) = __ldcg(reinterpret_cast<const uint2*>(src));
-            if (E == 8) *reinterpret_cast<uint4*>(h) = __ldcg(reinterpret_cast<const uint4*>(src));
+            if (E == 2) w[0] = __ldcg(reinterpret_cast<const uint32_t*>(src));
+            if (E == 4) {
+                const uint2 x = __ldcg(reinterpret_cast<const uint2*>(src));
+                w[0] = x.x;
+                w[1 % (E / 2)] = x.y;
+            }
+            if (E == 8) {
+                const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src));
+                w[0] = x.x;
+                w[1 % (E / 2)] = x.y;
+                w[2 % (E / 2)] = x.z;
+                w[3 % (E / 2)] = x.w;
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) h[e] = __ldcg(src + e);
+            for (int e = 0; e < E / 2; ++e) w[e] = __ldcg(src + 2 * e) | static_cast<uint32_t>(__ldcg(src + 2 * e + 1)) << 16;
         }
     }
-    float back = 1.0f;
-    if (dtype == ALLOYB_BF16) {
-        float x[E], top = 0.f;
+    // place(d): the shared address of element d.  bf16 rows are brought under 2^15 by a power of two, so that fp16 holds every element of at
+    // least 2^-29 of the row's largest exactly; returns the factor that puts the row's scores back.
+    template <typename Place>
+    __device__ __forceinline__ float put(const Place& place, int dtype, int lane) {
+        float back = 1.0f;
+        if (dtype == ALLOYB_BF16) {
+            float x[E], top = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = __uint_as_float(static_cast<uint32_t>(h[e]) << 16);
-            top = fmaxf(top, fabsf(x[e]));
+            for (int e = 0; e < E; ++e) {
+                x[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+                top = fmaxf(top, fabsf(x[e]));
+            }
+            top = warp_max(top);
+            const int ex = static_cast<int>(__float_as_uint(top) >> 23);
+            if (ex > 0 && ex < 255) {
+                const int field = min(268 - ex, 253);        // 2^(field - 127): the largest element lands in [2^14, 2^15)
+                const float f = __uint_as_float(static_cast<uint32_t>(field) << 23);
+                back = __uint_as_float(static_cast<uint32_t>(254 - field) << 23);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] *= f;
+            }
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
         }
-        top = warp_max(top);
-        const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-        if (ex > 0 && ex < 255) {
-            const int field = min(268 - ex, 253);            // 2^(field - 127): the largest element lands in [2^14, 2^15)
-            const float f = __uint_as_float(static_cast<uint32_t>(field) << 23);
-            back = __uint_as_float(static_cast<uint32_t>(254 - field) << 23);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] *= f;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) h[e] = __half_as_ushort(__float2half_rn(x[e]));
+        const uint32_t to = place(lane * E);
+        if (E == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(w[0]) : "memory");
+        if (E == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(w[0]), "r"(w[1 % (E / 2)]) : "memory");
+        if (E == 8) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1 % (E / 2)]), "r"(w[2 % (E / 2)]), "r"(w[3 % (E / 2)]) : "memory");
+        return back;
     }
-    const uint32_t to = place(lane * E);
-    if (E == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(*reinterpret_cast<uint32_t*>(h)) : "memory");
-    if (E == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(reinterpret_cast<uint32_t*>(h)[0]), "r"(reinterpret_cast<uint32_t*>(h)[1]) : "memory");
-    if (E == 8)
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(reinterpret_cast<uint32_t*>(h)[0]), "r"(reinterpret_cast<uint32_t*>(h)[1]),
-                     "r"(reinterpret_cast<uint32_t*>(h)[2]), "r"(reinterpret_cast<uint32_t*>(h)[3])
-                     : "memory");
-    return back;
-}
-
-template <int D>
-__device__ __forceinline__ float load_q_row(uint32_t dst, int r, const void* q, int64_t at, int dtype, bool vec, bool live, int lane) {
-    return load_q_row_to<D>([&](int d) { return dst + piece_at<D>(r, d >> 3) + (d & 7) * 2; }, q, at, dtype, vec, live, lane);
-}
+};
 
 // A warp's sixteen rows against NK * 16 keys of a tile: running maximum m, sum l (this lane's columns only; times 64) and output o of rows
 // g and g + 8, columns 8 i + 2 t of block i.

@@ -23,9 +23,8 @@ namespace st5 {
 using sp::Params;
 using sp::Seq;
 
-constexpr int ROWS = 256, KT = 128, STAGES = 2;
-constexpr int THREADS = 12 * 32;             // warp 1 MMA, warps 0, 2, 3 copies, warps 4-7 and 8-11 the groups' softmax
-constexpr int COPIERS = 96;
+constexpr int ROWS = 256, KT = 128, STAGES = 2, AHEAD = 3;
+constexpr int THREADS = 12 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-7 and 8-11 are their softmax
 constexpr int HALF = 128 * 128;              // bytes of 128 rows x 64 halves
 constexpr uint32_t SPIN = 1u << 22;
 
@@ -43,7 +42,7 @@ struct alignas(64) Args {
 };
 struct Bars {
     uint64_t k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
-    uint64_t s_full[2], p_full[2], o_full;
+    uint64_t s_full[2], p_full[2], o_full[2], turn[2];
     uint32_t tmem_base;
 };
 
@@ -150,6 +149,9 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
                  "r"(s32(bar)), "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -178,16 +180,17 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
-            bar_init(&bars->k_full[s], 3);
-            bar_init(&bars->v_full[s], 3);
-            bar_init(&bars->k_empty[s], 1);
-            bar_init(&bars->v_empty[s], 1);
+            bar_init(&bars->k_full[s], 1);
+            bar_init(&bars->v_full[s], 1);
+            bar_init(&bars->k_empty[s], 2);
+            bar_init(&bars->v_empty[s], 2);
         }
         for (int g = 0; g < 2; ++g) {
             bar_init(&bars->s_full[g], 1);
             bar_init(&bars->p_full[g], 4);
+            bar_init(&bars->o_full[g], 1);
+            bar_init(&bars->turn[g], 1);
         }
-        bar_init(&bars->o_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -203,12 +206,21 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     // ---- Q rows; dead rows are zero
-    for (int r = warp; r < ROWS; r += THREADS / 32) {
-        const int R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
-        const bool live = R < all_rows;
-        const float f = sp::load_q_row_to<D>([&](int d) { return q_s + (r >> 7) * TILE + piece_at(r & 127, d >> 3) + (d & 7) * 2; }, P.q,
-                                             rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_dtype, P.q_vec != 0, live, lane);
-        if (lane == 0) back[r] = f * P.scale_log2;
+    constexpr int WARPS = THREADS / 32, BATCH = 11;
+    for (int i0 = 0; i0 * WARPS < ROWS; i0 += BATCH) {
+        sp::QRow<D> qr[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = warp + (i0 + i) * WARPS, R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
+            qr[i].read(P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, r < ROWS && R < all_rows, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int r = warp + (i0 + i) * WARPS;
+            if (r >= ROWS) break;
+            const float f = qr[i].put([&](int d) { return q_s + (r >> 7) * TILE + piece_at(r & 127, d >> 3) + (d & 7) * 2; }, P.q_dtype, lane);
+            if (lane == 0) back[r] = f * P.scale_log2;
+        }
     }
     fence_async();
     fence_before();
@@ -218,78 +230,94 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     bool ok = true;
 
     if (warp < 4) {
-        if (warp == 1) {
-            // ------------------------------------------------ MMA issue (one lane)
+        if (warp == 1 || warp == 2) {
+            // ------------------------------------------------ MMA issue, a group each (one lane), in turns.  An issuer's own instructions
+            // between two MMAs (a wait that is over takes it a hundred clocks) pass under the other group's MMAs; the turns keep the groups
+            // apart: side by side, both would be in their softmax at once, and then both in the tensor pipe.
+            const int g = warp - 1;
+            const uint32_t d = tmem + g * C::COLS;
             if (lane == 0 && n_tiles > 0) {
-                auto scores = [&](int g, int s) {
+                auto scores = [&](int s) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-                        umma_ss(tmem + g * C::COLS, umma_desc(q_s + g * TILE + off, 16), umma_desc(k_s + s * TILE + off, 16), umma_idesc(KT, false), kk > 0);
+                        umma_ss(d, umma_desc(q_s + g * TILE + off, 16), umma_desc(k_s + s * TILE + off, 16), umma_idesc(KT, false), kk > 0);
                     }
-                    umma_commit(&bars->s_full[g]);
+                };
+                // group 0 begins; its turn n + 1 comes with group 1's turn n, which comes with group 0's turn n
+                auto my_turn = [&](int n) {
+                    if (g == 1 || n > 0) bar_wait(ok, &bars->turn[g], (g == 1 ? n : n - 1) & 1);
                 };
                 bar_wait(ok, &bars->k_full[0], 0);
+                my_turn(0);
                 fence_after();
                 if (ok) {
-                    scores(0, 0);
-                    scores(1, 0);
+                    scores(0);
+                    bar_arrive(&bars->turn[g ^ 1]);
+                    umma_commit(&bars->s_full[g]);
                     umma_commit(&bars->k_empty[0]);
                 }
                 for (int j = 0; j < n_tiles && ok; ++j) {
                     const int s = j % STAGES, s1 = (j + 1) % STAGES;
-                    for (int g = 0; g < 2 && ok; ++g) {
-                        bar_wait(ok, &bars->p_full[g], j & 1);
-                        if (g == 0) bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
-                        fence_after();
-                        if (!ok) break;
+                    const bool more = j + 1 < n_tiles;
+                    bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
+                    if (more) bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
+                    bar_wait(ok, &bars->p_full[g], j & 1);
+                    my_turn(j + 1);
+                    fence_after();
+                    if (!ok) break;
 #pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            umma_ts(tmem + g * C::COLS + 128, tmem + g * C::COLS + kk * 8, umma_desc(v_s + s * TILE + kk * 2048, HALF), umma_idesc(D, true),
-                                    j > 0 || kk > 0);
-                        if (g == 1) umma_commit(&bars->v_empty[s]);
-                        if (j + 1 < n_tiles) {
-                            if (g == 0) {
-                                bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
-                                fence_after();
-                            }
-                            if (ok) scores(g, s1);
-                            if (ok && g == 1) umma_commit(&bars->k_empty[s1]);
-                        }
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        umma_ts(d + 128, d + kk * 8, umma_desc(v_s + s * TILE + kk * 2048, HALF), umma_idesc(D, true), j > 0 || kk > 0);
+                    if (more) scores(s1);
+                    bar_arrive(&bars->turn[g ^ 1]);
+                    if (more) {
+                        umma_commit(&bars->s_full[g]);
+                        umma_commit(&bars->k_empty[s1]);
                     }
+                    umma_commit(&bars->v_empty[s]);
                 }
-                if (ok) umma_commit(&bars->o_full);
+                if (ok) umma_commit(&bars->o_full[g]);
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------ K and V tiles
-            const int ct = (warp == 0 ? 0 : warp - 1) * 32 + lane, c = ct % PIECES, r0 = ct / PIECES;
+            // ------------------------------------------------ tiles of K (warp 0) and V (warp 3)
+            const bool is_v = warp == 3;
+            const int c = lane % PIECES, r0 = lane / PIECES;
             const int z = PREFIX ? kvh : b * P.KV_H + kvh;
-            for (int n = 0; n < 2 * n_tiles; ++n) {                   // K of tile n / 2 (even), V (odd)
-                const int j = n >> 1, s = j % STAGES;
-                const bool is_v = n & 1;
+            const __half* src = PREFIX ? nullptr : (is_v ? P.v : P.k) + head + c * 8;
+            // Two stages of shared memory hide the way from L2; tiles on their way into L2 need none
+            auto ahead = [&](int j) {
+                const int place0 = (step0 + j) * KT;
+                if (lane == 0 && j < n_tiles && (PREFIX || (place0 >= sq.sink && place0 + KT <= sq.keys))) {
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) tma_prefetch_3d(is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z);
+                }
+            };
+            for (int j = STAGES; j < AHEAD; ++j) ahead(j);
+            for (int j = 0; j < n_tiles; ++j) {
+                const int s = j % STAGES;
+                ahead(j + AHEAD);
                 uint64_t* full = is_v ? &bars->v_full[s] : &bars->k_full[s];
                 if (j >= STAGES) bar_wait(ok, is_v ? &bars->v_empty[s] : &bars->k_empty[s], ((j / STAGES) - 1) & 1);
                 const uint32_t dst = (is_v ? v_s : k_s) + s * TILE;
                 const int place0 = (step0 + j) * KT;
                 // (rows past the prefix's last are outside the map: TMA fills them with zeros)
                 if (PREFIX || (place0 >= sq.sink && place0 + KT <= sq.keys)) {
-                    if (lane == 0) {
-                        if (warp == 0 && ok) {
-                            bar_expect(full, TILE);
+                    if (lane == 0 && ok) {
+                        bar_expect(full, TILE);
 #pragma unroll
-                            for (int h = 0; h < D / 64; ++h) tma_3d(dst + h * HALF, is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z, full);
-                        } else {
-                            bar_arrive(full);
-                        }
+                        for (int h = 0; h < D / 64; ++h) tma_3d(dst + h * HALF, is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z, full);
                     }
                 } else {
-                    const __half* src = (is_v ? P.v : P.k) + head + c * 8;
-                    if (ok)
-                        for (int r = r0; r < KT; r += COPIERS / PIECES) {
+                    if (ok) {
+#pragma unroll 8
+                        for (int i = 0; i < KT * PIECES / 32; ++i) {
+                            const int r = r0 + i * (32 / PIECES);
                             const bool live = place0 + r < sq.keys;
                             sp::copy16(dst + piece_at(r, c), src + static_cast<int64_t>(live ? sq.row_of(place0 + r) : 0) * D, live);
                         }
+                    }
                     sp::copy_commit();
                     sp::copy_wait<0>();
                     fence_async();                                    // to the tensor pipe's proxy
@@ -320,10 +348,15 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 whole = j1 <= first && (P.window <= 0 || (place0 >= sq.sink && j0 > last - P.window) || place0 + KT <= sq.sink);
             }
             if (!whole) {
+                // place e of the tile is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
+                const int hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - place0;
+                const int lo = PREFIX || P.window <= 0 ? -1 : pos - P.window - sq.lo + sq.sink - place0, sk = PREFIX ? 0 : P.sinks - place0;
 #pragma unroll
-                for (int e = 0; e < KT; ++e) {
-                    const int place = place0 + e;
-                    if (!(place < sq.keys && (PREFIX || sp::sees(P, pos, sq.row_of(place))))) s[e] = -INFINITY;
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t seen = sp::bits_below(hi + 1 - 32 * c) & (~sp::bits_below(lo + 1 - 32 * c) | sp::bits_below(sk - 32 * c));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen >> e & 1u)) s[c * 32 + e] = -INFINITY;
                 }
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -337,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 const float alpha = grow ? ex2(m_run - mx) : 1.0f;
                 if (grow) m_run = mx;
                 l_run *= alpha;
-                if (j > 0) {                                                  // (these scores came behind the last P V: it is complete)
+                if (j > 0) {                                                  // (these scores came behind the last P V, which is complete)
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         float o[16];
@@ -378,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         }
         // ---- normalise and store
         if (n_tiles > 0) {
-            bar_wait(ok, &bars->o_full, 0);
+            bar_wait(ok, &bars->o_full[g], 0);
             fence_after();
         }
         const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;

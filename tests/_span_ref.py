@@ -35,6 +35,33 @@ def attention(q, k, v, pos, *, window=0, sinks=0, prefix=None, scale=None):
     return out, w, mag, big
 
 
+def attention_wide(q, k, v, pos, *, window=0, sinks=0, prefix=None):
+    """The output and sum_j p |v| of ``attention`` by masks over whole score matrices, on the tensors' own device (for long calls)."""
+    b, h, n, d = q.shape
+    kv_h, s = k.shape[1], k.shape[2]
+    g = h // kv_h
+    out, mag = torch.zeros_like(q), torch.zeros_like(q)
+    j = torch.arange(s, device=q.device)
+    for i in range(b):
+        p = pos[i if len(pos) > 1 else 0]
+        if p < 0 or p + n > s:
+            continue
+        row = p + torch.arange(n, device=q.device)[:, None]
+        seen = j <= row
+        if window > 0:
+            seen &= (j > row - window) | (j < sinks)
+        any_row = seen.any(0)
+        for hq in range(h):
+            kk, vv, m = k[i, hq // g][any_row], v[i, hq // g][any_row], seen[:, any_row]
+            if prefix is not None:
+                kk, vv = torch.cat([prefix[0][hq // g], kk]), torch.cat([prefix[1][hq // g], vv])
+                m = torch.cat([torch.ones(n, prefix[0].shape[1], dtype=torch.bool, device=q.device), m], 1)
+            x = (q[i, hq] @ kk.T / math.sqrt(d)).masked_fill(~m, -math.inf)
+            pr = torch.softmax(x, -1)
+            out[i, hq], mag[i, hq] = pr @ vv, pr @ vv.abs()
+    return out, mag
+
+
 def out_bound(out, mag, dtype):
     """A probability enters P V rounded to fp16 (2^-11 of it); half as much again for the scores' and sums' 32 bits; the output is
     rounded once."""

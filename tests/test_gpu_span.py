@@ -227,6 +227,46 @@ def test_scored(b, h, kv_h, d, n, s, pos, dtype, layout, write):
         assert (off <= R.weight_bound(add[i][:, :p + n], big, d) + want[:, :p + n] * 2.0 ** -23).all()
 
 
+# calls large enough for the 5th-generation tensor cores (192 rows of a KV head, 4e9 operations)
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,window,sinks,dtype,layout,write", [
+    (1, 8, 1, 128, 700, 6000, [5100], 4000, 129, torch.float16, "model", True),
+    (1, 8, 1, 128, 700, 6000, [5300], 4000, 0, torch.float16, "model", False),     # to the cache's last row
+    (4, 24, 2, 64, 500, 5000, [4000, -1, 0, 777], 3500, 5, torch.bfloat16, "packed", True),
+    (2, 14, 2, 128, 1111, 1500, [389, 3], 9999, 7, torch.float16, "dense", True),   # causal, odd rows
+    (2, 32, 2, 64, 777, 4000, [3000, 100], 2000, 3000, torch.float16, "model", True),   # more sinks than window
+    (1, 64, 8, 128, 30, 20000, [19000], 16000, 64, torch.bfloat16, "model", True),  # few tiles: the keys are split
+])
+def test_window_long(b, h, kv_h, d, n, s, pos, window, sinks, dtype, layout, write):
+    c = Case(b, h, kv_h, d, n, s, pos, dtype, layout=layout)
+    k, v, k64, v64 = c.caches(write, window, sinks)
+    k0, v0 = k.clone(), v.clone()
+    out = OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), k, v, window, sinks, -1.0, write)
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, window=window, sinks=sinks)
+    check(out, ref.cpu(), mag.cpu(), dtype)
+    c.check_written(k0, k, c.nk64, write)
+    c.check_written(v0, v, c.nv64, write)
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,p,dtype", [
+    (70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], 14001, torch.float16),
+    (33, 32, 2, 64, 2, 24, [i % 23 - 1 for i in range(33)], 8100, torch.bfloat16),
+    (40, 64, 8, 128, 1, 3000, [i * 75 for i in range(40)], 3333, torch.float16),
+    (2, 32, 1, 128, 100, 900, [800, -1], 5000, torch.float16),                     # a chunk each, few sequences
+    (3, 64, 2, 64, 60, 9000, [8940, 10, 5000], 7000, torch.float16),               # the own keys too
+])
+def test_shared_prefix_long(b, h, kv_h, d, n, s, pos, p, dtype):
+    c = Case(b, h, kv_h, d, n, s, pos, dtype, prefix=p)
+    k, v, k64, v64 = c.caches(True)
+    k0 = k.clone()
+    store = [torch.full((kv_h, p + 8, d), BAD, dtype=torch.float16, device=DEV) for _ in range(2)]
+    for t, src in zip(store, (c.pk, c.pv)):
+        t[:, :p] = src.to(DEV)
+    out = OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), store[0][:, :p], store[1][:, :p], k, v)
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, prefix=(c.pk.double().to(DEV), c.pv.double().to(DEV)))
+    check(out, ref.cpu(), mag.cpu(), dtype)
+    c.check_written(k0, k, c.nk64, True)
+
+
 def evict_case(b, kv_h, s, s_out, d, lengths, kind="random", seed=0):
     g = torch.Generator().manual_seed(seed + s)
     k, v = torch.randn(b, kv_h, s, d, generator=g).half(), torch.randn(b, kv_h, s, d, generator=g).half()
