@@ -508,7 +508,8 @@ __global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
 
 // ---------------------------------------------------------------------------------------------------------------- joining
 constexpr int MERGE_WARPS = 8;
-constexpr int WEIGHT_KEYS = MERGE_WARPS * 32 * 4;                        // keys whose weights a CTA of the merge launch adds up
+constexpr int WEIGHT_KEYS = 256;                                         // keys whose weights a CTA of the merge launch adds up
+constexpr int WIDE_PARTS = 24;                                           // partial results from which a row gets a CTA, not a warp
 
 // Where the partial results of row R of a (sequence, KV head) lie.
 struct Parts {
@@ -551,40 +552,55 @@ __device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
     return p;
 }
 
-// The row's log-sum over all its parts, by a warp.
-__device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int lane) {
-    float top = -INFINITY;
-    for (int i = lane; i < p.own; i += 32) top = fmaxf(top, __ldcg(P.part_lse + p.own_index(i)));
-    for (int i = lane; i < p.pre; i += 32) top = fmaxf(top, __ldcg(P.pre_lse + p.pre_at + i * P.pre_tile_rows));
-    top = warp_max(top);
-    float l = 0.f;
-    for (int i = lane; i < p.own; i += 32) {
-        const float x = __ldcg(P.part_lse + p.own_index(i));
-        l += x == -INFINITY ? 0.f : ex2(x - top);                        // (a NaN stays one)
+// A running log-sum of log-sums, and the join of `lanes` neighbouring lanes' (a NaN stays one; -inf is nothing).
+struct LogSum {
+    float m = -INFINITY, l = 0.f;
+    __device__ __forceinline__ void add(float x) {
+        if (x == -INFINITY) return;
+        if (x > m) {
+            l = fmaf(l, ex2(m - x), 1.0f);
+            m = x;
+        } else {
+            l += ex2(x - m);
+        }
     }
-    for (int i = lane; i < p.pre; i += 32) {
-        const float x = __ldcg(P.pre_lse + p.pre_at + i * P.pre_tile_rows);
-        l += x == -INFINITY ? 0.f : ex2(x - top);
+    __device__ __forceinline__ float join(int lanes) {
+        for (int o = lanes >> 1; o > 0; o >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o);
+            const float top = fmaxf(m, om);
+            if (top != -INFINITY) l = l * ex2(m - top) + ol * ex2(om - top);
+            else l += ol;
+            m = top;
+        }
+        return l == 0.f ? -INFINITY : m + log2f(l);
     }
-    l = warp_sum(l);
-    return l == 0.f ? -INFINITY : top + log2f(l);
+};
+__device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int first, int lanes) {
+    LogSum s;
+#pragma unroll 4
+    for (int i = first; i < p.own; i += lanes) s.add(__ldcg(P.part_lse + p.own_index(i)));
+#pragma unroll 4
+    for (int i = first; i < p.pre; i += lanes) s.add(__ldcg(P.pre_lse + p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows));
+    return s.join(lanes);
 }
 
-// Grid (rows + CTAs for the weights, sequences * KV heads).
+// Grid (CTAs for the rows + CTAs for the weights, sequences * KV heads); P.merge_team warps a row, 1 or all.
 template <int D, bool STREAM, bool SCORED>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
     pdl_launch_dependents();
-    __shared__ float sm_o[MERGE_WARPS][D];
+    __shared__ float4 sm[D >= 128 || !SCORED ? MERGE_WARPS * D / 4 : WEIGHT_KEYS];   // rows: a warp's sums each; weights: a row group's each
     __shared__ float sm_lse[64];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, item = blockIdx.y, rows = P.n * P.G;
     const int b = item / P.KV_H, kvh = item - b * P.KV_H;
+    const int team = P.merge_team, row_ctas = (rows * team + MERGE_WARPS - 1) / MERGE_WARPS;
     pdl_wait();
     const int pos = live_pos(P, b, false);
-    if (static_cast<int>(blockIdx.x) < rows) {
-        const int R = blockIdx.x, tok = R / P.G, hg = R - tok * P.G;
+    if (static_cast<int>(blockIdx.x) < row_ctas) {
+        const int R = (blockIdx.x * MERGE_WARPS + warp) / team, w0 = warp % team;
+        if (R >= rows) return;                                           // (a whole CTA's row, or a warp's: nobody waits for it)
         const Parts p = parts_of<STREAM>(P, item, R);
         if (p.stored) return;
-        const float lse = row_lse(P, p, lane);
+        const float lse = row_lse(P, p, lane, 32);
         float acc[D / 32];
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
@@ -605,43 +621,58 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
         };
         if (pos >= 0) {
 #pragma unroll 4
-            for (int i = warp; i < p.own; i += MERGE_WARPS) add(P.part_lse, P.part_o, p.own_index(i));
+            for (int i = w0; i < p.own; i += team) add(P.part_lse, P.part_o, p.own_index(i));
 #pragma unroll 4
-            for (int i = warp; i < p.pre; i += MERGE_WARPS) add(P.pre_lse, P.pre_o, p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows);
+            for (int i = w0; i < p.pre; i += team) add(P.pre_lse, P.pre_o, p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows);
         }
+        const int tok = R / P.G, hg = R - tok * P.G;
+        const int64_t out = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+        if (team == 1) {
+#pragma unroll
+            for (int c = 0; c < PER; ++c) {
+                const int64_t at = out + (c * 32 + lane) * E;
+                if (E == 4) store4(P.out, P.q_dtype, at, acc[c * E], acc[c * E + 1], acc[c * E + 2 % E], acc[c * E + 3 % E]);
+                else store2(P.out, P.q_dtype, at, acc[c * E], acc[c * E + 1]);
+            }
+            return;
+        }
+        float* sm_o = reinterpret_cast<float*>(sm);
 #pragma unroll
         for (int c = 0; c < PER; ++c)
 #pragma unroll
-            for (int e = 0; e < E; ++e) sm_o[warp][(c * 32 + lane) * E + e] = acc[c * E + e];
+            for (int e = 0; e < E; ++e) sm_o[warp * D + (c * 32 + lane) * E + e] = acc[c * E + e];
         __syncthreads();
         if (threadIdx.x < D / 4) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < MERGE_WARPS; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(&sm_o[w][threadIdx.x * 4]);
+                const float4 v = sm[w * (D / 4) + threadIdx.x];
                 sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
             }
-            store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + threadIdx.x * 4, sum.x, sum.y, sum.z, sum.w);
+            store4(P.out, P.q_dtype, out + threadIdx.x * 4, sum.x, sum.y, sum.z, sum.w);
         }
         return;
     }
     if (SCORED) {
-        // weights of WEIGHT_KEYS positions: the rows' probabilities, summed in the rows' order
-        const int first_key = (blockIdx.x - rows) * WEIGHT_KEYS, j0 = first_key + threadIdx.x * 4, len = pos + P.n;
+        // weights of WEIGHT_KEYS positions: four groups of rows, a thread four keys; the rows' probabilities are summed in a fixed order
+        const int first_key = (blockIdx.x - row_ctas) * WEIGHT_KEYS, len = pos + P.n;
         if (pos < 0 || first_key >= len) return;
+        const int group = threadIdx.x >> 6, j0 = first_key + (threadIdx.x & 63) * 4;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < rows; r0 += 64) {
             __syncthreads();
-            for (int r = warp; r < 64 && r0 + r < rows; r += MERGE_WARPS) {
-                const float lse = row_lse(P, parts_of<STREAM>(P, item, r0 + r), lane);
-                if (lane == 0) sm_lse[r] = lse;
+            {
+                const int r = threadIdx.x >> 2;
+                float lse = 0.f;
+                if (r0 + (r & ~7) < rows) lse = row_lse(P, parts_of<STREAM>(P, item, min(r0 + r, rows - 1)), threadIdx.x & 3, 4);    // (a warp's eight rows)
+                if ((threadIdx.x & 3) == 0) sm_lse[r] = lse;
             }
             __syncthreads();
             if (j0 < len) {
                 const float* src = P.scores + (static_cast<int64_t>(item) * rows + r0) * P.pitch + j0;
                 const int count = min(64, rows - r0);
 #pragma unroll 8
-                for (int r = 0; r < count; ++r) {
+                for (int r = group; r < count; r += 4) {
                     // a key behind the row's last position has no score where its tile was not this row's
                     const float4 s = __ldcg(reinterpret_cast<const float4*>(src + r * P.pitch));
                     const int row_pos = pos + (r0 + r) / P.G;
@@ -653,13 +684,15 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
                 }
             }
         }
-        float* w = P.weights + static_cast<int64_t>(item) * P.S;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int j = j0 + e;
-            if (j < pos) w[j] += sum[e];
-            else if (j < len) w[j] = sum[e];
-        }
+        sm[threadIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        __syncthreads();
+        const int j = first_key + threadIdx.x;                           // a key each
+        if (j >= len) return;
+        const float* parts = reinterpret_cast<const float*>(sm) + threadIdx.x;
+        float w = (parts[0] + parts[WEIGHT_KEYS]) + (parts[2 * WEIGHT_KEYS] + parts[3 * WEIGHT_KEYS]);
+        float* to = P.weights + static_cast<int64_t>(item) * P.S + j;
+        if (j < pos) w += *to;
+        *to = w;
     }
 }
 
@@ -685,12 +718,13 @@ struct Plan {
 
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-// CTAs that share a tile's keys: rounds of resident CTAs times a CTA's steps (and about three steps' time to begin and to end it).
-static int choose_splits(int64_t ctas, int64_t steps, int resident) {
+// CTAs that share a tile's keys: rounds of resident CTAs times a CTA's steps (and about four steps' time to begin and to end it); joining
+// partial results costs `join` steps' time, and a little more with every part.
+static int choose_splits(int64_t ctas, int64_t steps, int resident, int join) {
     int best = 1;
     int64_t cost = INT64_MAX;
     for (int s = 1; s <= 64 && s <= steps; ++s) {
-        const int64_t c = ((ctas * s + resident - 1) / resident) * ((steps + s - 1) / s + 3) * 8 + s;
+        const int64_t c = ((ctas * s + resident - 1) / resident) * ((steps + s - 1) / s + 4) * 8 + (s > 1 ? 8 * join + s : 0);
         if (c < cost) {
             cost = c;
             best = s;
@@ -727,7 +761,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         const int kt = p.tc ? 128 : (D == 256 ? 32 : 64), tr = p.tc ? 256 : 64;
         p.tiles = static_cast<int>((rows + tr - 1) / tr);
         const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + tr < S ? static_cast<int64_t>(window) + sinks + tr : S;
-        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, p.tc ? SMS : 2 * SMS);
+        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, p.tc ? SMS : 2 * SMS, scored || P > 0 ? 0 : 6);
         lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * tr;
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
@@ -744,7 +778,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_WORK;
         const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
-        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, p.pre_tc ? SMS : 2 * SMS);
+        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, p.pre_tc ? SMS : 2 * SMS, 0);
         const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * tr;
         p.pre_lse = take(r * 4);
         p.pre_o = take(r * D * 4);
@@ -843,8 +877,11 @@ static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
     if (rc != ALLOYB_OK) return rc;
     if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
     const int more = SCORED ? (P.S + WEIGHT_KEYS - 1) / WEIGHT_KEYS : 0;
+    Params M = P;
+    M.merge_team = plan.pre_splits + (plan.stream ? (plan.ctas + items - 1) / items + 1 : plan.splits) >= WIDE_PARTS ? MERGE_WARPS : 1;
     auto merge = plan.stream ? span_merge_kernel<D, true, SCORED> : span_merge_kernel<D, false, SCORED>;
-    const cudaError_t e = launch_pdl(merge, dim3(rows + more, items), dim3(MERGE_WARPS * 32), 0, st, P);
+    const int row_ctas = (rows * M.merge_team + MERGE_WARPS - 1) / MERGE_WARPS;
+    const cudaError_t e = launch_pdl(merge, dim3(row_ctas + more, items), dim3(MERGE_WARPS * 32), 0, st, M);
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return ALLOYB_E_CUDA;

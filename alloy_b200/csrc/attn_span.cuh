@@ -42,6 +42,7 @@ struct Params {
     float* pre_o;                        // the prefix's partials, [KV head][tile][split][row][D]
     float* pre_lse;
     int pre_splits, pre_tile_rows;
+    int merge_team;                      // warps that join a row's partial results
     float* scores;                       // [sequence, KV head][row][pitch], log2 frame, for the weights
     int64_t pitch;
     float* weights;                      // (B, KV_H, S)
@@ -117,6 +118,11 @@ __device__ __forceinline__ void store4(void* out, int dtype, int64_t i, float a,
         w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
     }
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = w;
+}
+
+__device__ __forceinline__ void store2(void* out, int dtype, int64_t i, float a, float b) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + i) = dtype == ALLOYB_F16 ? pack_h2(a, b) : *reinterpret_cast<const uint32_t*>(&x);
 }
 
 // A query row on its way into shared memory as fp16, a warp's lanes D / 32 elements each.  Reading and placing are apart so that a warp

@@ -16,7 +16,8 @@ namespace ev {
 
 static __device__ int g_evict_status = 0;    // sticky: 1 once a length was out of range
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
-constexpr int BINS = 2048;
+constexpr int BINS = 2 * THREADS;                // eleven bits
+constexpr int KEYS = 48 * 1024;                  // weights that fit into shared memory
 
 struct Params {
     const __half *k, *v;                     // (B, KV_H, S, D)
@@ -44,10 +45,13 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
+// The weights' integer forms are read once and kept in shared memory, the first `cap` of them; more come from L2 in every pass.
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P, int cap) {
     pdl_launch_dependents();
-    __shared__ int hist[BINS], warp_above[WARPS], warp_equal[WARPS], found[3];
+    extern __shared__ uint32_t keys[];
+    __shared__ int hist[BINS], warp_sum[WARPS], warp_above[WARPS], warp_equal[WARPS], found[2];
     const int item = blockIdx.x, b = item / P.KV_H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
     pdl_wait();
     const int len = length_of(P, b, threadIdx.x == 0 && item == b * P.KV_H);
     int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
@@ -62,39 +66,49 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
     for (int i = threadIdx.x; i < P.recent; i += THREADS) kept[P.keep - P.recent + i] = last + i;
     if (want == 0) return;
     const float* w = P.w + static_cast<int64_t>(item) * P.S + first;
+    auto key = [&](int i) { return i < cap ? keys[i] : order_of(__ldcg(w + i)); };
+    __syncthreads();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+        const uint32_t u = order_of(__ldcg(w + i));
+        if (i < cap) keys[i] = u;
+        atomicAdd(&hist[u >> 21], 1);
+    }
     // the integer form of the want-th largest: `prefix` holds the digits found, `left` how many are wanted of those that share them
     uint32_t prefix = 0u;
     int left = want;
     constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
 #pragma unroll
     for (int digit = 0; digit < 3; ++digit) {
-        for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
-        __syncthreads();
-        const uint32_t mask = digit == 0 ? 0u : ~0u << (SHIFT[digit] + BITS[digit]);
+        if (digit > 0) {
+            const uint32_t mask = ~0u << (SHIFT[digit] + BITS[digit]);
 #pragma unroll 4
-        for (int i = threadIdx.x; i < count; i += THREADS) {
-            const uint32_t u = order_of(__ldcg(w + i));
-            if ((u & mask) == prefix) atomicAdd(&hist[(u >> SHIFT[digit]) & ((1u << BITS[digit]) - 1u)], 1);
+            for (int i = threadIdx.x; i < count; i += THREADS) {
+                const uint32_t u = key(i);
+                if ((u & mask) == prefix) atomicAdd(&hist[(u >> SHIFT[digit]) & ((1u << BITS[digit]) - 1u)], 1);
+            }
         }
         __syncthreads();
-        if (warp == 0) {
-            // from the top: the bin in which the count reaches `left`; a lane adds up BINS / 32 bins
-            constexpr int PER = BINS / 32;
-            int sum = 0;
-            for (int i = 0; i < PER; ++i) sum += hist[BINS - 1 - lane * PER - i];
-            int before = sum;
+        // from the top: the bin in which the count reaches `left`; a thread has two neighbouring bins, and clears them for the next digit
+        const int bin = BINS - 1 - 2 * threadIdx.x, h0 = hist[bin], h1 = hist[bin - 1];
+        hist[bin] = hist[bin - 1] = 0;
+        int upto = h0 + h1;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += y;
-            }
-            before -= sum;
-            if (before < left && before + sum >= left) {
-                int bin = BINS - 1 - lane * PER;
-                while (before + hist[bin] < left) before += hist[bin--];
-                found[0] = bin;
-                found[1] = left - before;
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) warp_sum[warp] = upto;
+        __syncthreads();
+        int above = lane < warp ? warp_sum[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        upto += above;
+        const int before = upto - h0 - h1;
+        if (before < left && upto >= left) {
+            const bool upper = before + h0 >= left;
+            found[0] = upper ? bin : bin - 1;
+            found[1] = left - before - (upper ? 0 : h0);
         }
         __syncthreads();
         prefix |= static_cast<uint32_t>(found[0]) << SHIFT[digit];
@@ -105,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
     int above = 0, equal = 0;
     for (int i0 = r0; i0 < r1; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t u = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+        const uint32_t u = i < r1 ? key(i) : 0u;
         above += __popc(__ballot_sync(0xffffffffu, i < r1 && u > prefix));
         equal += __popc(__ballot_sync(0xffffffffu, i < r1 && u == prefix));
     }
@@ -114,14 +128,16 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
         warp_equal[warp] = equal;
     }
     __syncthreads();
-    above = equal = 0;
-    for (int k = 0; k < warp; ++k) {
-        above += warp_above[k];
-        equal += warp_equal[k];
+    above = lane < warp ? warp_above[lane] : 0;
+    equal = lane < warp ? warp_equal[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        above += __shfl_xor_sync(0xffffffffu, above, o);
+        equal += __shfl_xor_sync(0xffffffffu, equal, o);
     }
     for (int i0 = r0; i0 < r1; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t u = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+        const uint32_t u = i < r1 ? key(i) : 0u;
         const uint32_t is_above = __ballot_sync(0xffffffffu, i < r1 && u > prefix), is_equal = __ballot_sync(0xffffffffu, i < r1 && u == prefix);
         const uint32_t below = (1u << lane) - 1u;
         const int a = above + __popc(is_above & below), e = equal + __popc(is_equal & below);
@@ -273,7 +289,16 @@ extern "C" int alloyb_kv_evict(const void* k, const void* v, const float* weight
     P.kept = kept; P.new_len = new_lengths;
     P.B = B; P.KV_H = KV_H; P.S = S; P.S_out = S_out; P.keep = keep; P.sinks = sinks; P.recent = recent;
     cudaStream_t st = as_stream(stream);
-    cudaError_t e = launch_pdl(ev::evict_select_kernel, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), 0, st, P);
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    cudaError_t e = cudaSuccess;
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(ev::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ev::KEYS * 4);
+        if (e == cudaSuccess) ready[dev] = true;
+    }
+    const int cap = S < ev::KEYS ? S : ev::KEYS;
+    if (e == cudaSuccess) e = launch_pdl(ev::evict_select_kernel, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), static_cast<size_t>(cap) * 4, st, P, cap);
     if (e == cudaSuccess) {
         switch (D) {
             case 64: e = ev::copy<64>(P, in_place, st); break;
