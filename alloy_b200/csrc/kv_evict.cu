@@ -17,7 +17,6 @@ namespace ev {
 static __device__ int g_evict_status = 0;    // sticky: 1 once a length was out of range
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int BINS = 2 * THREADS;                // eleven bits
-constexpr int KEYS = 48 * 1024;                  // weights that fit into shared memory
 
 struct Params {
     const __half *k, *v;                     // (B, KV_H, S, D)
@@ -45,11 +44,42 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The weights' integer forms are read once and kept in shared memory, the first `cap` of them; more come from L2 in every pass.
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P, int cap) {
+// One digit of the wanted weight, from the counts of its values in hist: the bin in which the count from the top reaches `left` is added to
+// `prefix`, and `left` becomes how many are wanted of that bin.  Clears hist for the next digit.  Every thread of the CTA calls it.
+__device__ __forceinline__ void take_digit(int* hist, int* warp_sum, int* found, int shift, uint32_t& prefix, int& left) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    const int bin = BINS - 1 - 2 * threadIdx.x, h0 = hist[bin], h1 = hist[bin - 1];      // two neighbouring bins a thread
+    hist[bin] = hist[bin - 1] = 0;
+    int upto = h0 + h1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    upto += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
+    const int before = upto - h0 - h1;
+    if (before < left && upto >= left) {
+        const bool upper = before + h0 >= left;
+        found[0] = upper ? bin : bin - 1;
+        found[1] = left - before - (upper ? 0 : h0);
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(found[0]) << shift;
+    left = found[1];
+}
+
+// R * THREADS weights at most, R of them in a thread's registers: position k * THREADS + thread.  R == 0: any number, read anew in every pass
+// (the positions of a warp then lie side by side in the last two).
+template <int R>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
     pdl_launch_dependents();
-    extern __shared__ uint32_t keys[];
-    __shared__ int hist[BINS], warp_sum[WARPS], warp_above[WARPS], warp_equal[WARPS], found[2];
+    constexpr int RUNS = R > 0 ? R * WARPS : WARPS;
+    __shared__ int hist[BINS], warp_sum[WARPS], found[2];
+    __shared__ uint32_t run_sum[RUNS];                       // of 32 positions (R == 0: of a warp's): how many above, and equal << 16
+    __shared__ int run_equal[R > 0 ? 1 : WARPS];
     const int item = blockIdx.x, b = item / P.KV_H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
     pdl_wait();
@@ -62,88 +92,101 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P, i
     }
     // len > keep >= sinks + recent: the three parts do not meet
     const int first = P.sinks, last = len - P.recent, count = last - first, want = P.keep - P.sinks - P.recent;
+    const float* w = P.w + static_cast<int64_t>(item) * P.S + first;
+    uint32_t u[R > 0 ? R : 1];
+    if (R > 0) {
+        float x[R > 0 ? R : 1];
+        const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+        for (int k = 0; k < R; ++k) x[k] = k * THREADS + threadIdx.x < count ? __ldcg(w + k * THREADS + threadIdx.x) : nan;
+        // (places past the last count as NaN: below everything, and behind every position that the limit may fall on)
+#pragma unroll
+        for (int k = 0; k < R; ++k) u[k] = order_of(x[k]);
+    }
     for (int i = threadIdx.x; i < P.sinks; i += THREADS) kept[i] = i;
     for (int i = threadIdx.x; i < P.recent; i += THREADS) kept[P.keep - P.recent + i] = last + i;
     if (want == 0) return;
-    const float* w = P.w + static_cast<int64_t>(item) * P.S + first;
-    auto key = [&](int i) { return i < cap ? keys[i] : order_of(__ldcg(w + i)); };
     __syncthreads();
-#pragma unroll 8
-    for (int i = threadIdx.x; i < count; i += THREADS) {
-        const uint32_t u = order_of(__ldcg(w + i));
-        if (i < cap) keys[i] = u;
-        atomicAdd(&hist[u >> 21], 1);
-    }
     // the integer form of the want-th largest: `prefix` holds the digits found, `left` how many are wanted of those that share them
     uint32_t prefix = 0u;
     int left = want;
     constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
 #pragma unroll
     for (int digit = 0; digit < 3; ++digit) {
-        if (digit > 0) {
-            const uint32_t mask = ~0u << (SHIFT[digit] + BITS[digit]);
-#pragma unroll 4
-            for (int i = threadIdx.x; i < count; i += THREADS) {
-                const uint32_t u = key(i);
-                if ((u & mask) == prefix) atomicAdd(&hist[(u >> SHIFT[digit]) & ((1u << BITS[digit]) - 1u)], 1);
+        auto tell = [&](uint32_t x) {
+            if (digit == 0 || x >> (SHIFT[digit] + BITS[digit]) == prefix >> (SHIFT[digit] + BITS[digit]))
+                atomicAdd(&hist[(x >> SHIFT[digit]) & ((1u << BITS[digit]) - 1u)], 1);
+        };
+        if (R > 0) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                if (k * THREADS >= count) break;
+                tell(u[k]);
             }
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < count; i += THREADS) tell(order_of(__ldcg(w + i)));
+        }
+        take_digit(hist, warp_sum, found, SHIFT[digit], prefix, left);
+    }
+    // positions above the limit, and the first `left` of those equal to it
+    const uint32_t below = (1u << lane) - 1u;
+    if (R > 0) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            if (k * THREADS >= count) break;
+            const uint32_t is_above = __ballot_sync(0xffffffffu, u[k] > prefix), is_equal = __ballot_sync(0xffffffffu, u[k] == prefix);
+            if (lane == 0) run_sum[k * WARPS + warp] = __popc(is_above) | __popc(is_equal) << 16;
         }
         __syncthreads();
-        // from the top: the bin in which the count reaches `left`; a thread has two neighbouring bins, and clears them for the next digit
-        const int bin = BINS - 1 - 2 * threadIdx.x, h0 = hist[bin], h1 = hist[bin - 1];
-        hist[bin] = hist[bin - 1] = 0;
-        int upto = h0 + h1;
+        // what lies before each run: a thread adds up its run and those of its warp before it, then the warps before
+        const int runs = (count + THREADS - 1) / THREADS * WARPS;
+        uint32_t own = static_cast<int>(threadIdx.x) < runs ? run_sum[threadIdx.x] : 0u, upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
         }
-        if (lane == 31) warp_sum[warp] = upto;
+        if (lane == 31) warp_sum[warp] = static_cast<int>(upto);
         __syncthreads();
-        int above = lane < warp ? warp_sum[lane] : 0;
+        upto += __reduce_add_sync(0xffffffffu, lane < warp ? static_cast<uint32_t>(warp_sum[lane]) : 0u);
+        if (static_cast<int>(threadIdx.x) < runs) run_sum[threadIdx.x] = upto - own;
+        __syncthreads();
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-        upto += above;
-        const int before = upto - h0 - h1;
-        if (before < left && upto >= left) {
-            const bool upper = before + h0 >= left;
-            found[0] = upper ? bin : bin - 1;
-            found[1] = left - before - (upper ? 0 : h0);
+        for (int k = 0; k < R; ++k) {
+            if (k * THREADS >= count) break;
+            const uint32_t is_above = __ballot_sync(0xffffffffu, u[k] > prefix), is_equal = __ballot_sync(0xffffffffu, u[k] == prefix);
+            const uint32_t before = run_sum[k * WARPS + warp];
+            const int a = static_cast<int>(before & 0xffffu) + __popc(is_above & below), e = static_cast<int>(before >> 16) + __popc(is_equal & below);
+            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + k * THREADS + threadIdx.x;
+        }
+    } else {
+        const int run = (count + WARPS * 32 - 1) / (WARPS * 32) * 32, r0 = min(count, warp * run), r1 = min(count, r0 + run);
+        int above = 0, equal = 0;
+#pragma unroll 4
+        for (int i0 = r0; i0 < r1; i0 += 32) {
+            const int i = i0 + lane;
+            const uint32_t x = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+            above += __popc(__ballot_sync(0xffffffffu, i < r1 && x > prefix));
+            equal += __popc(__ballot_sync(0xffffffffu, i < r1 && x == prefix));
+        }
+        if (lane == 0) {
+            run_sum[warp] = above;
+            run_equal[warp] = equal;
         }
         __syncthreads();
-        prefix |= static_cast<uint32_t>(found[0]) << SHIFT[digit];
-        left = found[1];
-    }
-    // positions above the limit, and the first `left` of those equal to it: a warp owns a run of positions
-    const int run = (count + WARPS * 32 - 1) / (WARPS * 32) * 32, r0 = min(count, warp * run), r1 = min(count, r0 + run);
-    int above = 0, equal = 0;
-    for (int i0 = r0; i0 < r1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t u = i < r1 ? key(i) : 0u;
-        above += __popc(__ballot_sync(0xffffffffu, i < r1 && u > prefix));
-        equal += __popc(__ballot_sync(0xffffffffu, i < r1 && u == prefix));
-    }
-    if (lane == 0) {
-        warp_above[warp] = above;
-        warp_equal[warp] = equal;
-    }
-    __syncthreads();
-    above = lane < warp ? warp_above[lane] : 0;
-    equal = lane < warp ? warp_equal[lane] : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        above += __shfl_xor_sync(0xffffffffu, above, o);
-        equal += __shfl_xor_sync(0xffffffffu, equal, o);
-    }
-    for (int i0 = r0; i0 < r1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t u = i < r1 ? key(i) : 0u;
-        const uint32_t is_above = __ballot_sync(0xffffffffu, i < r1 && u > prefix), is_equal = __ballot_sync(0xffffffffu, i < r1 && u == prefix);
-        const uint32_t below = (1u << lane) - 1u;
-        const int a = above + __popc(is_above & below), e = equal + __popc(is_equal & below);
-        if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + i;
-        above += __popc(is_above);
-        equal += __popc(is_equal);
+        above = static_cast<int>(__reduce_add_sync(0xffffffffu, lane < warp ? run_sum[lane] : 0u));
+        equal = __reduce_add_sync(0xffffffffu, lane < warp ? run_equal[lane] : 0);
+#pragma unroll 4
+        for (int i0 = r0; i0 < r1; i0 += 32) {
+            const int i = i0 + lane;
+            const uint32_t x = i < r1 ? order_of(__ldcg(w + i)) : 0u;
+            const uint32_t is_above = __ballot_sync(0xffffffffu, i < r1 && x > prefix), is_equal = __ballot_sync(0xffffffffu, i < r1 && x == prefix);
+            const int a = above + __popc(is_above & below), e = equal + __popc(is_equal & below);
+            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + i;
+            above += __popc(is_above);
+            equal += __popc(is_equal);
+        }
     }
 }
 
@@ -289,16 +332,9 @@ extern "C" int alloyb_kv_evict(const void* k, const void* v, const float* weight
     P.kept = kept; P.new_len = new_lengths;
     P.B = B; P.KV_H = KV_H; P.S = S; P.S_out = S_out; P.keep = keep; P.sinks = sinks; P.recent = recent;
     cudaStream_t st = as_stream(stream);
-    static bool ready[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    cudaError_t e = cudaSuccess;
-    if (!ready[dev]) {
-        e = cudaFuncSetAttribute(ev::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ev::KEYS * 4);
-        if (e == cudaSuccess) ready[dev] = true;
-    }
-    const int cap = S < ev::KEYS ? S : ev::KEYS;
-    if (e == cudaSuccess) e = launch_pdl(ev::evict_select_kernel, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), static_cast<size_t>(cap) * 4, st, P, cap);
+    // as many weights in registers as a cache of S positions can ask for (16384: 22 us from shared memory); past 32 a thread: none
+    auto select = S <= 8 * ev::THREADS ? ev::evict_select_kernel<8> : S <= 16 * ev::THREADS ? ev::evict_select_kernel<16> : S <= 32 * ev::THREADS ? ev::evict_select_kernel<32> : ev::evict_select_kernel<0>;
+    cudaError_t e = launch_pdl(select, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), 0, st, P);
     if (e == cudaSuccess) {
         switch (D) {
             case 64: e = ev::copy<64>(P, in_place, st); break;
