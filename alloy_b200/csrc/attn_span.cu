@@ -42,6 +42,38 @@ constexpr int MIN_STEPS = 2;
 
 __device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max((total + ctas - 1) / ctas, MIN_STEPS); }
 
+// Requests places [place0, place0 + ROWS) of a span: K's rows to dst, V's `v_off` bytes behind; LANES threads, this one is `thread`.  Rows in one
+// piece of the cache take the short way; the others (first rows next to the window, the sequence's end, new tokens) are told apart one by one,
+// places past the last key are filled with zeros: what the cache holds there is nobody's business.
+template <int D, int ROWS, int LANES>
+__device__ __forceinline__ void request_span(const Params& P, const Seq& sq, int b, int kvh, int place0, uint32_t dst, uint32_t v_off, int thread) {
+    using C = Copy<D, ROWS, LANES>;
+    const int64_t head = (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
+    const int first = sq.row_of(place0);
+    if (place0 + ROWS <= sq.keys && sq.row_of(place0 + ROWS - 1) == first + ROWS - 1 && (!P.nk || first + ROWS <= sq.pos)) {
+        const int64_t at = head + static_cast<int64_t>(first + C::row(thread)) * D + C::col(thread);
+        C::rows(dst + C::place(thread), P.k + at);
+        C::rows(dst + v_off + C::place(thread), P.v + at);
+        return;
+    }
+#pragma unroll 2
+    for (int i = 0; i < C::N; ++i) {
+        const int r = C::row(thread) + i * C::STRIDE, place = place0 + r;
+        const bool live = place < sq.keys;
+        const int j = live ? sq.row_of(place) : 0;
+        int64_t from = head + static_cast<int64_t>(j) * D;
+        const __half *k = P.k, *v = P.v;
+        if (P.nk && live && j >= sq.pos) {
+            from = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
+            k = P.nk;
+            v = P.nv;
+        }
+        const uint32_t to = dst + piece_at<D>(r, C::col(thread) / 8);
+        copy16(to, k + from + C::col(thread), live);
+        copy16(to + v_off, v + from + C::col(thread), live);
+    }
+}
+
 // What the warps of a CTA leave for its epilogue.
 struct StreamShared {
     float back[16], m[WARPS][16], l[WARPS][16];
@@ -56,29 +88,9 @@ __device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, 
     const int rows = P.n * P.G;
     const uint32_t q_s = s32(smem), ring = q_s + C::Q + warp * (C::SLOTS * C::SLOT);
     float* sm_o = reinterpret_cast<float*>(smem + C::Q);
-    const int64_t head = (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     auto request = [&](int i) {                                      // this warp's keys of the segment's i-th step
-        if (i < steps) {
-            constexpr int PIECES = D / 8;
-            const uint32_t dst = ring + i % C::SLOTS * C::SLOT;
-            const int place0 = (step0 + i) * STEP + warp * 16;
-#pragma unroll
-            for (int it = 0; it < PIECES / 2; ++it) {
-                const int r = (it * 32 + lane) / PIECES, c = (it * 32 + lane) % PIECES, place = place0 + r;
-                const bool live = place < sq.keys;
-                const int j = live ? sq.row_of(place) : 0;
-                int64_t at = head + static_cast<int64_t>(j) * D;
-                const __half *k = P.k, *v = P.v;
-                if (P.nk && live && j >= sq.pos) {
-                    at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
-                    k = P.nk;
-                    v = P.nv;
-                }
-                copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
-                copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
-            }
-        }
+        if (i < steps) request_span<D, 16, 32>(P, sq, b, kvh, (step0 + i) * STEP + warp * 16, ring + i % C::SLOTS * C::SLOT, C::TILE, lane);
         copy_commit();
     };
 #pragma unroll
@@ -110,7 +122,7 @@ __device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, 
         const uint32_t k_tile = ring + i % C::SLOTS * C::SLOT;
         if (place0 < sq.keys) {
             float s[2][4];
-            Rows<D>::template scores<1>(s, q_s, 0, k_tile, lane);
+            Rows<D>::template scores<1>(s, nullptr, q_s + Rows<D>::a_lane(lane), k_tile + Rows<D>::k_lane(lane));
             const bool whole = P.n == 1 && place0 + 16 <= sq.keys;   // one token sees every key of its spans
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -128,7 +140,7 @@ __device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, 
                         if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < sq.keys)
                             put(g + 8 * rr, place0 + 8 * n + 2 * t, make_float2(s[n][2 * rr], s[n][2 * rr + 1]));
             }
-            st.template take<1>(s, k_tile + C::TILE, lane);
+            st.template take<1>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
         }
         __syncwarp();                                                // the slot has been read: the next request may fill it
     }
@@ -182,79 +194,245 @@ __device__ __forceinline__ void append_rows(const Params& P, int b, int kvh, int
     }
 }
 
+// One place in a CTA's run of steps: a step of an item, i.e. of a (sequence, KV head).
+struct Cursor {
+    int b, kvh, step, steps;                                             // steps of the item
+    Seq sq;
+    __device__ __forceinline__ void enter(const Params& P) {             // sequence b, or the next that is not empty
+        for (; b < P.B; ++b) {
+            sq = seq_at(P, live_pos(P, b, false), 0, P.n);
+            steps = (sq.keys + STEP - 1) / STEP;
+            if (steps > 0) return;
+        }
+        b = P.B - 1;                                                     // (never, unless the positions change under the kernel)
+        sq.keys = 0;
+        steps = 1 << 30;
+    }
+    __device__ __forceinline__ void next_item(const Params& P) {
+        step = 0;
+        if (++kvh == P.KV_H) {
+            kvh = 0;
+            ++b;
+            enter(P);
+        }
+    }
+};
+
+// Columns of the outputs that the warps join at a time, and where: rows of 64 floats, groups of eight permuted so that a warp's stores of
+// eight rows spread over the banks.
+constexpr int JOIN_COLS = 64, JOIN_BYTES = WARPS * 16 * JOIN_COLS * 4;
+__device__ __forceinline__ int join_at(int w, int r, int c) { return (w * 16 + r) * JOIN_COLS + (c ^ ((r & 3) << 3)); }
+
+template <int D>
+struct RunCfg {
+    static constexpr int SLOTS = 3, TILE = 16 * D * 2, SLOT = 2 * TILE;
+    static constexpr int SMEM = JOIN_BYTES + WARPS * SLOTS * SLOT;       // the rows of q lie where the outputs are joined
+};
+
+// CTA `cta` of `ctas` over the steps of all items, an equal share each.  The rings run on from one item into the next.
 template <int D, bool SCORED, bool PREFIX>
-__global__ void __launch_bounds__(WARPS * 32) span_stream_kernel(const Params P) {
-    using C = StreamCfg<D>;
-    pdl_launch_dependents();
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int cum[MAX_BATCH + 1], seq_pos[MAX_BATCH];
+__device__ __forceinline__ void span_stream(const Params& P, int cta, int ctas) {
+    using C = RunCfg<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ StreamShared sh;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rows = P.n * P.G;
-    const float* sm_o = reinterpret_cast<const float*>(smem + C::Q);
-    pdl_wait();
-    if (warp == 0) {
+    const uint32_t q_s = s32(smem), ring = q_s + JOIN_BYTES + warp * (C::SLOTS * C::SLOT);
+    float* sm_o = reinterpret_cast<float*>(smem);
+    // steps before each sequence (every warp on its own): the total, then where this CTA's share begins
+    int total = 0, begin = 0, end = 0, b0 = 0, before = 0;
+    for (int pass = 0; pass < 2; ++pass) {
         int sum = 0;
-        if (lane == 0) cum[0] = 0;
-        for (int b0 = 0; b0 < P.B; b0 += 32) {
-            const int b = b0 + lane;
-            int x = 0;
-            if (b < P.B) {
-                const int pos = live_pos(P, b, blockIdx.x == 0);
-                seq_pos[b] = pos;
-                x = (seq_at(P, pos, 0, P.n).keys + STEP - 1) / STEP * P.KV_H;
-            }
+        for (int i0 = 0; i0 < P.B; i0 += 32) {
+            const int b = i0 + lane;
+            const int own = b < P.B ? (seq_at(P, live_pos(P, b, cta == 0 && pass == 0 && warp == 0), 0, P.n).keys + STEP - 1) / STEP * P.KV_H : 0;
+            int upto = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
             }
-            if (b < P.B) cum[b + 1] = sum + x;
-            sum += __shfl_sync(0xffffffffu, x, 31);
+            upto += sum;
+            if (pass == 1) {
+                if (cta == 0 && warp == 0 && b < P.B) P.cum[b + 1] = upto;
+                const uint32_t here = __ballot_sync(0xffffffffu, upto - own <= begin && begin < upto);
+                if (here) {
+                    b0 = i0 + __ffs(here) - 1;
+                    before = __shfl_sync(0xffffffffu, upto - own, __ffs(here) - 1);
+                }
+            }
+            sum = __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (pass == 0) {
+            total = sum;
+            const int per = steps_per_cta(total, ctas);
+            begin = min(total, cta * per);
+            end = min(total, begin + per);
         }
     }
-    __syncthreads();
-    const int total = cum[P.B], per = steps_per_cta(total, gridDim.x);
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= P.B; i += WARPS * 32) P.cum[i] = cum[i];
+    if (cta == 0 && threadIdx.x == 0) P.cum[0] = 0;
     if (P.nk) {
-        for (int i = blockIdx.x; i < P.B * P.KV_H; i += gridDim.x) {
-            const int b = i / P.KV_H;
-            if (seq_pos[b] >= 0) append_rows<D>(P, b, i - b * P.KV_H, seq_pos[b]);
+        for (int i = cta; i < P.B * P.KV_H; i += ctas) {
+            const int b = i / P.KV_H, pos = live_pos(P, b, false);
+            if (pos >= 0) append_rows<D>(P, b, i - b * P.KV_H, pos);
         }
     }
-    const int begin = min(total, static_cast<int>(blockIdx.x) * per), end = min(total, begin + per);
-    for (int s0 = begin; s0 < end;) {
-        int b = 0;
-        for (int hi = P.B; hi - b > 1;) {                                // the last sequence that begins at or before s0 and is not empty
-            const int mid = (b + hi) >> 1;
-            if (cum[mid] <= s0) b = mid;
-            else hi = mid;
+    const int count = end - begin;
+    if (count <= 0) return;
+    Cursor rq, at;                                                       // the next step to request, the next to work on
+    rq.b = b0;
+    rq.enter(P);
+    rq.kvh = (begin - before) / rq.steps;
+    rq.step = begin - before - rq.kvh * rq.steps;
+    at = rq;
+
+    int requested = 0, slot_rq = 0, slot_at = 0;
+    auto request = [&] {                                                 // this warp's sixteen keys of the next step
+        if (requested < count) {
+            request_span<D, 16, 32>(P, rq.sq, rq.b, rq.kvh, rq.step * STEP + warp * 16, ring + slot_rq * C::SLOT, C::TILE, lane);
+            slot_rq = slot_rq + 1 == C::SLOTS ? 0 : slot_rq + 1;
+            ++requested;
+            if (++rq.step == rq.steps && requested < count) rq.next_item(P);
         }
-        const int seq_steps = (cum[b + 1] - cum[b]) / P.KV_H, kvh = (s0 - cum[b]) / seq_steps, item = b * P.KV_H + kvh;
-        const int step0 = s0 - cum[b] - kvh * seq_steps, steps = min(seq_steps - step0, end - s0);
-        span_segment<D, SCORED>(P, sh, smem, b, kvh, seq_at(P, seq_pos[b], 0, P.n), step0, steps, [&](int r, int place, float2 s) {
-            *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + r) * P.pitch + place) = s;
-        });
-        const bool whole = steps == seq_steps;
-        const int64_t slot = whole ? 2 * gridDim.x + item : 2 * blockIdx.x + (s0 > begin);
-        for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
-            const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-            float top, l;
-            float4 acc = join_warps<D>(sh, sm_o, r, d, top, l);
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
-            acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            if (d == 0) P.part_lse[slot * 16 + r] = l == 0.f ? -INFINITY : top + log2f(l) - P_BIAS_LOG2;
-            if (whole && !PREFIX) {
-                const int tok = r / P.G, hg = r - tok * P.G;
-                store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + d, acc.x, acc.y, acc.z, acc.w);
-            } else {
-                *reinterpret_cast<float4*>(P.part_o + (slot * 16 + r) * D + d) = acc;
+        copy_commit();
+    };
+    QRow<D> qr[16 / WARPS];
+    auto read_q = [&](const Cursor& c) {
+#pragma unroll
+        for (int i = 0; i < 16 / WARPS; ++i) {
+            const int r = warp + i * WARPS, tok = r / P.G, hg = r - tok * P.G;
+            qr[i].read(P.q, c.b * P.q_bs + (c.kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, r < rows, lane);
+        }
+    };
+    auto put_q = [&] {
+#pragma unroll
+        for (int i = 0; i < 16 / WARPS; ++i) {
+            const int r = warp + i * WARPS;
+            const float f = qr[i].put([&](int d) { return q_s + piece_at<D>(r, d >> 3) + (d & 7) * 2; }, P.q_dtype, lane);
+            if (lane == 0) sh.back[r] = f * P.scale_log2;
+        }
+    };
+    // the query fragments stay in registers for an item (head_dim 256: the outputs leave no room, they are read anew for every step)
+    constexpr bool Q_REGS = D <= 128;
+    uint32_t qf[Q_REGS ? D / 16 : 1][4];
+    float scale[2];
+    auto take_q = [&] {
+        put_q();
+        __syncthreads();
+        scale[0] = sh.back[g];
+        scale[1] = sh.back[g + 8];
+        if constexpr (Q_REGS) Rows<D>::load_q(qf, q_s + Rows<D>::a_lane(lane));
+    };
+    read_q(at);
+#pragma unroll
+    for (int i = 0; i < C::SLOTS - 1; ++i) request();
+    take_q();
+
+    Rows<D> st;
+    st.clear();
+    int first = 0, first_step = at.step;                                 // of the segment: the share's step, the item's step
+    for (int i = 0; i < count; ++i) {
+        request();
+        copy_wait<C::SLOTS - 1>();
+        __syncwarp();
+        const int place0 = at.step * STEP + warp * 16;
+        const uint32_t k_tile = ring + slot_at * C::SLOT;
+        slot_at = slot_at + 1 == C::SLOTS ? 0 : slot_at + 1;
+        if (place0 < at.sq.keys) {
+            float s[2][4];
+            Rows<D>::template scores<1>(s, Q_REGS ? qf : nullptr, q_s + Rows<D>::a_lane(lane), k_tile + Rows<D>::k_lane(lane));
+            const bool whole = P.n == 1 && place0 + 16 <= at.sq.keys;    // one token sees every key of its spans
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int place = place0 + 8 * n + 2 * t + (e & 1);
+                    const bool seen = whole || (place < at.sq.keys && sees(P, at.sq.pos + (g + 8 * (e >> 1)) / P.G, at.sq.row_of(place)));
+                    s[n][e] = seen ? s[n][e] * scale[e >> 1] : -INFINITY;
+                }
+            if (SCORED) {
+                float* to = P.scores + static_cast<int64_t>(at.b * P.KV_H + at.kvh) * rows * P.pitch + place0 + 2 * t;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int rr = 0; rr < 2; ++rr)
+                        if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < at.sq.keys)
+                            *reinterpret_cast<float2*>(to + (g + 8 * rr) * P.pitch + 8 * n) = make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
+            }
+            st.template take<1>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
+        }
+        __syncwarp();                                                    // the slot has been read: the next request may fill it
+        if (++at.step < at.steps && i + 1 < count) continue;
+
+        // ---- the segment's end: the warps' results joined and stored, the next item's rows of q
+        Cursor next = at;
+        if (i + 1 < count) {
+            next.next_item(P);
+            read_q(next);
+        }
+        st.sum_lanes();
+        if (t == 0) {
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                sh.m[warp][g + 8 * rr] = st.m[rr];
+                sh.l[warp][g + 8 * rr] = st.l[rr];
             }
         }
-        __syncthreads();                                                 // the rings' memory is free again
-        s0 += steps;
+        __syncthreads();                                                 // every warp is done with q
+        const int item = at.b * P.KV_H + at.kvh;
+        const bool all = first_step == 0 && at.step == at.steps;
+        const int64_t slot = all ? 2 * ctas + item : 2 * cta + (first > 0);
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += JOIN_COLS) {
+            if (c0 > 0) __syncthreads();
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr)
+                if (g + 8 * rr < rows) {
+#pragma unroll
+                    for (int x = 0; x < JOIN_COLS / 8; ++x)
+                        *reinterpret_cast<float2*>(sm_o + join_at(warp, g + 8 * rr, 8 * x + 2 * t)) =
+                            make_float2(st.o[c0 / 8 + x][2 * rr], st.o[c0 / 8 + x][2 * rr + 1]);
+                }
+            __syncthreads();
+            for (int x = threadIdx.x; x < rows * (JOIN_COLS / 4); x += WARPS * 32) {
+                const int r = x / (JOIN_COLS / 4), d = x % (JOIN_COLS / 4) * 4;
+                float top = sh.m[0][r], l = 0.f;
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sh.m[w][r]);
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float f = sh.m[w][r] == -INFINITY && sh.l[w][r] == 0.f ? 0.f : ex2(sh.m[w][r] - top);
+                    const float4 o = *reinterpret_cast<const float4*>(sm_o + join_at(w, r, d));
+                    l = fmaf(f, sh.l[w][r], l);
+                    acc = make_float4(fmaf(f, o.x, acc.x), fmaf(f, o.y, acc.y), fmaf(f, o.z, acc.z), fmaf(f, o.w, acc.w));
+                }
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                if (c0 + d == 0) P.part_lse[slot * 16 + r] = l == 0.f ? -INFINITY : top + log2f(l) - P_BIAS_LOG2;
+                if (all && !PREFIX) {
+                    const int tok = r / P.G, hg = r - tok * P.G;
+                    store4(P.out, P.q_dtype, ((static_cast<int64_t>(at.b) * P.n + tok) * P.H + at.kvh * P.G + hg) * D + c0 + d, acc.x, acc.y, acc.z, acc.w);
+                } else {
+                    *reinterpret_cast<float4*>(P.part_o + (slot * 16 + r) * D + c0 + d) = acc;
+                }
+            }
+        }
+        if (i + 1 == count) break;
+        __syncthreads();                                                 // the join is over: q may lie there again
+        take_q();
+        at = next;
+        st.clear();
+        first = i + 1;
+        first_step = 0;
     }
+    copy_wait<0>();
+}
+template <int D, bool SCORED>
+__global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) span_stream_kernel(const Params P) {
+    pdl_launch_dependents();
+    pdl_wait();
+    span_stream<D, SCORED, false>(P, blockIdx.x, gridDim.x);
 }
 
 // Few (sequence, KV head)s of few keys: a cluster of CTAs each, joined through distributed shared memory, all in one launch.  The scored
@@ -282,7 +460,7 @@ template <int D, bool SCORED>
 __global__ void __launch_bounds__(WARPS * 32) span_cluster_kernel(const Params P) {
     using C = StreamCfg<D>;
     pdl_launch_dependents();
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ StreamShared sh;
     __shared__ float cta_m[16], cta_l[16], lse[16];
     const int item = blockIdx.y, b = item / P.KV_H, kvh = item - b * P.KV_H, rank = blockIdx.x, ranks = P.splits;
@@ -356,47 +534,45 @@ struct RowsCfg {
     static constexpr int SMEM = Q + STAGES * 2 * TILE;
 };
 
-// Grid (tiles * splits, KV_H, B).  PREFIX: rows of the whole batch over the shared prefix (grid z is 1), partial results only.
+// One CTA of a tile: `split` of `splits` CTAs that share its keys.  PREFIX: rows of the whole batch over the shared prefix, partial results only.
 template <int D, bool SCORED, bool PREFIX>
-__global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
+__device__ __forceinline__ void span_rows(const Params& P, int tile, int tiles, int split, int splits, int kvh, int b) {
     using C = RowsCfg<D>;
     constexpr int KT = C::KT;
-    pdl_launch_dependents();
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float back[64];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int splits = PREFIX ? P.pre_splits : P.splits, tiles = gridDim.x / splits;
-    const int split = blockIdx.x % splits, tile = tiles - 1 - blockIdx.x / splits;      // the rows with the most keys go first
-    const int kvh = blockIdx.y, b = blockIdx.z;
     const int rows = P.n * P.G, all_rows = PREFIX ? rows * P.B : rows, row0 = tile * 64;
     const uint32_t q_s = s32(smem), tiles_s = q_s + C::Q;
-    pdl_wait();
     const int tok0 = row0 / P.G, tok1 = min(P.n, (row0 + 63) / P.G + 1);                // of a chunk: the tokens of these rows
     Seq sq = {0, 0, 0, P.P};
     if (!PREFIX) sq = seq_at(P, live_pos(P, b, tile == 0 && kvh == 0 && split == 0 && threadIdx.x == 0), tok0, tok1);
     const int steps = (sq.keys + KT - 1) / KT, per = (steps + splits - 1) / splits;
     const int step0 = min(steps, split * per), step1 = min(steps, step0 + per);
-    const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
-    const __half *ck = PREFIX ? P.pk : P.k, *cv = PREFIX ? P.pv : P.v;
+    const int64_t head = (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     auto request = [&](int step) {
         if (step < step1) {
-            constexpr int PIECES = D / 8;
             const uint32_t dst = tiles_s + (step - step0) % C::STAGES * (2 * C::TILE);
-#pragma unroll
-            for (int it = 0; it < KT * PIECES / (WARPS * 32); ++it) {
-                const int i = it * (WARPS * 32) + threadIdx.x, r = i / PIECES, c = i % PIECES, place = step * KT + r;
-                const bool live = place < sq.keys;
-                const int j = live ? sq.row_of(place) : 0;
-                int64_t at = head + static_cast<int64_t>(j) * D;
-                const __half *k = ck, *v = cv;
-                if (!PREFIX && P.nk && live && j >= sq.pos) {
-                    at = b * P.n_bs + kvh * P.n_hs + (j - sq.pos) * P.n_ts;
-                    k = P.nk;
-                    v = P.nv;
+            if (!PREFIX) {
+                request_span<D, KT, WARPS * 32>(P, sq, b, kvh, step * KT, dst, C::TILE, threadIdx.x);
+            } else {
+                using Rq = Copy<D, KT, WARPS * 32>;
+                const int64_t at = kvh * P.p_hs + static_cast<int64_t>(step * KT + Rq::row(threadIdx.x)) * D + Rq::col(threadIdx.x);
+                if (step * KT + KT <= P.P) {
+                    Rq::rows(dst + Rq::place(threadIdx.x), P.pk + at);
+                    Rq::rows(dst + C::TILE + Rq::place(threadIdx.x), P.pv + at);
+                } else {
+#pragma unroll 2
+                    for (int i = 0; i < Rq::N; ++i) {
+                        const int r = Rq::row(threadIdx.x) + i * Rq::STRIDE;
+                        const bool live = step * KT + r < P.P;
+                        const int64_t from = live ? at + static_cast<int64_t>(i) * Rq::STRIDE * D : 0;
+                        const uint32_t to = dst + piece_at<D>(r, Rq::col(threadIdx.x) / 8);
+                        copy16(to, P.pk + from, live);
+                        copy16(to + C::TILE, P.pv + from, live);
+                    }
                 }
-                copy16(dst + piece_at<D>(r, c), k + at + c * 8, live);
-                copy16(dst + C::TILE + piece_at<D>(r, c), v + at + c * 8, live);
             }
         }
         copy_commit();
@@ -442,7 +618,7 @@ __global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
         __syncthreads();
         const uint32_t k_tile = tiles_s + (step - step0) % C::STAGES * (2 * C::TILE);
         float s[KT / 8][4];
-        Rows<D>::template scores<KT / 16>(s, q_s, warp * 16, k_tile, lane);
+        Rows<D>::template scores<KT / 16>(s, nullptr, q_s + warp * 16 * D * 2 + Rows<D>::a_lane(lane), k_tile + Rows<D>::k_lane(lane));
         const int place0 = step * KT;
         bool whole = place0 + KT <= sq.keys;
         if (!PREFIX && whole) {
@@ -474,7 +650,7 @@ __global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
                         *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + r_own[rr]) * P.pitch + place0 + 8 * n + 2 * t) =
                             make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
         }
-        st.template take<KT / 16>(s, k_tile + C::TILE, lane);
+        st.template take<KT / 16>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
         __syncthreads();                                                 // the tile has been read: its stage may be refilled
     }
     copy_wait<0>();
@@ -504,6 +680,31 @@ __global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
                 *reinterpret_cast<float2*>(po + (slot * 64 + r) * D + 8 * i + 2 * t) = make_float2(st.o[i][2 * rr] * inv, st.o[i][2 * rr + 1] * inv);
         }
     }
+}
+
+// Grid (tiles * splits, KV_H, B); the rows with the most keys go first.
+template <int D, bool SCORED>
+__global__ void __launch_bounds__(WARPS * 32) span_rows_kernel(const Params P) {
+    pdl_launch_dependents();
+    pdl_wait();
+    span_rows<D, SCORED, false>(P, P.tiles - 1 - blockIdx.x / P.splits, P.tiles, blockIdx.x % P.splits, P.splits, blockIdx.y, blockIdx.z);
+}
+// A shared prefix and the sequences' own keys in one launch: the first CTAs have the prefix, the last P.ctas the own keys (P.ctas 0: none,
+// they are many rows and have a launch of their own).
+template <int D>
+__global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) span_prefix_kernel(const Params P) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tiles = (P.B * P.n * P.G + 63) / 64, i = blockIdx.x, pre = static_cast<int>(gridDim.x) - P.ctas;
+    if (i < pre) span_rows<D, false, true>(P, i / P.pre_splits % tiles, tiles, i % P.pre_splits, P.pre_splits, i / (P.pre_splits * tiles), 0);
+    else span_stream<D, false, true>(P, i - pre, P.ctas);
+}
+// The own keys behind a prefix that the 5th-generation tensor cores have.
+template <int D>
+__global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) span_stream_prefix_kernel(const Params P) {
+    pdl_launch_dependents();
+    pdl_wait();
+    span_stream<D, false, true>(P, blockIdx.x, gridDim.x);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- joining
@@ -706,6 +907,9 @@ constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
 // Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
 constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
 
+// CTAs of the kernels for few rows that the GPU holds at once, by their shared memory.
+constexpr int resident_ctas(int D) { return SMS * (D == 64 ? 3 : (D == 128 ? 2 : 1)); }
+
 // How a call's work is laid out; a function of its sizes alone, so that the workspace's size is one too.
 struct Plan {
     bool stream;                         // few rows: span_stream_kernel
@@ -735,10 +939,12 @@ static int choose_splits(int64_t ctas, int64_t steps, int resident, int join) {
 
 static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int sinks, int P, bool scored) {
     Plan p = {};
+    if (n == 0) return p;
     const int64_t rows = static_cast<int64_t>(n) * (H / KV_H), items = static_cast<int64_t>(B) * KV_H;
     const int64_t seen = window > 0 && static_cast<int64_t>(window) + sinks + n < S ? static_cast<int64_t>(window) + sinks + n : S;
     p.stream = rows <= 16;
     size_t lse_rows, o_rows;
+    int64_t own_steps = 0;
     if (p.stream && P == 0) {
         const int64_t most = (seen + STEP - 1) / STEP;
         int ranks = 1;
@@ -752,8 +958,9 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     }
     if (p.stream) {
         const int64_t steps = items * ((seen + STEP - 1) / STEP), most = (steps + MIN_STEPS - 1) / MIN_STEPS;
-        const int resident = SMS * (D == 64 ? 3 : (D == 128 ? 2 : 1));
+        const int resident = resident_ctas(D);
         p.ctas = static_cast<int>(most < resident ? most : resident);
+        own_steps = steps;
         lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
     } else {
@@ -765,6 +972,24 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * tr;
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
+    if (P > 0) {
+        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_WORK;
+        const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
+        p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
+        const int64_t tiles = static_cast<int64_t>(p.pre_tiles) * KV_H, steps = (P + kt - 1) / kt;
+        if (p.stream && !p.pre_tc) {
+            // one launch: the resident CTAs are shared out by steps, an own step counted half (a cache is seldom full)
+            const int64_t resident = resident_ctas(D), share = resident * 2 * steps * tiles / (2 * steps * tiles + own_steps);
+            int64_t splits = (share + tiles - 1) / tiles;
+            if (splits > (steps + 1) / 2) splits = (steps + 1) / 2;
+            p.pre_splits = static_cast<int>(splits < 1 ? 1 : splits);
+            const int64_t rest = resident - p.pre_splits * tiles, least = resident / 4;
+            if (p.ctas > (rest > least ? rest : least)) p.ctas = static_cast<int>(rest > least ? rest : least);
+            lse_rows = o_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
+        } else {
+            p.pre_splits = choose_splits(tiles, steps, p.pre_tc ? SMS : 2 * SMS, 0);
+        }
+    }
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -775,10 +1000,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     p.part_lse = take(lse_rows * 4);
     p.part_o = take(o_rows * D * 4);
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_WORK;
-        const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
-        p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
-        p.pre_splits = choose_splits(static_cast<int64_t>(p.pre_tiles) * KV_H, (P + kt - 1) / kt, p.pre_tc ? SMS : 2 * SMS, 0);
+        const int tr = p.pre_tc ? 256 : 64;
         const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * tr;
         p.pre_lse = take(r * 4);
         p.pre_o = take(r * D * 4);
@@ -807,8 +1029,8 @@ static int allow_smem(K kern, int bytes, bool (&done)[64]) {
     return ALLOYB_OK;
 }
 template <typename K>
-static int launch(K kern, dim3 grid, int threads, int smem, bool (&done)[64], cudaStream_t st, const Params& P) {
-    const int rc = allow_smem(kern, smem, done);
+static int launch(K kern, dim3 grid, int threads, int smem, int most_smem, bool (&done)[64], cudaStream_t st, const Params& P) {
+    const int rc = allow_smem(kern, most_smem, done);
     if (rc != ALLOYB_OK) return rc;
     const cudaError_t e = launch_pdl(kern, grid, dim3(threads), smem, st, P);
     if (e != cudaSuccess) {
@@ -866,14 +1088,18 @@ static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
     const int items = P.B * P.KV_H, rows = P.n * P.G;
     int rc = ALLOYB_OK;
     if (!PREFIX && plan.cluster) return launch_cluster<D, SCORED>(plan, P, st);
+    constexpr int RUN = RunCfg<D>::SMEM, TILES = RowsCfg<D>::SMEM;
     if (PREFIX) {
-        const dim3 grid(plan.pre_tiles * plan.pre_splits, P.KV_H, 1);
-        rc = plan.pre_tc ? launch_span_tc(P, D, true, grid, st) : launch(span_rows_kernel<D, false, true>, grid, WARPS * 32, RowsCfg<D>::SMEM, ready[0], st, P);
+        const int ctas = plan.pre_tiles * plan.pre_splits * P.KV_H;
+        if (plan.pre_tc) rc = launch_span_tc(P, D, true, dim3(plan.pre_tiles * plan.pre_splits, P.KV_H, 1), st);
+        else rc = launch(span_prefix_kernel<D>, dim3(ctas + plan.ctas), WARPS * 32, plan.stream && RUN > TILES ? RUN : TILES, RUN > TILES ? RUN : TILES, ready[0], st, P);
+        if (rc == ALLOYB_OK && plan.stream && plan.pre_tc) rc = launch(span_stream_prefix_kernel<D>, dim3(plan.ctas), WARPS * 32, RUN, RUN, ready[3], st, P);
+    } else if (plan.stream) {
+        rc = launch(span_stream_kernel<D, SCORED>, dim3(plan.ctas), WARPS * 32, RUN, RUN, ready[1], st, P);
     }
-    if (rc != ALLOYB_OK) return rc;
-    if (plan.tc) rc = launch_span_tc(P, D, false, dim3(plan.tiles * plan.splits, P.KV_H, P.B), st);
-    else if (plan.stream) rc = launch(span_stream_kernel<D, SCORED, PREFIX>, dim3(plan.ctas), WARPS * 32, StreamCfg<D>::SMEM, ready[1], st, P);
-    else rc = launch(span_rows_kernel<D, SCORED, false>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, RowsCfg<D>::SMEM, ready[2], st, P);
+    if (rc == ALLOYB_OK && !plan.stream)
+        rc = plan.tc ? launch_span_tc(P, D, false, dim3(plan.tiles * plan.splits, P.KV_H, P.B), st)
+                     : launch(span_rows_kernel<D, SCORED>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, TILES, TILES, ready[2], st, P);
     if (rc != ALLOYB_OK) return rc;
     if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
     const int more = SCORED ? (P.S + WEIGHT_KEYS - 1) / WEIGHT_KEYS : 0;

@@ -108,6 +108,21 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 template <int D>
 __device__ __forceinline__ uint32_t piece_at(int r, int c) { return r * (D * 2) + ((c ^ (r & 7)) << 4); }
 
+// Sixteen rows (a warp) or 64 rows and more (a CTA of `lanes` threads) of a tile, from rows that lie in one piece.  at: address of the first row plus this
+// thread's piece; dst: the tile.  Everything but the row is a constant of the thread, and the rows' distances are offsets of the instruction.
+template <int D, int ROWS, int LANES>
+struct Copy {
+    static constexpr int PIECES = D / 8, STRIDE = LANES / PIECES, N = ROWS / STRIDE;       // rows apart, copies of a thread
+    __device__ __forceinline__ static int row(int thread) { return thread / PIECES; }
+    __device__ __forceinline__ static int col(int thread) { return thread % PIECES * 8; }
+    __device__ __forceinline__ static uint32_t place(int thread) { return piece_at<D>(row(thread), thread % PIECES); }
+    __device__ __forceinline__ static void rows(uint32_t dst, const __half* at) {          // dst: the tile plus place()
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((dst ^ ((i * STRIDE & 7) << 4)) + i * STRIDE * D * 2), "l"(at + i * STRIDE * D) : "memory");
+    }
+};
+
 // Four consecutive outputs, each rounded once from fp32.
 __device__ __forceinline__ void store4(void* out, int dtype, int64_t i, float a, float b, float c, float d) {
     uint2 w;
@@ -199,29 +214,41 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
-    // S = Q K^T of the tile at k_tile (rows of D halves, piece_at order); the query fragments are read where they are used
+    // A lane's place in a 16 x 16 block of a tile (rows of D halves, piece_at order), as an A operand, a B operand (K) and a transposed B operand
+    // (V).  Block c along the row is the same place with c << 5 exclusive-ored in: tiles begin on a multiple of their row's bytes.
+    __device__ __forceinline__ static uint32_t a_lane(int lane) { return piece_at<D>((lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) & 1); }
+    __device__ __forceinline__ static uint32_t k_lane(int lane) { return piece_at<D>((lane & 7) + ((lane >> 4) & 1) * 8, (lane >> 3) & 1); }
+    __device__ __forceinline__ static uint32_t v_lane(int lane) { return piece_at<D>((lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) & 1); }
+    __device__ __forceinline__ static void load_q(uint32_t (&q)[D / 16][4], uint32_t q_at) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) ldsm_x4(q_at ^ (kk << 5), q[kk]);
+    }
+    // S = Q K^T; k_at: the tile's address plus k_lane.  q: the fragments, or (null) read from q_at as they are used
     template <int NK>
-    __device__ __forceinline__ static void scores(float (&s)[2 * NK][4], uint32_t q_tile, int q_row, uint32_t k_tile, int lane) {
-        const int ar = q_row + (lane & 7) + ((lane >> 3) & 1) * 8, ac = (lane >> 4) & 1;
-        const int br = (lane & 7) + ((lane >> 4) & 1) * 8, bc = (lane >> 3) & 1;
+    __device__ __forceinline__ static void scores(float (&s)[2 * NK][4], const uint32_t (*q)[4], uint32_t q_at, uint32_t k_at) {
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t a[4];
-            ldsm_x4(q_tile + piece_at<D>(ar, 2 * kk + ac), a);
+            if (q) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = q[kk][e];
+            } else {
+                ldsm_x4(q_at ^ (kk << 5), a);
+            }
 #pragma unroll
             for (int n2 = 0; n2 < NK; ++n2) {
                 uint32_t b[4];
-                ldsm_x4(k_tile + n2 * 16 * D * 2 + piece_at<D>(br, 2 * kk + bc), b);
+                ldsm_x4((k_at ^ (kk << 5)) + n2 * 16 * D * 2, b);
                 mma16816(s[2 * n2], a, b[0], b[1]);
                 mma16816(s[2 * n2 + 1], a, b[2], b[3]);
             }
         }
     }
-    // s: scores in the log2 frame, -inf where a row does not see the key.  A NaN score makes the row NaN.
+    // s: scores in the log2 frame, -inf where a row does not see the key (a NaN score makes the row NaN); v_at: the tile's address plus v_lane
     template <int NK>
-    __device__ __forceinline__ void take(float (&s)[2 * NK][4], uint32_t v_tile, int lane) {
+    __device__ __forceinline__ void take(float (&s)[2 * NK][4], uint32_t v_at) {
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n) {
@@ -253,7 +280,6 @@ struct Rows {
             l[0] *= alpha[0];
             l[1] *= alpha[1];
         }
-        const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = (lane >> 4) & 1;
 #pragma unroll
         for (int k2 = 0; k2 < NK; ++k2) {
             // P is rounded to fp16 once (2^-11 of each weight at most, the sum l is of the unrounded ones): an output's error from it
@@ -271,7 +297,7 @@ struct Rows {
 #pragma unroll
             for (int n2 = 0; n2 < D / 16; ++n2) {
                 uint32_t b[4];
-                ldsm_x4_t(v_tile + k2 * 16 * D * 2 + piece_at<D>(vr, 2 * n2 + vc), b);
+                ldsm_x4_t((v_at ^ (n2 << 5)) + k2 * 16 * D * 2, b);
                 mma16816(o[2 * n2], p, b[0], b[1]);
                 mma16816(o[2 * n2 + 1], p, b[2], b[3]);
             }
