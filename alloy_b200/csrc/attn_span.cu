@@ -12,8 +12,8 @@
 // a warp 16 of them, and tiles of 64 keys (32 at head_dim 256) that its warps share; the keys are split where the tiles alone leave SMs
 // empty.
 //
-// The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and the
-// merge launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
+// The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and a
+// last launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
 //
 // New tokens' rows: keys from `pos` on are read from new_k / new_v directly, and written to the cache by whoever; nobody reads them there
 // in the same launch.
@@ -48,6 +48,7 @@ __device__ __forceinline__ int steps_per_cta(int total, int ctas) { return max((
 template <int D, int ROWS, int LANES>
 __device__ __forceinline__ void request_span(const Params& P, const Seq& sq, int b, int kvh, int place0, uint32_t dst, uint32_t v_off, int thread) {
     using C = Copy<D, ROWS, LANES>;
+    if (place0 >= sq.keys) return;                                       // (a warp's share of a last step: nobody looks at it)
     const int64_t head = (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
     const int first = sq.row_of(place0);
     if (place0 + ROWS <= sq.keys && sq.row_of(place0 + ROWS - 1) == first + ROWS - 1 && (!P.nk || first + ROWS <= sq.pos)) {
@@ -324,7 +325,7 @@ __device__ __forceinline__ void span_stream(const Params& P, int cta, int ctas) 
         if constexpr (Q_REGS) Rows<D>::load_q(qf, q_s + Rows<D>::a_lane(lane));
     };
     read_q(at);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < C::SLOTS - 1; ++i) request();
     take_q();
 
@@ -709,9 +710,6 @@ __global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) 
 
 // ---------------------------------------------------------------------------------------------------------------- joining
 constexpr int MERGE_WARPS = 8;
-constexpr int WEIGHT_KEYS = 256;                                         // keys whose weights a CTA of the merge launch adds up
-constexpr int WIDE_PARTS = 24;                                           // partial results from which a row gets a CTA, not a warp
-
 // Where the partial results of row R of a (sequence, KV head) lie.
 struct Parts {
     int own, pre;                                                        // how many of the row's own keys, of the prefix
@@ -719,14 +717,14 @@ struct Parts {
     bool stored;                                                         // the output is there already
     __device__ __forceinline__ int64_t own_index(int i) const { return i == 0 ? own_first : own_at + i * own_step; }
 };
+// (steps: of the sequences before this one, of them and it, of all)
 template <bool STREAM>
-__device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
+__device__ __forceinline__ Parts parts_of(const Params& P, int b, int kvh, int R, const int (&steps)[3]) {
     Parts p;
     const bool prefix = P.pre_o != nullptr;
-    const int b = item / P.KV_H, kvh = item - b * P.KV_H;
+    const int item = b * P.KV_H + kvh;
     if (STREAM) {
-        const int c0 = P.cum[b], seq_steps = (P.cum[b + 1] - c0) / P.KV_H, total = P.cum[P.B], per = steps_per_cta(total, P.ctas);
-        const int first = c0 + kvh * seq_steps;
+        const int seq_steps = (steps[1] - steps[0]) / P.KV_H, per = steps_per_cta(steps[2], P.ctas), first = steps[0] + kvh * seq_steps;
         p.stored = false;
         if (seq_steps == 0) {
             p.own = 0;
@@ -753,148 +751,158 @@ __device__ __forceinline__ Parts parts_of(const Params& P, int item, int R) {
     return p;
 }
 
-// A running log-sum of log-sums, and the join of `lanes` neighbouring lanes' (a NaN stays one; -inf is nothing).
-struct LogSum {
-    float m = -INFINITY, l = 0.f;
-    __device__ __forceinline__ void add(float x) {
-        if (x == -INFINITY) return;
-        if (x > m) {
-            l = fmaf(l, ex2(m - x), 1.0f);
-            m = x;
-        } else {
-            l += ex2(x - m);
-        }
-    }
-    __device__ __forceinline__ float join(int lanes) {
-        for (int o = lanes >> 1; o > 0; o >>= 1) {
-            const float om = __shfl_xor_sync(0xffffffffu, m, o), ol = __shfl_xor_sync(0xffffffffu, l, o);
-            const float top = fmaxf(m, om);
-            if (top != -INFINITY) l = l * ex2(m - top) + ol * ex2(om - top);
-            else l += ol;
-            m = top;
-        }
-        return l == 0.f ? -INFINITY : m + log2f(l);
-    }
-};
-__device__ __forceinline__ float row_lse(const Params& P, const Parts& p, int first, int lanes) {
-    LogSum s;
-#pragma unroll 4
-    for (int i = first; i < p.own; i += lanes) s.add(__ldcg(P.part_lse + p.own_index(i)));
-#pragma unroll 4
-    for (int i = first; i < p.pre; i += lanes) s.add(__ldcg(P.pre_lse + p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows));
-    return s.join(lanes);
-}
-
-// Grid (CTAs for the rows + CTAs for the weights, sequences * KV heads); P.merge_team warps a row, 1 or all.
-template <int D, bool STREAM, bool SCORED>
+// Grid (CTAs for the rows, sequences * KV heads); P.merge_team warps a row, 1 or all.  The scored form keeps the rows' log-sums.
+template <int D, bool STREAM>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
     pdl_launch_dependents();
-    __shared__ float4 sm[D >= 128 || !SCORED ? MERGE_WARPS * D / 4 : WEIGHT_KEYS];   // rows: a warp's sums each; weights: a row group's each
-    __shared__ float sm_lse[64];
+    __shared__ float4 sm[MERGE_WARPS * D / 4];                           // a warp's sums each
+    __shared__ float sm_m[MERGE_WARPS], sm_l[MERGE_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, item = blockIdx.y, rows = P.n * P.G;
     const int b = item / P.KV_H, kvh = item - b * P.KV_H;
-    const int team = P.merge_team, row_ctas = (rows * team + MERGE_WARPS - 1) / MERGE_WARPS;
+    const int team = P.merge_team;
     pdl_wait();
+    int steps[3] = {0, 0, 0};
+    if (STREAM) {                                                        // asked for along with the position, not behind it
+        steps[0] = P.cum[b];
+        steps[1] = P.cum[b + 1];
+        steps[2] = P.cum[P.B];
+    }
     const int pos = live_pos(P, b, false);
-    if (static_cast<int>(blockIdx.x) < row_ctas) {
-        const int R = (blockIdx.x * MERGE_WARPS + warp) / team, w0 = warp % team;
-        if (R >= rows) return;                                           // (a whole CTA's row, or a warp's: nobody waits for it)
-        const Parts p = parts_of<STREAM>(P, item, R);
-        if (p.stored) return;
-        const float lse = row_lse(P, p, lane, 32);
-        float acc[D / 32];
+    const int R = (blockIdx.x * MERGE_WARPS + warp) / team, w0 = warp % team;
+    if (R >= rows) return;                                               // (a whole CTA's row, or a warp's: nobody waits for it)
+    const Parts p = parts_of<STREAM>(P, b, kvh, R, steps);
+    if (p.stored) {
+        if (P.row_lse && w0 == 0 && lane == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = __ldcg(P.part_lse + p.own_first);
+        return;
+    }
+    // one pass: every part's log-sum and outputs are asked for at once, the running maximum and sum follow
+    constexpr int E = D / 32 < 4 ? D / 32 : 4, PER = D / 32 / E;     // elements of a lane's access, accesses
+    float m = -INFINITY, l = 0.f, acc[D / 32];
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-        constexpr int E = D / 32 < 4 ? D / 32 : 4, PER = D / 32 / E;     // elements of a lane's access, accesses
-        auto add = [&](const float* lses, const float* os, int64_t at) {
-            const float x = __ldcg(lses + at);
-            if (x == -INFINITY) return;                                  // (an empty part's rows are zeros, or were never written)
-            const float w = ex2(x - lse);
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    auto add = [&](const float* lses, const float* os, int64_t at) {
+        const float x = __ldcg(lses + at);
+        float v[D / 32];
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                float v[E];
-                const float* src = os + at * D + (c * 32 + lane) * E;
-                if (E == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(src));
-                else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(src));
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[c * E + e] = fmaf(w, v[e], acc[c * E + e]);
-            }
-        };
-        if (pos >= 0) {
-#pragma unroll 4
-            for (int i = w0; i < p.own; i += team) add(P.part_lse, P.part_o, p.own_index(i));
-#pragma unroll 4
-            for (int i = w0; i < p.pre; i += team) add(P.pre_lse, P.pre_o, p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows);
+        for (int c = 0; c < PER; ++c) {
+            const float* src = os + at * D + (c * 32 + lane) * E;
+            if (E == 4) *reinterpret_cast<float4*>(v + c * E) = __ldcg(reinterpret_cast<const float4*>(src));
+            else *reinterpret_cast<float2*>(v + c * E) = __ldcg(reinterpret_cast<const float2*>(src));
         }
-        const int tok = R / P.G, hg = R - tok * P.G;
-        const int64_t out = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
-        if (team == 1) {
+        const bool live = x != -INFINITY;                            // (an empty part's outputs were never written)
+        const float top = fmaxf(m, x), f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = live ? ex2(x - top) : 0.f;
+        l = fmaf(l, f0, f1);
 #pragma unroll
-            for (int c = 0; c < PER; ++c) {
-                const int64_t at = out + (c * 32 + lane) * E;
-                if (E == 4) store4(P.out, P.q_dtype, at, acc[c * E], acc[c * E + 1], acc[c * E + 2 % E], acc[c * E + 3 % E]);
-                else store2(P.out, P.q_dtype, at, acc[c * E], acc[c * E + 1]);
-            }
-            return;
-        }
-        float* sm_o = reinterpret_cast<float*>(sm);
+        for (int e = 0; e < D / 32; ++e) acc[e] = acc[e] * f0 + (live ? f1 * v[e] : 0.f);
+        m = top;
+    };
+    if (pos >= 0) {
+#pragma unroll 4
+        for (int i = w0; i < p.own; i += team) add(P.part_lse, P.part_o, p.own_index(i));
+#pragma unroll 4
+        for (int i = w0; i < p.pre; i += team) add(P.pre_lse, P.pre_o, p.pre_at + static_cast<int64_t>(i) * P.pre_tile_rows);
+    }
+    const int tok = R / P.G, hg = R - tok * P.G;
+    const int64_t out = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+    if (team == 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (P.row_lse && lane == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = l == 0.f ? -INFINITY : m + log2f(l);
 #pragma unroll
-        for (int c = 0; c < PER; ++c)
-#pragma unroll
-            for (int e = 0; e < E; ++e) sm_o[warp * D + (c * 32 + lane) * E + e] = acc[c * E + e];
-        __syncthreads();
-        if (threadIdx.x < D / 4) {
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < MERGE_WARPS; ++w) {
-                const float4 v = sm[w * (D / 4) + threadIdx.x];
-                sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
-            }
-            store4(P.out, P.q_dtype, out + threadIdx.x * 4, sum.x, sum.y, sum.z, sum.w);
+        for (int c = 0; c < PER; ++c) {
+            const int64_t at = out + (c * 32 + lane) * E;
+            if (E == 4) store4(P.out, P.q_dtype, at, acc[c * E] * inv, acc[c * E + 1] * inv, acc[c * E + 2 % E] * inv, acc[c * E + 3 % E] * inv);
+            else store2(P.out, P.q_dtype, at, acc[c * E] * inv, acc[c * E + 1] * inv);
         }
         return;
     }
-    if (SCORED) {
-        // weights of WEIGHT_KEYS positions: four groups of rows, a thread four keys; the rows' probabilities are summed in a fixed order
-        const int first_key = (blockIdx.x - row_ctas) * WEIGHT_KEYS, len = pos + P.n;
-        if (pos < 0 || first_key >= len) return;
-        const int group = threadIdx.x >> 6, j0 = first_key + (threadIdx.x & 63) * 4;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r0 = 0; r0 < rows; r0 += 64) {
-            __syncthreads();
-            {
-                const int r = threadIdx.x >> 2;
-                float lse = 0.f;
-                if (r0 + (r & ~7) < rows) lse = row_lse(P, parts_of<STREAM>(P, item, min(r0 + r, rows - 1)), threadIdx.x & 3, 4);    // (a warp's eight rows)
-                if ((threadIdx.x & 3) == 0) sm_lse[r] = lse;
-            }
-            __syncthreads();
-            if (j0 < len) {
-                const float* src = P.scores + (static_cast<int64_t>(item) * rows + r0) * P.pitch + j0;
-                const int count = min(64, rows - r0);
-#pragma unroll 8
-                for (int r = group; r < count; r += 4) {
-                    // a key behind the row's last position has no score where its tile was not this row's
-                    const float4 s = __ldcg(reinterpret_cast<const float4*>(src + r * P.pitch));
-                    const int row_pos = pos + (r0 + r) / P.G;
-                    const float lse = sm_lse[r];
-                    const float x[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j0 + e <= row_pos) sum[e] += ex2(x[e] - lse);
-                }
-            }
-        }
-        sm[threadIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-        __syncthreads();
-        const int j = first_key + threadIdx.x;                           // a key each
-        if (j >= len) return;
-        const float* parts = reinterpret_cast<const float*>(sm) + threadIdx.x;
-        float w = (parts[0] + parts[WEIGHT_KEYS]) + (parts[2 * WEIGHT_KEYS] + parts[3 * WEIGHT_KEYS]);
-        float* to = P.weights + static_cast<int64_t>(item) * P.S + j;
-        if (j < pos) w += *to;
-        *to = w;
+    float* sm_o = reinterpret_cast<float*>(sm);
+    if (lane == 0) {
+        sm_m[warp] = m;
+        sm_l[warp] = l;
     }
+#pragma unroll
+    for (int c = 0; c < PER; ++c)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sm_o[warp * D + (c * 32 + lane) * E + e] = acc[c * E + e];
+    __syncthreads();
+    if (threadIdx.x < D / 4) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, sm_m[w]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < MERGE_WARPS; ++w) {
+            const float4 v = sm[w * (D / 4) + threadIdx.x];
+            const float f = sm_m[w] == -INFINITY && sm_l[w] == 0.f ? 0.f : ex2(sm_m[w] - top);
+            sum = fmaf(f, sm_l[w], sum);
+            x = make_float4(fmaf(f, v.x, x.x), fmaf(f, v.y, x.y), fmaf(f, v.z, x.z), fmaf(f, v.w, x.w));
+        }
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        if (P.row_lse && threadIdx.x == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = sum == 0.f ? -INFINITY : top + log2f(sum);
+        store4(P.out, P.q_dtype, out + threadIdx.x * 4, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    }
+}
+
+// The weights of the scored form, once the rows' log-sums are known: a thread adds up four keys' probabilities, of up to 16 rows all, of more
+// rows (MANY) a quarter, in a fixed order.  Grid (key chunks, sequences * KV heads).
+template <bool MANY>
+struct Weights {
+    static constexpr int THREADS = 256, GROUPS = MANY ? 4 : 1, KEYS = THREADS * 4 / GROUPS;
+};
+template <bool MANY>
+__global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
+    using W = Weights<MANY>;
+    pdl_launch_dependents();
+    __shared__ float4 sm[MANY ? W::THREADS : 1];
+    const int item = blockIdx.y, rows = P.n * P.G, first_key = blockIdx.x * W::KEYS, group = threadIdx.x / (W::KEYS / 4);
+    const int j0 = first_key + threadIdx.x % (W::KEYS / 4) * 4;
+    float* weights = P.weights + static_cast<int64_t>(item) * P.S;
+    const float* scores = P.scores + static_cast<int64_t>(item) * rows * P.pitch + j0;
+    const float* lse = P.row_lse + static_cast<int64_t>(item) * rows;
+    pdl_wait();
+    const int pos = live_pos(P, item / P.KV_H, false), len = pos + P.n;
+    if (pos < 0 || first_key >= len) return;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (j0 + 3 <= pos) {                                                 // every row sees the four keys
+#pragma unroll 8
+        for (int r = group; r < rows; r += W::GROUPS) {
+            const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + r * P.pitch));
+            const float x = __ldcg(lse + r);
+            sum[0] += ex2(s.x - x);
+            sum[1] += ex2(s.y - x);
+            sum[2] += ex2(s.z - x);
+            sum[3] += ex2(s.w - x);
+        }
+    } else if (j0 < len) {                                               // (a key behind the row's own position may have no score)
+        for (int r = group; r < rows; r += W::GROUPS) {
+            const float x = __ldcg(lse + r);
+            const int room = min(3, pos + r / P.G - j0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e <= room) sum[e] += ex2(__ldcg(scores + r * P.pitch + e) - x);
+        }
+    }
+    if (!MANY) {
+        if (P.S % 4 == 0 && reinterpret_cast<uintptr_t>(P.weights) % 16 == 0 && j0 + 3 < pos) {
+            float4* to = reinterpret_cast<float4*>(weights + j0);
+            const float4 was = *to;
+            *to = make_float4(was.x + sum[0], was.y + sum[1], was.z + sum[2], was.w + sum[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j0 + e < len) weights[j0 + e] = j0 + e < pos ? weights[j0 + e] + sum[e] : sum[e];
+        }
+        return;
+    }
+    sm[threadIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    const int j = first_key + threadIdx.x;                               // a key each
+    if (j >= len) return;
+    const float* parts = reinterpret_cast<const float*>(sm) + threadIdx.x;
+    float w = 0.f;
+#pragma unroll
+    for (int k = 0; k < W::GROUPS; ++k) w += parts[k * W::KEYS];
+    weights[j] = j < pos ? weights[j] + w : w;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -916,7 +924,7 @@ struct Plan {
     int cluster, cluster_steps;          // few rows, few steps: span_cluster_kernel with this many CTAs, of this many steps at most
     bool tc, pre_tc;                     // more rows, the own keys / the prefix: span_tc_kernel, not span_rows_kernel
     int ctas, splits, tiles, pre_splits, pre_tiles;
-    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;         // byte offsets in the workspace
+    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, row_lse, bytes;    // byte offsets in the workspace
     int64_t pitch;
 };
 
@@ -1008,6 +1016,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     if (scored) {
         p.pitch = (static_cast<int64_t>(S) + 3) / 4 * 4;
         p.scores = take(static_cast<size_t>(items) * rows * p.pitch * 4);
+        p.row_lse = take(static_cast<size_t>(items) * rows * 4);
     }
     p.bytes = at;
     return p;
@@ -1102,12 +1111,17 @@ static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
                      : launch(span_rows_kernel<D, SCORED>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, TILES, TILES, ready[2], st, P);
     if (rc != ALLOYB_OK) return rc;
     if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
-    const int more = SCORED ? (P.S + WEIGHT_KEYS - 1) / WEIGHT_KEYS : 0;
     Params M = P;
-    M.merge_team = plan.pre_splits + (plan.stream ? (plan.ctas + items - 1) / items + 1 : plan.splits) >= WIDE_PARTS ? MERGE_WARPS : 1;
-    auto merge = plan.stream ? span_merge_kernel<D, true, SCORED> : span_merge_kernel<D, false, SCORED>;
-    const int row_ctas = (rows * M.merge_team + MERGE_WARPS - 1) / MERGE_WARPS;
-    const cudaError_t e = launch_pdl(merge, dim3(row_ctas + more, items), dim3(MERGE_WARPS * 32), 0, st, M);
+    // a CTA a row where it has many parts, and the GPU holds all of them at once (16 sequences of 4 heads behind 4096 rows: 4 us sooner); else
+    // a warp a row (64 sequences of 8 heads: 12 us sooner)
+    const int64_t parts = plan.pre_splits + (plan.stream ? plan.ctas / items + 2 : plan.splits);
+    M.merge_team = parts > MERGE_WARPS && static_cast<int64_t>(rows) * items <= 8 * SMS ? MERGE_WARPS : 1;
+    auto merge = plan.stream ? span_merge_kernel<D, true> : span_merge_kernel<D, false>;
+    cudaError_t e = launch_pdl(merge, dim3((rows * M.merge_team + MERGE_WARPS - 1) / MERGE_WARPS, items), dim3(MERGE_WARPS * 32), 0, st, M);
+    if (e == cudaSuccess && SCORED) {
+        const int keys = plan.stream ? Weights<false>::KEYS : Weights<true>::KEYS;
+        e = launch_pdl(plan.stream ? span_weights_kernel<false> : span_weights_kernel<true>, dim3((P.S + keys - 1) / keys, items), dim3(256), 0, st, P);
+    }
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return ALLOYB_E_CUDA;
@@ -1137,6 +1151,11 @@ static int fill(Params& P, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_
     if (!q || !k || !v || !pos || !out || (nk != nullptr) != (nv != nullptr)) return ALLOYB_E_NULL;
     const int rc = sizes_ok(B, H, KV_H, D, n, S);
     if (rc != ALLOYB_OK) return rc;
+    // the stride of a dimension of one element says nothing
+    if (B == 1) q_bs = n_bs = 0;
+    if (H == 1) q_hs = 0;
+    if (KV_H == 1) n_hs = 0;
+    if (n <= 1) q_ts = n_ts = 0;
     if (pos_count != 1 && pos_count != B) return ALLOYB_E_SHAPE;
     if (q_dtype != ALLOYB_F16 && q_dtype != ALLOYB_BF16) return ALLOYB_E_DTYPE;
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(nk) | reinterpret_cast<uintptr_t>(nv)) % 16 ||
@@ -1172,6 +1191,7 @@ static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_
     }
     if (plan.pitch) {
         P.scores = reinterpret_cast<float*>(ws + plan.scores);
+        P.row_lse = reinterpret_cast<float*>(ws + plan.row_lse);
         P.pitch = plan.pitch;
     }
     return ALLOYB_OK;

@@ -759,24 +759,15 @@ def _on_device(fn):
     """Run an op on its first tensor's device (the kernels launch on the current one)."""
     @functools.wraps(fn)
     def run(t, *args):
-        if t.device.index == _current_device():
+        if t.get_device() == _current_device():
             return fn(t, *args)
         with torch.cuda.device(t.device):
             return fn(t, *args)
     return run
 
 
-def _together(dev: torch.device, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.device != dev:
-            raise ValueError(f"all tensors must be on {dev}, got one on {t.device}")
-
-
-def _strides3(t: torch.Tensor) -> tuple[int, int, int]:
-    """Strides of the first three dimensions (0 where there is nothing to step over)."""
-    a, b, c, _ = t.stride()
-    na, nb, nc, _ = t.shape
-    return a if na > 1 else 0, b if nb > 1 else 0, c if nc > 1 else 0
+def _apart(*tensors: torch.Tensor) -> None:
+    raise ValueError(f"all tensors must be on one device, got {', '.join(str(t.device) for t in tensors)}")
 
 
 def _span_pos(pos: torch.Tensor, b: int) -> torch.Tensor:
@@ -816,53 +807,52 @@ def _span_refuse(q, new_k, new_v, k_cache, v_cache) -> None:
         raise ValueError("K and V caches must have the same shape")
     if s > k_cache.shape[2]:
         raise ValueError(f"{s} tokens do not fit a cache of {k_cache.shape[2]} rows")
+    raise ValueError("K and V caches must be (B, KV_H, S, D)")
+
+
+_F16, _BF16, _I32 = torch.float16, torch.bfloat16, torch.int32
 
 
 def _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv):
     """What the attention ops over spans of an fp16 cache share: checks, the output, and the leading arguments of their C entries.
-    (One decode step's call costs the host about as much as the device: the checks are one expression, taken apart only on failure.)"""
-    f16 = torch.float16
+    (One decode step's call costs the host more than the device, so the checks are one expression, taken apart only on failure.)"""
     dtype = q.dtype
-    row_shape, cache_shape = new_k.shape, k_cache.shape
-    if not (q.ndim == 4 and len(row_shape) == 4 and len(cache_shape) == 4):
+    if q.ndim != 4 or new_k.ndim != 4 or k_cache.ndim != 4:
         _span_refuse(q, new_k, new_v, k_cache, v_cache)
-        raise ValueError("K and V caches must be (B, KV_H, S, D)")
-    b, h, s, d = q.shape
-    kv_h = row_shape[1]
-    s_max = cache_shape[2]
-    if not ((dtype == f16 or dtype == torch.bfloat16) and (d == 128 or d == 64 or d == 256) and kv_h > 0 and h > 0 and h % kv_h == 0
-            and new_k.dtype == f16 and new_v.dtype == f16 and k_cache.dtype == f16 and v_cache.dtype == f16
-            and row_shape == (b, kv_h, s, d) and new_v.shape == row_shape and cache_shape[0] >= b and cache_shape[1] == kv_h
-            and cache_shape[3] == d and v_cache.shape == cache_shape and k_cache.is_contiguous() and v_cache.is_contiguous() and s <= s_max):
+    b, h, s, d = shape = q.shape
+    cb, kv_h, s_max, cd = cache_shape = k_cache.shape
+    if not ((dtype == _F16 or dtype == _BF16) and (d == 128 or d == 64 or d == 256) and kv_h > 0 and h > 0 and h % kv_h == 0
+            and cd == d and cb >= b and s <= s_max and new_k.dtype == new_v.dtype == k_cache.dtype == v_cache.dtype == _F16
+            and new_k.shape == new_v.shape == (b, kv_h, s, d) and v_cache.shape == cache_shape
+            and k_cache.is_contiguous() and v_cache.is_contiguous()):
         _span_refuse(q, new_k, new_v, k_cache, v_cache)
-    pos = _span_pos(cache_pos, b)
-    dev = q.device
-    _together(dev, new_k, new_v, pos, k_cache, v_cache)
-    if q.stride(3) != 1:
+    n = cache_pos.numel()
+    if (n != 1 and n != b) or cache_pos.dtype != _I32 or not cache_pos.is_contiguous():
+        cache_pos = _span_pos(cache_pos, b)
+    if not q.get_device() == new_k.get_device() == new_v.get_device() == cache_pos.get_device() == k_cache.get_device() == v_cache.get_device():
+        _apart(q, new_k, new_v, cache_pos, k_cache, v_cache)
+    q0, q1, q2, q3 = q.stride()
+    if q3 != 1:
         q = q.contiguous()
+        q0, q1, q2, q3 = q.stride()
+    k_at = v_at = None
+    n0 = n1 = n2 = 0
     if write_kv:
-        n0, n1, n2 = ns = _strides3(new_k)
+        n0, n1, n2, n3 = new_k.stride()
         k_at, v_at = new_k.data_ptr(), new_v.data_ptr()
-        if new_k.stride(3) != 1 or new_v.stride(3) != 1 or ns != _strides3(new_v) or (n0 | n1 | n2) % 8 or (k_at | v_at) % 16:
+        if n3 != 1 or new_v.stride() != (n0, n1, n2, 1) or (n0 | n1 | n2) & 7 or (k_at | v_at) & 15:
             new_k, new_v = (t.clone(memory_format=torch.contiguous_format) for t in (new_k, new_v))
+            n0, n1, n2 = kv_h * s * d, s * d, d
             k_at, v_at = new_k.data_ptr(), new_v.data_ptr()
-            n0, n1, n2 = _strides3(new_k)
-    else:
-        k_at = v_at = None
-        n0 = n1 = n2 = 0
-    out = q.new_empty((b, s, h, d))
-    return (out, (b, h, kv_h, d, s, s_max), (q.data_ptr(), *_strides3(q), _DTYPES[dtype]),
-            (k_at, v_at, n0, n1, n2, pos.data_ptr(), pos.numel()), (q, new_k, new_v, pos))
+    # (B, S, H, D) in memory, as the next linear reads it
+    out = q.new_empty_strided(shape, (s * h * d, d, h * d, 1))
+    return (out, (b, h, kv_h, d, s, s_max), (q.data_ptr(), q0, q1, q2, _DTYPES[dtype]), (k_at, v_at, n0, n1, n2, cache_pos.data_ptr(), n),
+            (q, new_k, new_v, cache_pos))
 
 
-def _span_workspace(out, *size):
-    """(address, bytes, the tensor that keeps it) of a call's workspace.  Every call has its own: calls on several streams, and graphs
-    that replay at the same time, share nothing."""
-    n = _span_workspace_bytes(*size)
-    if n == 0:
-        return None, 0, None
-    ws = torch.empty(n, dtype=torch.uint8, device=out.device)
-    return ws.data_ptr(), n, ws
+def _span_workspace(out, n: int):
+    """A call's workspace: every call has its own, so calls on several streams, and graphs that replay at the same time, share nothing."""
+    return torch.empty(n, dtype=torch.uint8, device=out.device)
 
 
 @torch.library.impl(lib, "attention_cache_window", "CUDA")
@@ -872,13 +862,18 @@ def _attention_cache_window(q, new_k, new_v, cache_pos, k_cache, v_cache, window
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
     if out.numel():
-        window, sinks = min(window, size[5]), min(sinks, size[5])
-        ws, n, _ws = _span_workspace(out, *size, window, sinks, 0, 0)
-        rc = _lib.load().alloyb_attn_window(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, window, sinks, scale, ws, n,
-                                            _stream())
+        s_max = size[5]
+        if window > s_max:
+            window = s_max
+        if sinks > s_max:
+            sinks = s_max
+        n = _span_workspace_bytes(*size, window, sinks, 0, 0)
+        ws = _span_workspace(out, n) if n else None
+        rc = _lib.load().alloyb_attn_window(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, window, sinks, scale,
+                                            ws.data_ptr() if n else None, n, _stream())
         if rc:
             check(rc, "alloyb_attn_window")
-    return out.transpose(1, 2)
+    return out
 
 
 @torch.library.impl(lib, "attention_shared_prefix", "CUDA")
@@ -887,78 +882,87 @@ def _attention_shared_prefix(q, new_k, new_v, cache_pos, prefix_k, prefix_v, k_c
     out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
     _, _, kv_h, d, _, _ = size
     for name, t in (("prefix_k", prefix_k), ("prefix_v", prefix_v)):
-        if t.dtype != torch.float16:
+        if t.dtype != _F16:
             raise TypeError(f"{name} must be float16, got {t.dtype}")
         if t.ndim != 3 or t.shape[0] != kv_h or t.shape[2] != d:
             raise ValueError(f"{name} must be ({kv_h}, P, {d}), got {tuple(t.shape)}")
-    if prefix_k.shape != prefix_v.shape:
+    shape = prefix_k.shape
+    if prefix_v.shape != shape:
         raise ValueError("prefix_k and prefix_v must have the same shape")
-    _together(q.device, prefix_k, prefix_v)
-    p = prefix_k.shape[1]
-
-    def dense_rows(t):
-        return t.stride(2) == 1 and (p <= 1 or t.stride(1) == d) and (kv_h == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= p * d)) and t.data_ptr() % 16 == 0
-
-    if not (dense_rows(prefix_k) and dense_rows(prefix_v) and prefix_k.stride(0) == prefix_v.stride(0)):
+    if not prefix_k.get_device() == prefix_v.get_device() == out.get_device():
+        _apart(q, prefix_k, prefix_v)
+    p = shape[1]
+    stride = p0, p1, p2 = prefix_k.stride()
+    pk_at, pv_at = prefix_k.data_ptr(), prefix_v.data_ptr()
+    # rows dense, heads any distance apart that 16-byte copies can step over
+    if prefix_v.stride() != stride or p2 != 1 or p1 != d or p0 < p * d or p0 & 7 or (pk_at | pv_at) & 15:
         prefix_k, prefix_v = (t.clone(memory_format=torch.contiguous_format) for t in (prefix_k, prefix_v))
+        p0 = p * d
+        pk_at, pv_at = prefix_k.data_ptr(), prefix_v.data_ptr()
     if out.numel():
-        ws, n, _ws = _span_workspace(out, *size, 0, 0, p, 0)
-        rc = _lib.load().alloyb_attn_shared_prefix(*head, prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(0) if kv_h > 1 else 0, p,
-                                                   k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size, scale, ws, n, _stream())
+        n = _span_workspace_bytes(*size, 0, 0, p, 0)
+        ws = _span_workspace(out, n) if n else None
+        rc = _lib.load().alloyb_attn_shared_prefix(*head, pk_at, pv_at, p0, p, k_cache.data_ptr(), v_cache.data_ptr(), *tail, out.data_ptr(), *size,
+                                                   scale, ws.data_ptr() if n else None, n, _stream())
         if rc:
             check(rc, "alloyb_attn_shared_prefix")
-    return out.transpose(1, 2)
+    return out
 
 
-def _check_weights(name, weights, cache):
+def _check_weights(name, weights, cache_shape):
     if weights.dtype != torch.float32:
         raise TypeError(f"{name} must be float32, got {weights.dtype}")
-    if weights.shape != cache.shape[:3] or not weights.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {tuple(cache.shape[:3])}, got {tuple(weights.shape)}")
+    if weights.shape != cache_shape[:3] or not weights.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {tuple(cache_shape[:3])}, got {tuple(weights.shape)}")
 
 
 @torch.library.impl(lib, "attention_cache_scored", "CUDA")
 @_on_device
 def _attention_cache_scored(q, new_k, new_v, cache_pos, k_cache, v_cache, weights, scale=-1.0, write_kv=True):
     out, size, head, tail, _keep = _span_args(q, new_k, new_v, cache_pos, k_cache, v_cache, write_kv)
-    _check_weights("weights", weights, k_cache)
-    _together(q.device, weights)
+    _check_weights("weights", weights, k_cache.shape)
+    if weights.get_device() != out.get_device():
+        _apart(q, weights)
     if out.numel():
-        ws, n, _ws = _span_workspace(out, *size, 0, 0, 0, 1)
-        rc = _lib.load().alloyb_attn_scored(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, weights.data_ptr(), out.data_ptr(), *size, scale, ws,
-                                            n, _stream())
+        n = _span_workspace_bytes(*size, 0, 0, 0, 1)
+        ws = _span_workspace(out, n) if n else None
+        rc = _lib.load().alloyb_attn_scored(*head, k_cache.data_ptr(), v_cache.data_ptr(), *tail, weights.data_ptr(), out.data_ptr(), *size, scale,
+                                            ws.data_ptr() if n else None, n, _stream())
         if rc:
             check(rc, "alloyb_attn_scored")
-    return out.transpose(1, 2)
+    return out
 
 
 @torch.library.impl(lib, "kv_evict", "CUDA")
 @_on_device
 def _kv_evict(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out, keep, sinks=0, recent=0):
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_out", k_out), ("v_out", v_out)):
-        if t.dtype != torch.float16:
-            raise TypeError(f"{name} must be float16, got {t.dtype}")
-        if t.ndim != 4 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous (B, KV_H, S, D), got {tuple(t.shape)}")
-    b, kv_h, s, d = k_cache.shape
-    if d not in (64, 128, 256):
+    if not k_cache.dtype == v_cache.dtype == k_out.dtype == v_out.dtype == _F16:
+        raise TypeError(f"caches must be float16, got {k_cache.dtype}, {v_cache.dtype}, {k_out.dtype}, {v_out.dtype}")
+    shape, out_shape = k_cache.shape, k_out.shape
+    if k_cache.ndim != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_out.is_contiguous() and v_out.is_contiguous()):
+        raise ValueError("caches must be contiguous (B, KV_H, S, D)")
+    b, kv_h, s, d = shape
+    if d != 128 and d != 64 and d != 256:
         raise NotImplementedError(f"built for head_dim 64, 128 and 256, got {d}")
-    s_out = k_out.shape[2]
-    if v_cache.shape != k_cache.shape or k_out.shape != (b, kv_h, s_out, d) or v_out.shape != k_out.shape:
+    if v_cache.shape != shape or k_out.ndim != 4 or out_shape != (b, kv_h, out_shape[2], d) or v_out.shape != out_shape:
         raise ValueError("K and V must have the same shape, and the outputs theirs but for the number of rows")
-    _check_weights("weights", weights, k_cache)
-    _check_weights("weights_out", weights_out, k_out)
+    s_out = out_shape[2]
+    _check_weights("weights", weights, shape)
+    _check_weights("weights_out", weights_out, out_shape)
     if keep < 1 or keep > s_out or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"need sinks + recent <= keep <= rows of the outputs, got {sinks} + {recent}, {keep}, {s_out}")
     lengths = _span_pos(lengths, b)
-    _together(k_cache.device, v_cache, weights, lengths, k_out, v_out, weights_out)
-    kept = torch.empty((b, kv_h, keep), dtype=torch.int32, device=k_cache.device)
-    new_lengths = torch.empty((b,), dtype=torch.int32, device=k_cache.device)
+    if not (k_cache.get_device() == v_cache.get_device() == weights.get_device() == lengths.get_device() == k_out.get_device() ==
+            v_out.get_device() == weights_out.get_device()):
+        _apart(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out)
+    kept = lengths.new_empty((b, kv_h, keep))
+    new_lengths = lengths.new_empty((b,))
     if k_cache.numel():
-        check(_lib.load().alloyb_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lengths.data_ptr(), lengths.numel(),
-                                          k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), kept.data_ptr(),
-                                          new_lengths.data_ptr(), b, kv_h, d, s, s_out, keep, sinks, recent, _stream()),
-              "alloyb_kv_evict")
+        rc = _lib.load().alloyb_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lengths.data_ptr(), lengths.numel(),
+                                         k_out.data_ptr(), v_out.data_ptr(), weights_out.data_ptr(), kept.data_ptr(), new_lengths.data_ptr(), b, kv_h,
+                                         d, s, s_out, keep, sinks, recent, _stream())
+        if rc:
+            check(rc, "alloyb_kv_evict")
     return kept, new_lengths
 
 
