@@ -908,9 +908,12 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
-// Rows of a KV head, and operations of a call, from which they go to the 5th-generation tensor cores.
+// Rows of a KV head, and operations (4 D rows keys, by the sizes of the call), from which the own keys / a prefix go to the 5th-generation tensor
+// cores.  Own keys, 32/8 heads, there / on mma.sync: 128 tokens of head_dim 128 over a window of 1024 (2.2e9) 31.3 / 29.6 us, 256 tokens (4.3e9)
+// 31.8 / 31.2, 128 tokens over 4096 (8.5e9) 34 / 45.  A prefix of 1024, 32/8 heads: 64 sequences of head_dim 128 (1.1e9) 38 / 37, 128 of
+// head_dim 64 (1.1e9) 38 / 40, 128 of head_dim 128 (2.2e9) 47 / 73.
 constexpr int TC_ROWS = 192;
-constexpr int64_t TC_WORK = 4000000000ll;
+constexpr int64_t TC_WORK = 4000000000ll, TC_PREFIX_WORK = 1500000000ll;
 constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
 // Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
 constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
@@ -981,7 +984,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_WORK;
+        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_PREFIX_WORK;
         const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
         const int64_t tiles = static_cast<int64_t>(p.pre_tiles) * KV_H, steps = (P + kt - 1) / kt;

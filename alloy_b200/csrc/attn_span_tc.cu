@@ -9,8 +9,9 @@
 //   in one piece (the first rows, the end of a sequence) come in by cp.async, places past the last key zero-filled: what a cache holds there
 //   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.  (All tiles by cp.async, and the new
 //   tokens' rows from their own tensors: 314 us for 2048 tokens behind 6000 under a window of 4096, 32/8 heads, head_dim 128.)
-// * Scores and output accumulators in tensor memory.  A thread owns a row and keeps its 128 scores in registers between the maximum and
-//   the exponentials; P (fp16, rounded once) overwrites the scores and is read from there as the A operand.
+// * Scores and output accumulators in tensor memory.  Two threads share a row, 64 scores each, which stay in registers between the maximum
+//   (exchanged through shared memory) and the exponentials; P (fp16, rounded once) overwrites the scores and is read from there as the A
+//   operand.
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
 #include <cuda.h>
@@ -24,7 +25,7 @@ using sp::Params;
 using sp::Seq;
 
 constexpr int ROWS = 256, KT = 128, STAGES = 2, AHEAD = 3;
-constexpr int THREADS = 12 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-7 and 8-11 are their softmax
+constexpr int THREADS = 20 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-11 and 12-19 are their softmax
 constexpr int HALF = 128 * 128;              // bytes of 128 rows x 64 halves
 constexpr uint32_t SPIN = 1u << 22;
 
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     constexpr int TILE = C::TILE, PIECES = D / 8;
     pdl_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
-    __shared__ float back[ROWS];
+    __shared__ float back[ROWS], half_max[2][ROWS], half_sum[ROWS];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t q_s = s32(smem), k_s = q_s + 2 * TILE, v_s = k_s + STAGES * TILE;
     Bars* bars = reinterpret_cast<Bars*>(smem + 2 * TILE + 2 * STAGES * TILE);
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         }
         for (int g = 0; g < 2; ++g) {
             bar_init(&bars->s_full[g], 1);
-            bar_init(&bars->p_full[g], 4);
+            bar_init(&bars->p_full[g], 8);
             bar_init(&bars->o_full[g], 1);
             bar_init(&bars->turn[g], 1);
         }
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     // ---- Q rows; dead rows are zero
-    constexpr int WARPS = THREADS / 32, BATCH = 11;
+    constexpr int WARPS = THREADS / 32, BATCH = 13;
     for (int i0 = 0; i0 * WARPS < ROWS; i0 += BATCH) {
         sp::QRow<D> qr[BATCH];
 #pragma unroll
@@ -327,20 +328,22 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
         }
     } else {
-        // ------------------------------------------------ softmax: a thread per row
-        const int g = (warp - 4) >> 2, r = g * 128 + (warp & 3) * 32 + lane;
+        // ------------------------------------------------ softmax: two threads a row, the one the first half of a tile's keys, one the second
+        constexpr int COLS = KT / 2;
+        const int g = (warp - 4) >> 3, half = (warp >> 2) & 1 ^ 1, r = g * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * C::COLS;
+        const int pair = 1 + g * 4 + (warp & 3);                              // named barrier of the two warps that share rows
         const int R = row0 + r, pos = sq.pos + R / P.G;                       // (of a chunk) last row of the cache that this one may see
         const int first = sq.pos + (R - lane) / P.G, last = sq.pos + (R - lane + 31) / P.G;
         const float scale = back[r];
-        float m_run = -INFINITY, l_run = 0.f;                                 // (l times 64, like the accumulators)
+        float m_run = -INFINITY, l_run = 0.f;                                 // (l: of this half, times 64 like the accumulators)
         for (int j = 0; j < n_tiles; ++j) {
             const int place0 = (step0 + j) * KT;
             bar_wait(ok, &bars->s_full[g], j & 1);
             fence_after();
-            float s[KT];
+            float s[COLS];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(lanes + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+            for (int c = 0; c < 2; ++c) tmem_ld32(lanes + half * COLS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
             wait_ld();
             bool whole = place0 + KT <= sq.keys;                              // (uniform in the warp)
             if (!PREFIX && whole) {
@@ -348,11 +351,11 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 whole = j1 <= first && (P.window <= 0 || (place0 >= sq.sink && j0 > last - P.window) || place0 + KT <= sq.sink);
             }
             if (!whole) {
-                // place e of the tile is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
-                const int hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - place0;
-                const int lo = PREFIX || P.window <= 0 ? -1 : pos - P.window - sq.lo + sq.sink - place0, sk = PREFIX ? 0 : P.sinks - place0;
+                // place e of this half is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
+                const int at = place0 + half * COLS, hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - at;
+                const int lo = PREFIX || P.window <= 0 ? -1 : pos - P.window - sq.lo + sq.sink - at, sk = PREFIX ? 0 : P.sinks - at;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     const uint32_t seen = sp::bits_below(hi + 1 - 32 * c) & (~sp::bits_below(lo + 1 - 32 * c) | sp::bits_below(sk - 32 * c));
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -361,10 +364,15 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < KT; e += 8)
+            for (int e = 0; e < COLS; e += 8)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], s[e + k], s[e + 4 + k]);
-            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
+            float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
+            // the other half's maximum.  Behind the barrier both halves' scores are in registers, and P may overwrite them; the next tile's
+            // scores, and with them the next write to half_max, come behind both halves' P
+            half_max[half][r] = mx;
+            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+            mx = fmaxf(mx, half_max[half ^ 1][r]);
             const bool grow = mx > m_run + sp::RESCALE_LOG2;
             if (__any_sync(0xffffffffu, grow)) {
                 const float alpha = grow ? ex2(m_run - mx) : 1.0f;
@@ -372,14 +380,15 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 l_run *= alpha;
                 if (j > 0) {                                                  // (these scores came behind the last P V, which is complete)
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
+                    for (int c = 0; c < D / 32; ++c) {
                         float o[16];
                         uint32_t w[16];
-                        tmem_ld16(lanes + 128 + c * 16, o);
+                        const uint32_t at = lanes + 128 + half * (D / 2) + c * 16;
+                        tmem_ld16(at, o);
                         wait_ld();
 #pragma unroll
                         for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * alpha);
-                        tmem_st16(lanes + 128 + c * 16, w);
+                        tmem_st16(at, w);
                     }
                     wait_st();
                 }
@@ -388,17 +397,18 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             const uint64_t scale2 = f2(scale, scale), sub2 = f2(sub, sub);
             uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     float x0, x1;
                     unf2(f2_fma(f2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, sub2), x0, x1);
-                    const float p0 = ex2(x0), p1 = ex2(x1);
-                    sum[e & 1] = f2_add(sum[e & 1], f2(p0, p1));
-                    p[e] = pack_h2(p0, p1);
+                    x0 = ex2(x0);
+                    x1 = ex2(x1);
+                    sum[e & 1] = f2_add(sum[e & 1], f2(x0, x1));
+                    p[e] = pack_h2(x0, x1);
                 }
-                tmem_st16(lanes + c * 16, p);
+                tmem_st16(lanes + half * (COLS / 2) + c * 16, p);
             }
             float a0, a1, b0, b1;
             unf2(sum[0], a0, a1);
@@ -409,7 +419,15 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             __syncwarp();
             if (lane == 0) bar_arrive(&bars->p_full[g]);
         }
-        // ---- normalise and store
+        // ---- normalise and store, half of the columns each
+        if (half == 1) half_sum[r] = l_run;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        if (half == 0) {
+            l_run += half_sum[r];
+            half_sum[r] = l_run;
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        l_run = half_sum[r];
         if (n_tiles > 0) {
             bar_wait(ok, &bars->o_full[g], 0);
             fence_after();
@@ -418,12 +436,12 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         const bool row_live = ok && R < all_rows, direct = !PREFIX && splits == 1 && P.pre_o == nullptr;
         const int tok = R / P.G, hg = R - tok * P.G;
         const int64_t slot = ((static_cast<int64_t>(PREFIX ? 0 : b) * P.KV_H + kvh) * tiles + tile) * splits + split;
-        if (row_live && !direct)
+        if (row_live && !direct && half == 0)
             (PREFIX ? P.pre_lse : P.part_lse)[slot * ROWS + r] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run) - sp::P_BIAS_LOG2;
         float* po = (PREFIX ? P.pre_o : P.part_o) + (slot * ROWS + r) * D;
         const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
             float o[32];
             if (n_tiles > 0) {
                 tmem_ld32(lanes + 128 + c * 32, o);
