@@ -914,9 +914,13 @@ constexpr int SMS = 148;
 // head_dim 64 (1.1e9) 38 / 40, 128 of head_dim 128 (2.2e9) 47 / 73.
 constexpr int TC_ROWS = 192;
 constexpr int64_t TC_WORK = 4000000000ll, TC_PREFIX_WORK = 1500000000ll;
-constexpr int CLUSTER_MAX = 16, CLUSTER_CTAS = 2 * SMS, CLUSTER_STEPS = 8;
-// Rows times steps whose scores a CTA of the cluster kernel keeps (256 bytes each), next to its rings.
-constexpr int cluster_scores(int D) { return D == 256 ? 64 : 128; }
+// One launch of clusters, or the stream kernel and the join: as long as a CTA has 16 steps at most and all CTAs run at once.  Captured in a graph,
+// 32/8 heads, clusters / stream: head_dim 128, one sequence of 4000 keys 10.3 / 11.3 us, 4 of 2000 10.1 / 14.2, 16 of 1000 13.9 / 18.7, 32 of 1000
+// 25.8 / 29.2, 64 of 500 (more CTAs than at once) stays 30.6; head_dim 64, 8 of 1000 8.2 / 13.8.  Clusters of 16 find room in a GPC only where an SM holds
+// two of its CTAs, and then one a GPC: 2 sequences of 4000 keys at head_dim 128 took 19.4 us in sixteens, 13.4 streamed; with one CTA an SM, also
+// those of 8 only as many as there are GPCs.
+constexpr int CLUSTER_MAX = 16, CLUSTER_STEPS = 16, SM_SMEM = 228 * 1024;
+constexpr size_t cluster_smem(int D) { return D == 64 ? StreamCfg<64>::SMEM : (D == 128 ? StreamCfg<128>::SMEM : StreamCfg<256>::SMEM); }
 
 // CTAs of the kernels for few rows that the GPU holds at once, by their shared memory.
 constexpr int resident_ctas(int D) { return SMS * (D == 64 ? 3 : (D == 128 ? 2 : 1)); }
@@ -957,11 +961,15 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     size_t lse_rows, o_rows;
     int64_t own_steps = 0;
     if (p.stream && P == 0) {
+        // as many CTAs a (sequence, KV head) as there are steps for, the GPU holds at once and clusters may have
         const int64_t most = (seen + STEP - 1) / STEP;
-        int ranks = 1;
-        while (ranks < CLUSTER_MAX && ranks < most) ranks *= 2;
-        const int64_t per = (most + ranks - 1) / ranks;
-        if (items * ranks <= CLUSTER_CTAS && per <= CLUSTER_STEPS && (!scored || rows * per <= cluster_scores(D))) {
+        for (int ranks = CLUSTER_MAX; ranks >= 1; ranks /= 2) {
+            const int64_t per = (most + ranks - 1) / ranks;
+            const size_t smem = cluster_smem(D) + (scored ? rows * per * STEP * 4 : 0);
+            const int64_t ctas = static_cast<int64_t>((SM_SMEM - 1) / (smem + 2048));           // of an SM (a little kept by the kernel and by the GPU)
+            if (ranks / 2 >= most || per > CLUSTER_STEPS || ctas < 1 || items * ranks > SMS * ctas) continue;
+            if (ranks == 16 && (items > 8 * (ctas - 1) || per > CLUSTER_STEPS / 2)) continue;
+            if (ranks == 8 && ctas == 1 && items > 8) continue;
             p.cluster = ranks;
             p.cluster_steps = static_cast<int>(per);
             return p;
@@ -1056,8 +1064,8 @@ template <int D, bool SCORED>
 static int launch_cluster(const Plan& plan, const Params& P, cudaStream_t st) {
     static bool ready[64] = {}, wide[64] = {};
     auto kern = span_cluster_kernel<D, SCORED>;
-    const int rows = P.n * P.G, extra = SCORED ? rows * plan.cluster_steps * STEP * 4 : 0;
-    int rc = allow_smem(kern, StreamCfg<D>::SMEM + (SCORED ? cluster_scores(D) * STEP * 4 : 0), ready);
+    const int extra = SCORED ? P.n * P.G * plan.cluster_steps * STEP * 4 : 0;
+    int rc = allow_smem(kern, SM_SMEM - 3 * 1024, ready);
     if (rc != ALLOYB_OK) return rc;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
