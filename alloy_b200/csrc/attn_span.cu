@@ -4,19 +4,22 @@
 //
 // Few rows (one token, or as many as give 16 rows of a KV head; span_stream_kernel).  Bound: HBM, 4 D bytes a key for 4 D G n operations.
 // Every sequence's keys are cut into steps of 64, all sequences' steps laid end to end and dealt out evenly to as many CTAs as the GPU
-// holds at once, whatever the lengths: a CTA may finish one sequence and begin the next.  A warp takes 16 of a step's keys through a ring
-// of its own (cp.async, no barrier but its own), S and P V on mma.sync with the rows padded to 16.  A (sequence, KV head) that one CTA
-// covers is stored by it; the others' partial results go to a workspace and span_merge_kernel joins them.
+// holds at once, whatever the lengths: a CTA may finish one sequence and begin the next, and its rings of tiles run on.  A warp takes 16 of a
+// step's keys through a ring of its own (cp.async, three tiles of K and V, no barrier but its own), S and P V on mma.sync with the rows
+// padded to 16.  A (sequence, KV head) that one CTA covers is stored by it; the others' partial results go to a workspace and
+// span_merge_kernel joins them.  32 sequences of 4096 keys each at positions 2000 .. 16300, 32/8 heads, head_dim 128: 91 us = 5.7 TB/s.
+// Where there is little to do, clusters that join through distributed shared memory do it in one launch (span_cluster_kernel).
 //
 // More rows (chunks, and all the batch's rows over a shared prefix; span_rows_kernel).  Bound: mma.sync.  A CTA owns 64 (token, head) rows,
 // a warp 16 of them, and tiles of 64 keys (32 at head_dim 256) that its warps share; the keys are split where the tiles alone leave SMs
-// empty.
+// empty.  Tiles of 32 keys and three CTAs an SM were slower (4 x 16 tokens looking back over 5000 to 8100 keys: 68 -> 81 us), a third stage gave
+// nothing.  Many rows with much to do go to attn_span_tc.cu.
 //
 // The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and a
 // last launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
 //
-// New tokens' rows: keys from `pos` on are read from new_k / new_v directly, and written to the cache by whoever; nobody reads them there
-// in the same launch.
+// New tokens' rows: keys from `pos` on are read from new_k / new_v, by every CTA that needs them, and written to the cache by one; nobody reads
+// them there in the same launch.
 #include "attn_span.cuh"
 
 namespace alloyb {
@@ -244,9 +247,10 @@ __device__ __forceinline__ void span_stream(const Params& P, int cta, int ctas) 
     int total = 0, begin = 0, end = 0, b0 = 0, before = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int sum = 0;
+        int next = lane < P.B ? live_pos(P, lane, cta == 0 && pass == 0 && warp == 0) : -1;
         for (int i0 = 0; i0 < P.B; i0 += 32) {
-            const int b = i0 + lane;
-            const int own = b < P.B ? (seq_at(P, live_pos(P, b, cta == 0 && pass == 0 && warp == 0), 0, P.n).keys + STEP - 1) / STEP * P.KV_H : 0;
+            const int b = i0 + lane, own = (seq_at(P, next, 0, P.n).keys + STEP - 1) / STEP * P.KV_H;
+            next = b + 32 < P.B ? live_pos(P, b + 32, cta == 0 && pass == 0 && warp == 0) : -1;      // (asked for a round ahead)
             int upto = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(WARPS * 32) span_cluster_kernel(const Params P
             const int j = step0 * STEP + i;
             float sum = 0.f;
             for (int r = 0; r < rows; ++r) sum += ex2(sm_s[r * (P.tiles * STEP) + i] - lse[r]);
-            if (j < pos) sum += w[j];
+            if (j < pos) sum += __ldcg(w + j);
             w[j] = sum;
         }
     }
@@ -763,9 +767,9 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
     pdl_wait();
     int steps[3] = {0, 0, 0};
     if (STREAM) {                                                        // asked for along with the position, not behind it
-        steps[0] = P.cum[b];
-        steps[1] = P.cum[b + 1];
-        steps[2] = P.cum[P.B];
+        steps[0] = __ldcg(P.cum + b);
+        steps[1] = __ldcg(P.cum + b + 1);
+        steps[2] = __ldcg(P.cum + P.B);
     }
     const int pos = live_pos(P, b, false);
     const int R = (blockIdx.x * MERGE_WARPS + warp) / team, w0 = warp % team;
@@ -885,12 +889,12 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
     if (!MANY) {
         if (P.S % 4 == 0 && reinterpret_cast<uintptr_t>(P.weights) % 16 == 0 && j0 + 3 < pos) {
             float4* to = reinterpret_cast<float4*>(weights + j0);
-            const float4 was = *to;
+            const float4 was = __ldcg(to);
             *to = make_float4(was.x + sum[0], was.y + sum[1], was.z + sum[2], was.w + sum[3]);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (j0 + e < len) weights[j0 + e] = j0 + e < pos ? weights[j0 + e] + sum[e] : sum[e];
+                if (j0 + e < len) weights[j0 + e] = j0 + e < pos ? __ldcg(weights + j0 + e) + sum[e] : sum[e];
         }
         return;
     }
@@ -902,7 +906,7 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
     float w = 0.f;
 #pragma unroll
     for (int k = 0; k < W::GROUPS; ++k) w += parts[k * W::KEYS];
-    weights[j] = j < pos ? weights[j] + w : w;
+    weights[j] = j < pos ? __ldcg(weights + j) + w : w;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -913,13 +917,14 @@ constexpr int SMS = 148;
 // 31.8 / 31.2, 128 tokens over 4096 (8.5e9) 34 / 45.  A prefix of 1024, 32/8 heads: 64 sequences of head_dim 128 (1.1e9) 38 / 37, 128 of
 // head_dim 64 (1.1e9) 38 / 40, 128 of head_dim 128 (2.2e9) 47 / 73.
 constexpr int TC_ROWS = 192;
-constexpr int64_t TC_WORK = 4000000000ll, TC_PREFIX_WORK = 1500000000ll;
+constexpr double TC_WORK = 4e9, TC_PREFIX_WORK = 1.5e9;
+static double work_of(int D, int64_t rows, int64_t items, int64_t keys) { return 4.0 * D * static_cast<double>(rows) * static_cast<double>(items) * static_cast<double>(keys); }
 // One launch of clusters, or the stream kernel and the join: as long as a CTA has 16 steps at most and all CTAs run at once.  Captured in a graph,
 // 32/8 heads, clusters / stream: head_dim 128, one sequence of 4000 keys 10.3 / 11.3 us, 4 of 2000 10.1 / 14.2, 16 of 1000 13.9 / 18.7, 32 of 1000
 // 25.8 / 29.2, 64 of 500 (more CTAs than at once) stays 30.6; head_dim 64, 8 of 1000 8.2 / 13.8.  Clusters of 16 find room in a GPC only where an SM holds
 // two of its CTAs, and then one a GPC: 2 sequences of 4000 keys at head_dim 128 took 19.4 us in sixteens, 13.4 streamed; with one CTA an SM, also
 // those of 8 only as many as there are GPCs.
-constexpr int CLUSTER_MAX = 16, CLUSTER_STEPS = 16, SM_SMEM = 228 * 1024;
+constexpr int CLUSTER_MAX = 16, CLUSTER_STEPS = 16, SM_SMEM = 228 * 1024, CLUSTER_SMEM = 225 * 1024;      // (most a CTA may ask for, beside what it has statically)
 constexpr size_t cluster_smem(int D) { return D == 64 ? StreamCfg<64>::SMEM : (D == 128 ? StreamCfg<128>::SMEM : StreamCfg<256>::SMEM); }
 
 // CTAs of the kernels for few rows that the GPU holds at once, by their shared memory.
@@ -967,7 +972,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
             const int64_t per = (most + ranks - 1) / ranks;
             const size_t smem = cluster_smem(D) + (scored ? rows * per * STEP * 4 : 0);
             const int64_t ctas = static_cast<int64_t>((SM_SMEM - 1) / (smem + 2048));           // of an SM (a little kept by the kernel and by the GPU)
-            if (ranks / 2 >= most || per > CLUSTER_STEPS || ctas < 1 || items * ranks > SMS * ctas) continue;
+            if (ranks / 2 >= most || per > CLUSTER_STEPS || smem > CLUSTER_SMEM || items * ranks > SMS * ctas) continue;
             if (ranks == 16 && (items > 8 * (ctas - 1) || per > CLUSTER_STEPS / 2)) continue;
             if (ranks == 8 && ctas == 1 && items > 8) continue;
             p.cluster = ranks;
@@ -983,7 +988,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
     } else {
-        p.tc = !scored && D <= 128 && rows >= TC_ROWS && 4 * D * rows * items * seen >= TC_WORK;
+        p.tc = !scored && D <= 128 && rows >= TC_ROWS && work_of(D, rows, items, seen) >= TC_WORK;
         const int kt = p.tc ? 128 : (D == 256 ? 32 : 64), tr = p.tc ? 256 : 64;
         p.tiles = static_cast<int>((rows + tr - 1) / tr);
         const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + tr < S ? static_cast<int64_t>(window) + sinks + tr : S;
@@ -992,7 +997,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && 4 * D * rows * items * P >= TC_PREFIX_WORK;
+        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && work_of(D, rows, items, P) >= TC_PREFIX_WORK;
         const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
         const int64_t tiles = static_cast<int64_t>(p.pre_tiles) * KV_H, steps = (P + kt - 1) / kt;
@@ -1065,7 +1070,7 @@ static int launch_cluster(const Plan& plan, const Params& P, cudaStream_t st) {
     static bool ready[64] = {}, wide[64] = {};
     auto kern = span_cluster_kernel<D, SCORED>;
     const int extra = SCORED ? P.n * P.G * plan.cluster_steps * STEP * 4 : 0;
-    int rc = allow_smem(kern, SM_SMEM - 3 * 1024, ready);
+    int rc = allow_smem(kern, CLUSTER_SMEM, ready);
     if (rc != ALLOYB_OK) return rc;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;

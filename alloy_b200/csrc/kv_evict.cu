@@ -30,7 +30,7 @@ struct Params {
 };
 
 __device__ __forceinline__ int length_of(const Params& P, int b, bool tell) {
-    const int n = P.len[P.len_count == 1 ? 0 : b];
+    const int n = __ldcg(P.len + (P.len_count == 1 ? 0 : b));
     if (n > P.S || n < 0) {
         if (tell) atomicOr(&g_evict_status, 1);
         return 0;

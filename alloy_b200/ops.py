@@ -963,6 +963,9 @@ def _kv_evict(k_cache, v_cache, weights, lengths, k_out, v_out, weights_out, kee
                                          d, s, s_out, keep, sinks, recent, _stream())
         if rc:
             check(rc, "alloyb_kv_evict")
+    else:
+        kept.fill_(-1)
+        new_lengths.zero_()
     return kept, new_lengths
 
 

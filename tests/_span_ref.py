@@ -35,8 +35,9 @@ def attention(q, k, v, pos, *, window=0, sinks=0, prefix=None, scale=None):
     return out, w, mag, big
 
 
-def attention_wide(q, k, v, pos, *, window=0, sinks=0, prefix=None):
-    """The output and sum_j p |v| of ``attention`` by masks over whole score matrices, on the tensors' own device (for long calls)."""
+def attention_wide(q, k, v, pos, *, window=0, sinks=0, prefix=None, weights=None):
+    """The output and sum_j p |v| of ``attention`` by masks over whole score matrices, on the tensors' own device (for long calls).
+    ``weights`` (B, KV_H, S) grows by the probabilities."""
     b, h, n, d = q.shape
     kv_h, s = k.shape[1], k.shape[2]
     g = h // kv_h
@@ -59,6 +60,8 @@ def attention_wide(q, k, v, pos, *, window=0, sinks=0, prefix=None):
             x = (q[i, hq] @ kk.T / math.sqrt(d)).masked_fill(~m, -math.inf)
             pr = torch.softmax(x, -1)
             out[i, hq], mag[i, hq] = pr @ vv, pr @ vv.abs()
+            if weights is not None:
+                weights[i, hq // g, any_row] += pr.sum(0)
     return out, mag
 
 

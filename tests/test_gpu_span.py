@@ -267,6 +267,53 @@ def test_shared_prefix_long(b, h, kv_h, d, n, s, pos, p, dtype):
     c.check_written(k0, k, c.nk64, True)
 
 
+# calls past what clusters take: more (sequence, KV head)s than CTAs run at once, or long sequences
+STREAMED = [
+    # b, h, kv_h, d, n, s, pos, window, sinks, dtype, layout, write
+    (40, 16, 8, 128, 1, 300, [(i * 37) % 300 if i % 9 else -1 for i in range(40)], 100, 4, torch.float16, "model", True),
+    (60, 16, 8, 64, 2, 200, [(i * 31) % 199 if i % 7 else -1 for i in range(60)], 70, 20, torch.bfloat16, "packed", True),
+    (20, 24, 8, 256, 1, 150, [(i * 17) % 150 for i in range(20)], 64, 1, torch.float16, "dense", False),
+    (40, 8, 8, 128, 5, 128, [123 - i for i in range(40)], 300, 0, torch.float16, "model", True),
+    (300, 2, 1, 64, 1, 40, [i % 41 - 1 for i in range(300)], 11, 2, torch.float16, "model", True),
+    (1, 8, 2, 128, 1, 20000, [19999], 12000, 70, torch.float16, "model", True),
+    (2, 14, 2, 64, 2, 33000, [32998, 5], 32000, 0, torch.bfloat16, "packed", True),
+    (1, 16, 1, 256, 1, 9000, [8800], 8700, 3, torch.float16, "model", False),
+    (3, 3, 3, 128, 1, 30000, [29990, 0, 17], 40000, 0, torch.float16, "model", True),
+]
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,window,sinks,dtype,layout,write", STREAMED)
+def test_window_streamed(b, h, kv_h, d, n, s, pos, window, sinks, dtype, layout, write):
+    c = Case(b, h, kv_h, d, n, s, pos, dtype, layout=layout)
+    k, v, k64, v64 = c.caches(write, window, sinks)
+    k0, v0 = k.clone(), v.clone()
+    out = OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), k, v, window, sinks, -1.0, write)
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, window=window, sinks=sinks)
+    check(out, ref.cpu(), mag.cpu(), dtype)
+    c.check_written(k0, k, c.nk64, write)
+    c.check_written(v0, v, c.nv64, write)
+    assert ops.span_status() == 0
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,window,sinks,dtype,layout,write", STREAMED)
+def test_scored_streamed(b, h, kv_h, d, n, s, pos, window, sinks, dtype, layout, write):
+    c = Case(b, h, kv_h, d, n, s, pos, dtype, layout=layout)
+    k, v, k64, v64 = c.caches(write)
+    w = torch.rand(b, kv_h, s, generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = w.double()
+    for i in range(b):
+        if c.place(i) is not None:
+            w[i, :, c.place(i):c.place(i) + n] = BAD
+            want[i, :, c.place(i):c.place(i) + n] = 0.0
+    before, add = want.clone(), torch.zeros_like(want)
+    out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w, -1.0, write)
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, weights=add)
+    check(out, ref.cpu(), mag.cpu(), dtype)
+    big = float((c.q64.abs().amax() * c.k.abs().amax()) * d ** 0.5)            # above every scale * sum |q k|
+    off = (w.double() - before - add).abs()
+    assert (off <= R.weight_bound(add, big, d) + (before + add) * 2.0 ** -23).all()
+
+
 def evict_case(b, kv_h, s, s_out, d, lengths, kind="random", seed=0):
     g = torch.Generator().manual_seed(seed + s)
     k, v = torch.randn(b, kv_h, s, d, generator=g).half(), torch.randn(b, kv_h, s, d, generator=g).half()
@@ -297,7 +344,11 @@ def evict_case(b, kv_h, s, s_out, d, lengths, kind="random", seed=0):
     (1, 2, 1500, 64, [1400], 333, 1, 1, "equal"),
     (2, 2, 1500, 128, [1500, 1200], 600, 2, 3, "odd"),
     (1, 1, 1, 64, [1], 1, 0, 0, "random"),
+    (1, 2, 12000, 64, [11999], 5000, 3, 700, "random"),
+    (2, 1, 30000, 64, [30000, 29000], 7001, 4, 100, "odd"),
+    (1, 1, 32768, 64, [32768], 32767, 0, 0, "equal"),
     (1, 1, 40000, 64, [40000], 39999, 0, 0, "ties"),
+    (1, 1, 70000, 64, [69999], 100, 10, 20, "odd"),
 ])
 def test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place):
     k, v, w = evict_case(b, kv_h, s, keep, d, lengths, kind)
@@ -429,6 +480,19 @@ def test_same_bits_again_and_on_another_stream():
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         assert torch.equal(first, again) and torch.equal(w, w2)
+
+
+def test_prefix_layouts():
+    """One head's rows for all KV heads (a stride of zero), rows with gaps, K and V of different strides: as the dense prefix."""
+    c = Case(3, 8, 2, 128, 1, 64, [5, 20, 63], prefix=90)
+    one_k, one_v = c.pk[:1].to(DEV), c.pv[:1].to(DEV)
+    gaps = torch.zeros(2, 180, 128, dtype=torch.float16, device=DEV)[:, ::2]
+    gaps.copy_(one_v.expand(2, -1, -1))
+    outs = []
+    for pk, pv in ((one_k.repeat(2, 1, 1), one_v.repeat(2, 1, 1)), (one_k.expand(2, -1, -1), one_v.expand(2, -1, -1)), (one_k.repeat(2, 1, 1), gaps)):
+        k, v, _, _ = c.caches(True)
+        outs.append(OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), pk, pv, k, v))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
 def test_nothing_to_do():

@@ -104,7 +104,8 @@ def test_the_definitions_themselves():
     assert torch.allclose(full, cut)
     assert math.isclose(float(w.sum()), 4 * 2)
     for kw in (dict(), dict(window=3, sinks=2), dict(prefix=(k[0, :, :9], v[0, :, :9]))):
-        a, b = R.attention(q, k, v, [15], **kw), R.attention_wide(q, k, v, [15], **kw)
-        assert torch.allclose(a[0], b[0]) and torch.allclose(a[2], b[1])
+        grown = torch.zeros(1, 2, 20, dtype=torch.float64)
+        a, b = R.attention(q, k, v, [15], **kw), R.attention_wide(q, k, v, [15], weights=None if "prefix" in kw else grown, **kw)
+        assert torch.allclose(a[0], b[0]) and torch.allclose(a[2], b[1]) and torch.allclose(a[1], grown)
     assert R.evict([5, 1, 3, 3, 2, 9, 0, 0], 8, 5, 1, 1) == [0, 2, 3, 5, 7]
     assert R.evict([1.0, float("nan"), 0.0, 1.0], 4, 3, 0, 0) == [0, 2, 3]
