@@ -2,17 +2,21 @@
 // prompt under a window, and a large batch's rows over a shared prefix.  attn_span.cu has the rest, and joins partial results.
 //
 // What bounds it: a tile of 256 rows x 128 keys takes 2048 clocks of the tensor pipe at head_dim 128 (S and P V), and its 32768
-// exponentials 2048 clocks of the SM's sixteen a clock.  So a CTA works on two groups of 128 rows in turns: while one group's scores
-// are in its softmax warps, the tensor pipe has the other's.
+// exponentials 2048 clocks of the SM's sixteen a clock; neither is reached, since scores, exponentials and P V of a row wait for one
+// another (about 1100 clocks from P to the next scores in the softmax's hands).  So a CTA works on two groups of 128 rows, and a group on
+// two half tiles: while a group's softmax has the one, the tensor pipe has the other one's products and the other group's.
 //
 // * Q (two groups), K and V tiles of 128 keys in shared memory, 128-byte swizzle, K and V in two stages by TMA.  Tiles that are not 128 rows
 //   in one piece (the first rows, the end of a sequence) come in by cp.async, places past the last key zero-filled: what a cache holds there
-//   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.  (All tiles by cp.async, and the new
-//   tokens' rows from their own tensors: 314 us for 2048 tokens behind 6000 under a window of 4096, 32/8 heads, head_dim 128.)
-// * Scores and output accumulators in tensor memory.  Two threads share a row, 64 scores each, which stay in registers between the maximum
-//   (exchanged through shared memory) and the exponentials; P (fp16, rounded once) overwrites the scores and is read from there as the A
-//   operand.
+//   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.
+// * Scores (two buffers of 64 keys a group) and output accumulators in tensor memory, which they fill.  A thread has a row's 64 scores; P
+//   (fp16, rounded once) overwrites them, 32 keys at a time, and is read from there as the A operand.  (One buffer of 128 keys a group and two
+//   threads a row, which have to agree on the maximum: 172 us where this takes 147.)
+// * Which half tiles every row of a warp sees is worked out once, not per tile (10 us of the same call).
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
+// Measured, 32/8 heads, head_dim 128: 2048 tokens behind 6000 under a window of 4096 in 148 us (930 TFLOP/s of the products that the rows see,
+// 1020 of those that 256 tiles of 35 x 128 keys take; 1.73 rounds of tiles cost two); 64 sequences of 64/8 heads over a prefix of 32768 in
+// 73 us (940 TFLOP/s).
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
 #include <cuda.h>
 
@@ -24,8 +28,8 @@ namespace st5 {
 using sp::Params;
 using sp::Seq;
 
-constexpr int ROWS = 256, KT = 128, STAGES = 2, AHEAD = 3;
-constexpr int THREADS = 20 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-11 and 12-19 are their softmax
+constexpr int ROWS = 256, KT = 128, SUB = 64, STAGES = 2, AHEAD = 3;
+constexpr int THREADS = 12 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-7 and 8-11 are their softmax
 constexpr int HALF = 128 * 128;              // bytes of 128 rows x 64 halves
 constexpr uint32_t SPIN = 1u << 22;
 
@@ -35,7 +39,7 @@ template <int D>
 struct Cfg {
     static constexpr int TILE = D / 64 * HALF;
     static constexpr int SMEM = 1024 + 2 * TILE + 2 * STAGES * TILE + 256;
-    static constexpr int COLS = 256;         // tensor-memory columns of a group: 128 of scores, D of outputs
+    static constexpr int COLS = 256;         // tensor-memory columns of a group: twice 64 of scores, D of outputs
 };
 struct alignas(64) Args {
     CUtensorMap k, v;                        // (D, rows, heads), boxes of 64 elements x 128 rows, 128-byte swizzle
@@ -43,7 +47,7 @@ struct alignas(64) Args {
 };
 struct Bars {
     uint64_t k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
-    uint64_t s_full[2], p_full[2], o_full[2], turn[2];
+    uint64_t s_full[2][2], p_half[2][2], p_full[2][2];       // [group][buffer]
     uint32_t tmem_base;
 };
 
@@ -82,18 +86,25 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t leading) {
 __device__ __forceinline__ constexpr uint32_t umma_idesc(int n, bool b_mn) {
     return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n) >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(idesc), "r"(accumulate)
+// A warp's issue, all lanes in step: `lead` is 1 in the lane that does it.
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate), "r"(lead)
                  : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-                 "r"(idesc), "r"(accumulate)
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate), "r"(lead)
                  : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(b)) : "memory");
+__device__ __forceinline__ void umma_commit(uint64_t* b, uint32_t lead) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(s32(b)), "r"(lead)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t* u = reinterpret_cast<uint32_t*>(v);
@@ -169,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     constexpr int TILE = C::TILE, PIECES = D / 8;
     pdl_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
-    __shared__ float back[ROWS], half_max[2][ROWS], half_sum[ROWS];
+    __shared__ float back[ROWS];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t q_s = s32(smem), k_s = q_s + 2 * TILE, v_s = k_s + STAGES * TILE;
     Bars* bars = reinterpret_cast<Bars*>(smem + 2 * TILE + 2 * STAGES * TILE);
@@ -186,11 +197,10 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             bar_init(&bars->k_empty[s], 2);
             bar_init(&bars->v_empty[s], 2);
         }
-        for (int g = 0; g < 2; ++g) {
-            bar_init(&bars->s_full[g], 1);
-            bar_init(&bars->p_full[g], 8);
-            bar_init(&bars->o_full[g], 1);
-            bar_init(&bars->turn[g], 1);
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&bars->s_full[i >> 1][i & 1], 1);
+            bar_init(&bars->p_half[i >> 1][i & 1], 4);
+            bar_init(&bars->p_full[i >> 1][i & 1], 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -207,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     // ---- Q rows; dead rows are zero
-    constexpr int WARPS = THREADS / 32, BATCH = 13;
+    constexpr int WARPS = THREADS / 32, BATCH = 11;
     for (int i0 = 0; i0 * WARPS < ROWS; i0 += BATCH) {
         sp::QRow<D> qr[BATCH];
 #pragma unroll
@@ -232,53 +242,51 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
 
     if (warp < 4) {
         if (warp == 1 || warp == 2) {
-            // ------------------------------------------------ MMA issue, a group each (one lane), in turns.  An issuer's own instructions
-            // between two MMAs (a wait that is over takes it a hundred clocks) pass under the other group's MMAs; the turns keep the groups
-            // apart: side by side, both would be in their softmax at once, and then both in the tensor pipe.
+            // ------------------------------------------------ MMA issue, a group each
             const int g = warp - 1;
-            const uint32_t d = tmem + g * C::COLS;
-            if (lane == 0 && n_tiles > 0) {
-                auto scores = [&](int s) {
+            const uint32_t d = tmem + g * C::COLS, lead = elect();
+            const uint64_t q_desc = umma_desc(q_s + g * TILE, 16), k_desc = umma_desc(k_s, 16), v_desc = umma_desc(v_s, HALF);
+            auto scores = [&](int s, int h) {                                 // half h of a tile in stage s, into buffer h
+                const uint64_t kd = k_desc + ((s * TILE + h * SUB * 128) >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-                        umma_ss(d, umma_desc(q_s + g * TILE + off, 16), umma_desc(k_s + s * TILE + off, 16), umma_idesc(KT, false), kk > 0);
-                    }
-                };
-                // group 0 begins; its turn n + 1 comes with group 1's turn n, which comes with group 0's turn n
-                auto my_turn = [&](int n) {
-                    if (g == 1 || n > 0) bar_wait(ok, &bars->turn[g], (g == 1 ? n : n - 1) & 1);
-                };
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk >> 2) * HALF + (kk & 3) * 32) >> 4;
+                    umma_ss(d + h * SUB, q_desc + off, kd + off, umma_idesc(SUB, false), kk > 0, lead);
+                }
+                umma_commit(&bars->s_full[g][h], lead);
+            };
+            if (n_tiles > 0) {
                 bar_wait(ok, &bars->k_full[0], 0);
-                my_turn(0);
                 fence_after();
                 if (ok) {
-                    scores(0);
-                    bar_arrive(&bars->turn[g ^ 1]);
-                    umma_commit(&bars->s_full[g]);
-                    umma_commit(&bars->k_empty[0]);
+                    scores(0, 0);
+                    scores(0, 1);
+                    umma_commit(&bars->k_empty[0], lead);
                 }
-                for (int j = 0; j < n_tiles && ok; ++j) {
-                    const int s = j % STAGES, s1 = (j + 1) % STAGES;
-                    const bool more = j + 1 < n_tiles;
-                    bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
-                    if (more) bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
-                    bar_wait(ok, &bars->p_full[g], j & 1);
-                    my_turn(j + 1);
-                    fence_after();
-                    if (!ok) break;
+            }
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const int s = j % STAGES, s1 = (j + 1) % STAGES;
+                const bool more = j + 1 < n_tiles;
+                bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
+                if (more) bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
 #pragma unroll
-                    for (int kk = 0; kk < KT / 16; ++kk)
-                        umma_ts(d + 128, d + kk * 8, umma_desc(v_s + s * TILE + kk * 2048, HALF), umma_idesc(D, true), j > 0 || kk > 0);
-                    if (more) scores(s1);
-                    bar_arrive(&bars->turn[g ^ 1]);
-                    if (more) {
-                        umma_commit(&bars->s_full[g]);
-                        umma_commit(&bars->k_empty[s1]);
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int kk = 0; kk < SUB / 16; ++kk) {
+                        if (kk == 0 || kk == SUB / 32) {                      // P comes in two pieces
+                            bar_wait(ok, kk == 0 ? &bars->p_half[g][h] : &bars->p_full[g][h], j & 1);
+                            fence_after();
+                            if (!ok) break;
+                        }
+                        umma_ts(d + 2 * SUB, d + h * SUB + kk * 8, v_desc + ((s * TILE + (h * (SUB / 16) + kk) * 2048) >> 4), umma_idesc(D, true), j > 0 || h > 0 || kk > 0, lead);
                     }
-                    umma_commit(&bars->v_empty[s]);
+                    if (!ok) break;
+                    // behind P V, in the order of issue: S may take P's place, and whoever sees it complete has that P V too
+                    if (more) scores(s1, h);
+                    else umma_commit(&bars->s_full[g][h], lead);
                 }
-                if (ok) umma_commit(&bars->o_full[g]);
+                if (more) umma_commit(&bars->k_empty[s1], lead);
+                umma_commit(&bars->v_empty[s], lead);
             }
             __syncwarp();
         } else {
@@ -328,34 +336,35 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
         }
     } else {
-        // ------------------------------------------------ softmax: two threads a row, the one the first half of a tile's keys, one the second
-        constexpr int COLS = KT / 2;
-        const int g = (warp - 4) >> 3, half = (warp >> 2) & 1 ^ 1, r = g * 128 + (warp & 3) * 32 + lane;
+        // ------------------------------------------------ softmax, a thread a row, half a tile at a time
+        const int g = (warp - 4) >> 2, r = g * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * C::COLS;
-        const int pair = 1 + g * 4 + (warp & 3);                              // named barrier of the two warps that share rows
         const int R = row0 + r, pos = sq.pos + R / P.G;                       // (of a chunk) last row of the cache that this one may see
-        const int first = sq.pos + (R - lane) / P.G, last = sq.pos + (R - lane + 31) / P.G;
         const float scale = back[r];
-        float m_run = -INFINITY, l_run = 0.f;                                 // (l: of this half, times 64 like the accumulators)
-        for (int j = 0; j < n_tiles; ++j) {
-            const int place0 = (step0 + j) * KT;
-            bar_wait(ok, &bars->s_full[g], j & 1);
+        // half tiles whole0 .. whole1 - 1 of the sequence are seen by all rows of the warp: no key behind the earliest row, none before the
+        // latest row's window
+        int whole0 = 0, whole1 = sq.keys / SUB;
+        if (!PREFIX) {
+            const int first = sq.pos + (R - lane) / P.G, last = sq.pos + (R - lane + 31) / P.G;
+            whole1 = min(whole1, (first + 1 - sq.lo + sq.sink) / SUB);
+            if (P.window > 0) whole0 = max((sq.sink + SUB - 1) / SUB, (last - P.window + 1 - sq.lo + sq.sink + SUB - 1) / SUB);
+        }
+        float m_run = -INFINITY, l_run = 0.f;                                 // (l: times 64 like the accumulators)
+        const int n_sub = 2 * n_tiles, sub0 = 2 * step0;
+        for (int i = 0; i < n_sub; ++i) {
+            const uint32_t buf = lanes + (i & 1) * SUB;
+            bar_wait(ok, &bars->s_full[g][i & 1], (i >> 1) & 1);
             fence_after();
-            float s[COLS];
+            float s[SUB];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) tmem_ld32(lanes + half * COLS + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+            for (int c = 0; c < SUB / 32; ++c) tmem_ld32(buf + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
             wait_ld();
-            bool whole = place0 + KT <= sq.keys;                              // (uniform in the warp)
-            if (!PREFIX && whole) {
-                const int j0 = sq.row_of(place0), j1 = sq.row_of(place0 + KT - 1);
-                whole = j1 <= first && (P.window <= 0 || (place0 >= sq.sink && j0 > last - P.window) || place0 + KT <= sq.sink);
-            }
-            if (!whole) {
-                // place e of this half is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
-                const int at = place0 + half * COLS, hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - at;
+            if (sub0 + i < whole0 || sub0 + i >= whole1) {
+                // place e of this half tile is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
+                const int at = (sub0 + i) * SUB, hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - at;
                 const int lo = PREFIX || P.window <= 0 ? -1 : pos - P.window - sq.lo + sq.sink - at, sk = PREFIX ? 0 : P.sinks - at;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < SUB / 32; ++c) {
                     const uint32_t seen = sp::bits_below(hi + 1 - 32 * c) & (~sp::bits_below(lo + 1 - 32 * c) | sp::bits_below(sk - 32 * c));
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -364,26 +373,23 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < COLS; e += 8)
+            for (int e = 0; e < SUB; e += 8)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], s[e + k], s[e + 4 + k]);
-            float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
-            // the other half's maximum.  Behind the barrier both halves' scores are in registers, and P may overwrite them; the next tile's
-            // scores, and with them the next write to half_max, come behind both halves' P
-            half_max[half][r] = mx;
-            asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-            mx = fmaxf(mx, half_max[half ^ 1][r]);
+            const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
             const bool grow = mx > m_run + sp::RESCALE_LOG2;
             if (__any_sync(0xffffffffu, grow)) {
                 const float alpha = grow ? ex2(m_run - mx) : 1.0f;
                 if (grow) m_run = mx;
                 l_run *= alpha;
-                if (j > 0) {                                                  // (these scores came behind the last P V, which is complete)
+                if (i > 0) {
+                    bar_wait(ok, &bars->s_full[g][(i & 1) ^ 1], (((i - 1) >> 1) + 1) & 1);       // behind the last P V
+                    fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
+                    for (int c = 0; c < D / 16; ++c) {
                         float o[16];
                         uint32_t w[16];
-                        const uint32_t at = lanes + 128 + half * (D / 2) + c * 16;
+                        const uint32_t at = lanes + 2 * SUB + c * 16;
                         tmem_ld16(at, o);
                         wait_ld();
 #pragma unroll
@@ -397,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             const uint64_t scale2 = f2(scale, scale), sub2 = f2(sub, sub);
             uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < SUB / 32; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -408,43 +414,35 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                     sum[e & 1] = f2_add(sum[e & 1], f2(x0, x1));
                     p[e] = pack_h2(x0, x1);
                 }
-                tmem_st16(lanes + half * (COLS / 2) + c * 16, p);
+                tmem_st16(buf + c * 16, p);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(c == 0 ? &bars->p_half[g][i & 1] : &bars->p_full[g][i & 1]);
             }
             float a0, a1, b0, b1;
             unf2(sum[0], a0, a1);
             unf2(sum[1], b0, b1);
             l_run += (a0 + a1) + (b0 + b1);
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bars->p_full[g]);
         }
-        // ---- normalise and store, half of the columns each
-        if (half == 1) half_sum[r] = l_run;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-        if (half == 0) {
-            l_run += half_sum[r];
-            half_sum[r] = l_run;
-        }
-        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-        l_run = half_sum[r];
+        // ---- normalise and store
         if (n_tiles > 0) {
-            bar_wait(ok, &bars->o_full[g], 0);
+            bar_wait(ok, &bars->s_full[g][1], n_tiles & 1);
             fence_after();
         }
         const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
         const bool row_live = ok && R < all_rows, direct = !PREFIX && splits == 1 && P.pre_o == nullptr;
         const int tok = R / P.G, hg = R - tok * P.G;
         const int64_t slot = ((static_cast<int64_t>(PREFIX ? 0 : b) * P.KV_H + kvh) * tiles + tile) * splits + split;
-        if (row_live && !direct && half == 0)
+        if (row_live && !direct)
             (PREFIX ? P.pre_lse : P.part_lse)[slot * ROWS + r] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run) - sp::P_BIAS_LOG2;
         float* po = (PREFIX ? P.pre_o : P.part_o) + (slot * ROWS + r) * D;
         const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
 #pragma unroll 1
-        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+        for (int c = 0; c < D / 32; ++c) {
             float o[32];
             if (n_tiles > 0) {
-                tmem_ld32(lanes + 128 + c * 32, o);
+                tmem_ld32(lanes + 2 * SUB + c * 32, o);
                 wait_ld();
             } else {
 #pragma unroll
@@ -460,6 +458,8 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
         }
     }
+    if (!ok)
+        for (uint32_t i = 0; i < 1024; ++i) __nanosleep(512);                 // a wait ran out: let copies and products in flight end
     fence_before();
     __syncthreads();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
