@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     const Params& P = A.p;
     using C = Cfg<D>;
     constexpr int TILE = C::TILE, PIECES = D / 8;
-    pdl_launch_dependents();
+    if (!PREFIX) pdl_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     __shared__ float back[ROWS];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     pdl_wait();
+    if (PREFIX) pdl_launch_dependents();
     const int tok0 = row0 / P.G, tok1 = min(P.n, (row0 + ROWS - 1) / P.G + 1);
     Seq sq = {0, 0, 0, P.P};
     if (!PREFIX) sq = sp::seq_at(P, sp::live_pos(P, b, tile == 0 && kvh == 0 && split == 0 && threadIdx.x == 0), tok0, tok1);
