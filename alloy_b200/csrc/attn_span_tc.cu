@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
 template <int D>
 __global__ void __launch_bounds__(256) span_append_kernel(const Params P) {
     pdl_launch_dependents();
-    const int i = blockIdx.x * 256 + threadIdx.x, tok = i / (D / 8), c = i % (D / 8) * 8, kvh = blockIdx.y, b = blockIdx.z;
+    constexpr int PIECES = D / 8;
+    const int tok = blockIdx.x * (256 / PIECES) + threadIdx.x / PIECES, c = threadIdx.x % PIECES * 8, kvh = blockIdx.y, b = blockIdx.z;
     pdl_wait();
     if (tok >= P.n) return;
     const int pos = sp::live_pos(P, b, false);
@@ -518,7 +519,7 @@ static int launch(dim3 grid, cudaStream_t st, const Params& P) {
                                          map_rows(&a.v, P.v, D, P.S, static_cast<int64_t>(P.B) * P.KV_H, static_cast<int64_t>(P.S) * D);
         if (!mapped) e = cudaErrorInvalidValue;
     }
-    if (e == cudaSuccess && !PREFIX && P.nk) e = launch_pdl(span_append_kernel<D>, dim3((P.n * (D / 8) + 255) / 256, P.KV_H, P.B), dim3(256), 0, st, P);
+    if (e == cudaSuccess && !PREFIX && P.nk) e = launch_pdl(span_append_kernel<D>, dim3((P.n + 2048 / D - 1) / (2048 / D), P.KV_H, P.B), dim3(256), 0, st, P);
     if (e == cudaSuccess) e = launch_pdl(span_tc_kernel<D, PREFIX>, grid, dim3(THREADS), Cfg<D>::SMEM, st, a);
     if (e != cudaSuccess) {
         set_cuda_error(e);

@@ -377,6 +377,19 @@ def test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place):
     assert ops.span_status() == 0
 
 
+@pytest.mark.parametrize("b,kv_h,s,d,lengths,keep,sinks,recent", [
+    (2, 2, 900, 128, [900, 640], 640, 0, 640),                         # nothing is decided by weight, all of it recent
+    (2, 2, 900, 128, [900, 650], 641, 1, 640),
+    (3, 2, 900, 128, [900, 300, 0], 512, 130, 320),                    # sinks past a CTA's rows; nothing to evict; no rows
+    (2, 1, 1100, 64, [1100, 701], 700, 5, 300),
+    (2, 1, 500, 256, [500, 431], 430, 33, 97),
+    (5, 4, 3000, 128, [3000, 2048, 2049, 1, 2700], 2048, 4, 1500),
+])
+def test_evict_many_recent_rows(b, kv_h, s, d, lengths, keep, sinks, recent):
+    test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, "random", False)
+    test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, "ties", False)
+
+
 def test_evict_length_out_of_range():
     k, v, w = (t.to(DEV) for t in evict_case(2, 1, 50, 20, 64, [50, 50]))
     k0 = k.clone()
@@ -463,6 +476,54 @@ def test_captured_and_replayed_with_moving_positions():
             for x, y in zip(mine, want):
                 assert torch.equal(x, y)
         assert ops.span_status() == (2 if -1 in pos else 0)          # (-1 is an idle sequence's position, but no length)
+
+
+def test_calls_in_a_row():
+    """Launches begin under the ones before them: calls whose workspaces, caches and outputs follow one another without a pause give the
+    bits that each gives alone."""
+    p = 14001
+    prefix = [Case(70, 8, 2, 128, 1, 32, [(i * 5 + j) % 32 for i in range(70)], prefix=p, seed=j) for j in range(2)]
+    shared = [[t.to(DEV) for t in (c.pk, c.pv)] for c in prefix]
+    chunk = Case(1, 8, 1, 128, 700, 6000, [5100])
+    step = Case(40, 16, 8, 128, 1, 300, [(i * 37) % 300 for i in range(40)])
+    weights = torch.rand(40, 8, 300, generator=torch.Generator().manual_seed(3)).to(DEV)
+    lengths = torch.tensor([260 + i for i in range(40)], dtype=torch.int32, device=DEV)
+
+    def behind(j):
+        k, v, _, _ = prefix[j].caches(True)
+        c = prefix[j]
+        return lambda: (OPS.attention_shared_prefix(c.q, c.nk, c.nv, pos[j], *shared[j], kc := k.clone(), vc := v.clone()), kc, vc)
+
+    def window():
+        k, v, _, _ = chunk.caches(True)
+        at = chunk.pos_t()
+        return lambda: (OPS.attention_cache_window(chunk.q, chunk.nk, chunk.nv, at, kc := k.clone(), vc := v.clone(), 4000, 129), kc, vc)
+
+    def scored_and_evicted():
+        k, v = (x.to(DEV) for x in (step.k, step.v))
+        at = step.pos_t()
+
+        def run():
+            kc, vc, w = k.clone(), v.clone(), weights.clone()
+            out = OPS.attention_cache_scored(step.q, step.nk, step.nv, at, kc, vc, w)
+            ko, vo, wo = (torch.zeros_like(x[:, :, :200]) for x in (kc, vc, w))
+            return out, w, ko, vo, wo, *OPS.kv_evict(kc, vc, w, lengths, ko, vo, wo, 200, 4, 150)
+        return run
+
+    pos = [c.pos_t() for c in prefix]
+    calls = [behind(0), window(), behind(1), scored_and_evicted()]
+    alone = []
+    for f in calls:
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in f()])
+        torch.cuda.synchronize()
+    rounds = [[f() for f in calls] for _ in range(4)]
+    torch.cuda.synchronize()
+    for got in rounds:
+        for a, z in zip(alone, got):
+            for x, y in zip(a, z):
+                bits = torch.int16 if x.element_size() == 2 else torch.int32
+                assert torch.equal(x.view(bits), y.view(bits))
 
 
 def test_same_bits_again_and_on_another_stream():
