@@ -924,8 +924,8 @@ constexpr int SMS = 148;
 // cores.  Own keys, 32/8 heads, there / on mma.sync: 128 tokens of head_dim 128 over a window of 1024 (2.2e9) 31.3 / 29.6 us, 256 tokens (4.3e9)
 // 31.8 / 31.2, 128 tokens over 4096 (8.5e9) 34 / 45.  A prefix of 1024, 32/8 heads: 64 sequences of head_dim 128 (1.1e9) 38 / 37, 128 of
 // head_dim 64 (1.1e9) 38 / 40, 128 of head_dim 128 (2.2e9) 47 / 73.
-constexpr int TC_ROWS = 192;
-constexpr double TC_WORK = 4e9, TC_PREFIX_WORK = 1.5e9;
+constexpr int TC_TILE = 128, TC_PREFIX_ROWS = 32;           // rows of a tile; fewer rows leave most of it empty
+constexpr double TC_WORK = 5e9, TC_PREFIX_WORK = 1.5e9;
 static double work_of(int D, int64_t rows, int64_t items, int64_t keys) { return 4.0 * D * static_cast<double>(rows) * static_cast<double>(items) * static_cast<double>(keys); }
 // One launch of clusters, or the stream kernel and the join: as long as a CTA has 16 steps at most and all CTAs run at once.  Captured in a graph,
 // 32/8 heads, clusters / stream: head_dim 128, one sequence of 4000 keys 10.3 / 11.3 us, 4 of 2000 10.1 / 14.2, 16 of 1000 13.9 / 18.7, 32 of 1000
@@ -996,17 +996,17 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         lse_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         o_rows = P > 0 ? lse_rows : 2 * static_cast<size_t>(p.ctas) * 16;
     } else {
-        p.tc = !scored && D <= 128 && rows >= TC_ROWS && work_of(D, rows, items, seen) >= TC_WORK;
-        const int kt = p.tc ? 128 : (D == 256 ? 32 : 64), tr = p.tc ? 256 : 64;
+        p.tc = !scored && D <= 128 && work_of(D, rows, items, seen) >= TC_WORK;
+        const int kt = D == 256 ? 32 : 64, tr = p.tc ? TC_TILE : 64;
         p.tiles = static_cast<int>((rows + tr - 1) / tr);
         const int64_t span = window > 0 && static_cast<int64_t>(window) + sinks + tr < S ? static_cast<int64_t>(window) + sinks + tr : S;
-        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, p.tc ? SMS : 2 * SMS, scored || P > 0 ? 0 : 6);
+        p.splits = choose_splits(items * p.tiles, (span + kt - 1) / kt, 2 * SMS, scored || P > 0 ? 0 : 6);
         lse_rows = static_cast<size_t>(items) * p.tiles * p.splits * tr;
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_ROWS && work_of(D, rows, items, P) >= TC_PREFIX_WORK;
-        const int kt = p.pre_tc ? 128 : (D == 256 ? 32 : 64), tr = p.pre_tc ? 256 : 64;
+        p.pre_tc = D <= 128 && rows * B >= TC_PREFIX_ROWS && work_of(D, rows, items, P) >= TC_PREFIX_WORK;
+        const int kt = D == 256 ? 32 : 64, tr = p.pre_tc ? TC_TILE : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
         const int64_t tiles = static_cast<int64_t>(p.pre_tiles) * KV_H, steps = (P + kt - 1) / kt;
         if (p.stream && !p.pre_tc) {
@@ -1019,7 +1019,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
             if (p.ctas > (rest > least ? rest : least)) p.ctas = static_cast<int>(rest > least ? rest : least);
             lse_rows = o_rows = (2 * static_cast<size_t>(p.ctas) + items) * 16;
         } else {
-            p.pre_splits = choose_splits(tiles, steps, p.pre_tc ? SMS : 2 * SMS, 0);
+            p.pre_splits = choose_splits(tiles, steps, 2 * SMS, 0);
         }
     }
     size_t at = 0;
@@ -1032,7 +1032,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     p.part_lse = take(lse_rows * 4);
     p.part_o = take(o_rows * D * 4);
     if (P > 0) {
-        const int tr = p.pre_tc ? 256 : 64;
+        const int tr = p.pre_tc ? TC_TILE : 64;
         const size_t r = static_cast<size_t>(p.pre_tiles) * KV_H * p.pre_splits * tr;
         p.pre_lse = take(r * 4);
         p.pre_o = take(r * D * 4);
@@ -1207,8 +1207,8 @@ static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_
     P.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
     P.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     P.ctas = plan.ctas; P.splits = plan.splits; P.tiles = plan.tiles; P.pre_splits = plan.pre_splits;
-    P.tile_rows = plan.tc ? 256 : 64;
-    P.pre_tile_rows = plan.pre_tc ? 256 : 64;
+    P.tile_rows = plan.tc ? TC_TILE : 64;
+    P.pre_tile_rows = plan.pre_tc ? TC_TILE : 64;
     if (plan.pre_splits) {
         P.pre_lse = reinterpret_cast<float*>(ws + plan.pre_lse);
         P.pre_o = reinterpret_cast<float*>(ws + plan.pre_o);

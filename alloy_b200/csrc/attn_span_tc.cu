@@ -28,26 +28,26 @@ namespace st5 {
 using sp::Params;
 using sp::Seq;
 
-constexpr int ROWS = 256, KT = 128, SUB = 64, STAGES = 2, AHEAD = 3;
-constexpr int THREADS = 12 * 32;             // warps 0 and 3 copy K and V, 1 and 2 issue the groups' MMAs, 4-7 and 8-11 are their softmax
-constexpr int HALF = 128 * 128;              // bytes of 128 rows x 64 halves
+constexpr int ROWS = 128, KT = 64, STAGES = 2, AHEAD = 3;
+constexpr int THREADS = 8 * 32;              // warps 0 and 3 copy K and V, 1 issues the MMAs, 4-7 are the softmax
+constexpr int Q_HALF = ROWS * 128, KV_HALF = KT * 128;       // bytes of a tile's rows x 64 halves
 constexpr uint32_t SPIN = 1u << 22;
 
 static __device__ int g_tc_error = 0;        // sticky: a bounded wait of this file's kernel ran out
 
 template <int D>
 struct Cfg {
-    static constexpr int TILE = D / 64 * HALF;
-    static constexpr int SMEM = 1024 + 2 * TILE + 2 * STAGES * TILE + 256;
-    static constexpr int COLS = 256;         // tensor-memory columns of a group: twice 64 of scores, D of outputs
+    static constexpr int Q = D / 64 * Q_HALF, TILE = D / 64 * KV_HALF;
+    static constexpr int SMEM = 1024 + Q + 2 * STAGES * TILE + 256;
+    static constexpr int COLS = 256;         // tensor-memory columns: two buffers of 64 scores, D of outputs; two CTAs an SM have all of it
 };
 struct alignas(64) Args {
-    CUtensorMap k, v;                        // (D, rows, heads), boxes of 64 elements x 128 rows, 128-byte swizzle
+    CUtensorMap k, v;                        // (D, rows, heads), boxes of 64 elements x KT rows, 128-byte swizzle
     Params p;
 };
 struct Bars {
     uint64_t k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES];
-    uint64_t s_full[2][2], p_half[2][2], p_full[2][2];       // [group][buffer]
+    uint64_t s_full[2], p_half[2], p_full[2];        // [buffer]
     uint32_t tmem_base;
 };
 
@@ -169,21 +169,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// Byte offset of 16-byte piece c of a row in a tile: halves of 64 elements, each in the 128-byte swizzle.
-__device__ __forceinline__ uint32_t piece_at(int row, int c) { return (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4); }
+// Byte offset of 16-byte piece c of a row in a tile: halves of 64 elements (`half` bytes), each in the 128-byte swizzle.
+__device__ __forceinline__ uint32_t piece_at(int row, int c, int half) { return (c >> 3) * half + row * 128 + (((c & 7) ^ (row & 7)) << 4); }
 
 // Grid (tiles * splits, KV_H, B); PREFIX: rows of the whole batch over the shared prefix, grid z 1, partial results only.
 template <int D, bool PREFIX>
-__global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(THREADS, 2) span_tc_kernel(const __grid_constant__ Args A) {
     const Params& P = A.p;
     using C = Cfg<D>;
     constexpr int TILE = C::TILE, PIECES = D / 8;
-    if (!PREFIX) pdl_launch_dependents();
     extern __shared__ uint8_t smem_raw[];
     __shared__ float back[ROWS];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t q_s = s32(smem), k_s = q_s + 2 * TILE, v_s = k_s + STAGES * TILE;
-    Bars* bars = reinterpret_cast<Bars*>(smem + 2 * TILE + 2 * STAGES * TILE);
+    const uint32_t q_s = s32(smem), k_s = q_s + C::Q, v_s = k_s + STAGES * TILE;
+    Bars* bars = reinterpret_cast<Bars*>(smem + C::Q + 2 * STAGES * TILE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int splits = PREFIX ? P.pre_splits : P.splits, tiles = gridDim.x / splits;
     const int split = blockIdx.x % splits, tile = tiles - 1 - blockIdx.x / splits;      // the rows with the most keys go first
@@ -194,22 +193,23 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         for (int s = 0; s < STAGES; ++s) {
             bar_init(&bars->k_full[s], 1);
             bar_init(&bars->v_full[s], 1);
-            bar_init(&bars->k_empty[s], 2);
-            bar_init(&bars->v_empty[s], 2);
+            bar_init(&bars->k_empty[s], 1);
+            bar_init(&bars->v_empty[s], 1);
         }
-        for (int i = 0; i < 4; ++i) {
-            bar_init(&bars->s_full[i >> 1][i & 1], 1);
-            bar_init(&bars->p_half[i >> 1][i & 1], 4);
-            bar_init(&bars->p_full[i >> 1][i & 1], 4);
+        for (int h = 0; h < 2; ++h) {
+            bar_init(&bars->s_full[h], 1);
+            bar_init(&bars->p_half[h], 4);
+            bar_init(&bars->p_full[h], 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Tensor memory behind the wait, and what follows may begin only once every CTA has its own: a CTA of the launch before or behind that
+    // shares the SM could otherwise wait for the columns that this one holds while this one waits for it.
+    pdl_wait();
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&bars->tmem_base)), "r"(512));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&bars->tmem_base)), "r"(C::COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    pdl_wait();
-    if (PREFIX) pdl_launch_dependents();
     const int tok0 = row0 / P.G, tok1 = min(P.n, (row0 + ROWS - 1) / P.G + 1);
     Seq sq = {0, 0, 0, P.P};
     if (!PREFIX) sq = sp::seq_at(P, sp::live_pos(P, b, tile == 0 && kvh == 0 && split == 0 && threadIdx.x == 0), tok0, tok1);
@@ -218,19 +218,18 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     const int64_t head = PREFIX ? kvh * P.p_hs : (static_cast<int64_t>(b) * P.KV_H + kvh) * P.S * D;
 
     // ---- Q rows; dead rows are zero
-    constexpr int WARPS = THREADS / 32, BATCH = 11;
+    constexpr int WARPS = THREADS / 32, BATCH = 8;
     for (int i0 = 0; i0 * WARPS < ROWS; i0 += BATCH) {
         sp::QRow<D> qr[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int r = warp + (i0 + i) * WARPS, R = row0 + r, rb = PREFIX ? R / rows : b, rest = PREFIX ? R - rb * rows : R, tok = rest / P.G, hg = rest - tok * P.G;
-            qr[i].read(P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, r < ROWS && R < all_rows, lane);
+            qr[i].read(P.q, rb * P.q_bs + (kvh * P.G + hg) * P.q_hs + tok * P.q_ts, P.q_vec != 0, R < all_rows, lane);
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int r = warp + (i0 + i) * WARPS;
-            if (r >= ROWS) break;
-            const float f = qr[i].put([&](int d) { return q_s + (r >> 7) * TILE + piece_at(r & 127, d >> 3) + (d & 7) * 2; }, P.q_dtype, lane);
+            const float f = qr[i].put([&](int d) { return q_s + piece_at(r, d >> 3, Q_HALF) + (d & 7) * 2; }, P.q_dtype, lane);
             if (lane == 0) back[r] = f * P.scale_log2;
         }
     }
@@ -238,59 +237,54 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
     fence_before();
     __syncthreads();
     fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = bars->tmem_base;
     bool ok = true;
 
     if (warp < 4) {
-        if (warp == 1 || warp == 2) {
-            // ------------------------------------------------ MMA issue, a group each
-            const int g = warp - 1;
-            const uint32_t d = tmem + g * C::COLS, lead = elect();
-            const uint64_t q_desc = umma_desc(q_s + g * TILE, 16), k_desc = umma_desc(k_s, 16), v_desc = umma_desc(v_s, HALF);
-            auto scores = [&](int s, int h) {                                 // half h of a tile in stage s, into buffer h
-                const uint64_t kd = k_desc + ((s * TILE + h * SUB * 128) >> 4);
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * HALF + (kk & 3) * 32) >> 4;
-                    umma_ss(d + h * SUB, q_desc + off, kd + off, umma_idesc(SUB, false), kk > 0, lead);
-                }
-                umma_commit(&bars->s_full[g][h], lead);
-            };
-            if (n_tiles > 0) {
-                bar_wait(ok, &bars->k_full[0], 0);
+        if (warp == 1) {
+            // ------------------------------------------------ MMA issue
+            const uint32_t lead = elect();
+            const uint64_t q_desc = umma_desc(q_s, 16), k_desc = umma_desc(k_s, 16), v_desc = umma_desc(v_s, KV_HALF);
+            auto scores = [&](int j, int h) {                                 // of tile j, into buffer h
+                const int s = j % STAGES;
+                bar_wait(ok, &bars->k_full[s], (j / STAGES) & 1);
                 fence_after();
-                if (ok) {
-                    scores(0, 0);
-                    scores(0, 1);
-                    umma_commit(&bars->k_empty[0], lead);
-                }
-            }
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                const int s = j % STAGES, s1 = (j + 1) % STAGES;
-                const bool more = j + 1 < n_tiles;
-                bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
-                if (more) bar_wait(ok, &bars->k_full[s1], ((j + 1) / STAGES) & 1);
+                if (!ok) return;
+                const uint64_t kd = k_desc + ((s * TILE) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_ss(tmem + h * KT, q_desc + (((kk >> 2) * Q_HALF + (kk & 3) * 32) >> 4), kd + (((kk >> 2) * KV_HALF + (kk & 3) * 32) >> 4),
+                            umma_idesc(KT, false), kk > 0, lead);
+                umma_commit(&bars->s_full[h], lead);
+                umma_commit(&bars->k_empty[s], lead);
+            };
+            if (n_tiles > 0) scores(0, 0);
+            if (n_tiles > 1) scores(1, 1);
+            for (int j0 = 0; j0 < n_tiles && ok; j0 += 2) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const int j = j0 + h, s = j % STAGES;
+                    if (j >= n_tiles) break;
+                    bar_wait(ok, &bars->v_full[s], (j / STAGES) & 1);
 #pragma unroll
-                    for (int kk = 0; kk < SUB / 16; ++kk) {
-                        if (kk == 0 || kk == SUB / 32) {                      // P comes in two pieces
-                            bar_wait(ok, kk == 0 ? &bars->p_half[g][h] : &bars->p_full[g][h], j & 1);
+                    for (int kk = 0; kk < KT / 16; ++kk) {
+                        if (kk == 0 || kk == KT / 32) {                       // P comes in two pieces
+                            bar_wait(ok, kk == 0 ? &bars->p_half[h] : &bars->p_full[h], (j >> 1) & 1);
                             fence_after();
                             if (!ok) break;
                         }
-                        umma_ts(d + 2 * SUB, d + h * SUB + kk * 8, v_desc + ((s * TILE + (h * (SUB / 16) + kk) * 2048) >> 4), umma_idesc(D, true), j > 0 || h > 0 || kk > 0, lead);
+                        umma_ts(tmem + 2 * KT, tmem + h * KT + kk * 8, v_desc + ((s * TILE + kk * 2048) >> 4), umma_idesc(D, true), j > 0 || kk > 0, lead);
                     }
                     if (!ok) break;
+                    umma_commit(&bars->v_empty[s], lead);
                     // behind P V, in the order of issue: S may take P's place, and whoever sees it complete has that P V too
-                    if (more) scores(s1, h);
-                    else umma_commit(&bars->s_full[g][h], lead);
+                    if (j + 2 < n_tiles) scores(j + 2, h);
+                    else umma_commit(&bars->s_full[h], lead);
                 }
-                if (more) umma_commit(&bars->k_empty[s1], lead);
-                umma_commit(&bars->v_empty[s], lead);
             }
             __syncwarp();
-        } else {
+        } else if (warp == 0 || warp == 3) {
             // ------------------------------------------------ tiles of K (warp 0) and V (warp 3)
             const bool is_v = warp == 3;
             const int c = lane % PIECES, r0 = lane / PIECES;
@@ -317,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                     if (lane == 0 && ok) {
                         bar_expect(full, TILE);
 #pragma unroll
-                        for (int h = 0; h < D / 64; ++h) tma_3d(dst + h * HALF, is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z, full);
+                        for (int h = 0; h < D / 64; ++h) tma_3d(dst + h * KV_HALF, is_v ? &A.v : &A.k, h * 64, PREFIX ? place0 : sq.row_of(place0), z, full);
                     }
                 } else {
                     if (ok) {
@@ -325,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                         for (int i = 0; i < KT * PIECES / 32; ++i) {
                             const int r = r0 + i * (32 / PIECES);
                             const bool live = place0 + r < sq.keys;
-                            sp::copy16(dst + piece_at(r, c), src + static_cast<int64_t>(live ? sq.row_of(place0 + r) : 0) * D, live);
+                            sp::copy16(dst + piece_at(r, c, KV_HALF), src + static_cast<int64_t>(live ? sq.row_of(place0 + r) : 0) * D, live);
                         }
                     }
                     sp::copy_commit();
@@ -337,35 +331,34 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
         }
     } else {
-        // ------------------------------------------------ softmax, a thread a row, half a tile at a time
-        const int g = (warp - 4) >> 2, r = g * 128 + (warp & 3) * 32 + lane;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * C::COLS;
+        // ------------------------------------------------ softmax, a thread a row
+        const int r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int R = row0 + r, pos = sq.pos + R / P.G;                       // (of a chunk) last row of the cache that this one may see
         const float scale = back[r];
-        // half tiles whole0 .. whole1 - 1 of the sequence are seen by all rows of the warp: no key behind the earliest row, none before the
-        // latest row's window
-        int whole0 = 0, whole1 = sq.keys / SUB;
+        // tiles whole0 .. whole1 - 1 of the sequence are seen by all rows of the warp: no key behind the earliest row, none before the latest
+        // row's window
+        int whole0 = 0, whole1 = sq.keys / KT;
         if (!PREFIX) {
             const int first = sq.pos + (R - lane) / P.G, last = sq.pos + (R - lane + 31) / P.G;
-            whole1 = min(whole1, (first + 1 - sq.lo + sq.sink) / SUB);
-            if (P.window > 0) whole0 = max((sq.sink + SUB - 1) / SUB, (last - P.window + 1 - sq.lo + sq.sink + SUB - 1) / SUB);
+            whole1 = min(whole1, (first + 1 - sq.lo + sq.sink) / KT);
+            if (P.window > 0) whole0 = max((sq.sink + KT - 1) / KT, (last - P.window + 1 - sq.lo + sq.sink + KT - 1) / KT);
         }
         float m_run = -INFINITY, l_run = 0.f;                                 // (l: times 64 like the accumulators)
-        const int n_sub = 2 * n_tiles, sub0 = 2 * step0;
-        for (int i = 0; i < n_sub; ++i) {
-            const uint32_t buf = lanes + (i & 1) * SUB;
-            bar_wait(ok, &bars->s_full[g][i & 1], (i >> 1) & 1);
+        for (int j = 0; j < n_tiles; ++j) {
+            const uint32_t buf = lanes + (j & 1) * KT;
+            bar_wait(ok, &bars->s_full[j & 1], (j >> 1) & 1);
             fence_after();
-            float s[SUB];
+            float s[KT];
 #pragma unroll
-            for (int c = 0; c < SUB / 32; ++c) tmem_ld32(buf + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+            for (int c = 0; c < KT / 32; ++c) tmem_ld32(buf + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
             wait_ld();
-            if (sub0 + i < whole0 || sub0 + i >= whole1) {
-                // place e of this half tile is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
-                const int at = (sub0 + i) * SUB, hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - at;
+            if (step0 + j < whole0 || step0 + j >= whole1) {
+                // place e of this tile is seen if e <= hi and (e > lo or e < sk): as bits, 32 places a word
+                const int at = (step0 + j) * KT, hi = min(sq.keys - 1, PREFIX ? sq.keys - 1 : pos - sq.lo + sq.sink) - at;
                 const int lo = PREFIX || P.window <= 0 ? -1 : pos - P.window - sq.lo + sq.sink - at, sk = PREFIX ? 0 : P.sinks - at;
 #pragma unroll
-                for (int c = 0; c < SUB / 32; ++c) {
+                for (int c = 0; c < KT / 32; ++c) {
                     const uint32_t seen = sp::bits_below(hi + 1 - 32 * c) & (~sp::bits_below(lo + 1 - 32 * c) | sp::bits_below(sk - 32 * c));
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -374,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < SUB; e += 8)
+            for (int e = 0; e < KT; e += 8)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], s[e + k], s[e + 4 + k]);
             const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]) * scale;
@@ -383,14 +376,14 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 const float alpha = grow ? ex2(m_run - mx) : 1.0f;
                 if (grow) m_run = mx;
                 l_run *= alpha;
-                if (i > 0) {
-                    bar_wait(ok, &bars->s_full[g][(i & 1) ^ 1], (((i - 1) >> 1) + 1) & 1);       // behind the last P V
+                if (j > 0) {
+                    bar_wait(ok, &bars->s_full[(j & 1) ^ 1], (((j - 1) >> 1) + 1) & 1);       // behind the last P V
                     fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         float o[16];
                         uint32_t w[16];
-                        const uint32_t at = lanes + 2 * SUB + c * 16;
+                        const uint32_t at = lanes + 2 * KT + c * 16;
                         tmem_ld16(at, o);
                         wait_ld();
 #pragma unroll
@@ -404,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
             const uint64_t scale2 = f2(scale, scale), sub2 = f2(sub, sub);
             uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < SUB / 32; ++c) {
+            for (int c = 0; c < KT / 32; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -419,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(c == 0 ? &bars->p_half[g][i & 1] : &bars->p_full[g][i & 1]);
+                if (lane == 0) bar_arrive(c == 0 ? &bars->p_half[j & 1] : &bars->p_full[j & 1]);
             }
             float a0, a1, b0, b1;
             unf2(sum[0], a0, a1);
@@ -428,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         }
         // ---- normalise and store
         if (n_tiles > 0) {
-            bar_wait(ok, &bars->s_full[g][1], n_tiles & 1);
+            bar_wait(ok, &bars->s_full[(n_tiles - 1) & 1], (((n_tiles - 1) >> 1) + 1) & 1);
             fence_after();
         }
         const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
@@ -443,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
             if (n_tiles > 0) {
-                tmem_ld32(lanes + 2 * SUB + c * 32, o);
+                tmem_ld32(lanes + 2 * KT + c * 32, o);
                 wait_ld();
             } else {
 #pragma unroll
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, 1) span_tc_kernel(const __grid_consta
         for (uint32_t i = 0; i < 1024; ++i) __nanosleep(512);                 // a wait ran out: let copies and products in flight end
     fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS));
 }
 
 // The new tokens' rows into the cache, ahead of a kernel that reads them there.
@@ -502,25 +495,24 @@ static bool map_rows(CUtensorMap* m, const __half* base, int D, int64_t rows, in
 
 template <int D, bool PREFIX>
 static int launch(dim3 grid, cudaStream_t st, const Params& P) {
+    auto kern = span_tc_kernel<D, PREFIX>;
     static bool ready[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
     cudaError_t e = encode_fn() ? cudaSuccess : cudaErrorNotSupported;
     if (e == cudaSuccess && !ready[dev]) {
-        e = cudaFuncSetAttribute(span_tc_kernel<D, PREFIX>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
         if (e == cudaSuccess) ready[dev] = true;
     }
     Args a;
     a.p = P;
     if (e == cudaSuccess) {
-        const bool mapped = PREFIX ? map_rows(&a.k, P.pk, D, P.P, P.KV_H, P.KV_H > 1 ? P.p_hs : static_cast<int64_t>(P.P) * D) &&
-                                         map_rows(&a.v, P.pv, D, P.P, P.KV_H, P.KV_H > 1 ? P.p_hs : static_cast<int64_t>(P.P) * D)
-                                   : map_rows(&a.k, P.k, D, P.S, static_cast<int64_t>(P.B) * P.KV_H, static_cast<int64_t>(P.S) * D) &&
-                                         map_rows(&a.v, P.v, D, P.S, static_cast<int64_t>(P.B) * P.KV_H, static_cast<int64_t>(P.S) * D);
-        if (!mapped) e = cudaErrorInvalidValue;
+        const int64_t rows = PREFIX ? P.P : P.S, heads = PREFIX ? P.KV_H : static_cast<int64_t>(P.B) * P.KV_H, apart = PREFIX && P.KV_H > 1 ? P.p_hs : rows * D;
+        if (!map_rows(&a.k, PREFIX ? P.pk : P.k, D, rows, heads, apart) || !map_rows(&a.v, PREFIX ? P.pv : P.v, D, rows, heads, apart))
+            e = cudaErrorInvalidValue;
     }
     if (e == cudaSuccess && !PREFIX && P.nk) e = launch_pdl(span_append_kernel<D>, dim3((P.n + 2048 / D - 1) / (2048 / D), P.KV_H, P.B), dim3(256), 0, st, P);
-    if (e == cudaSuccess) e = launch_pdl(span_tc_kernel<D, PREFIX>, grid, dim3(THREADS), Cfg<D>::SMEM, st, a);
+    if (e == cudaSuccess) e = launch_pdl(kern, grid, dim3(THREADS), Cfg<D>::SMEM, st, a);
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return ALLOYB_E_CUDA;
