@@ -13,7 +13,7 @@
 // More rows (chunks, and all the batch's rows over a shared prefix; span_rows_kernel).  Bound: mma.sync.  A CTA owns 64 (token, head) rows,
 // a warp 16 of them, and tiles of 64 keys (32 at head_dim 256) that its warps share; the keys are split where the tiles alone leave SMs
 // empty.  Tiles of 32 keys and three CTAs an SM were slower (4 x 16 tokens looking back over 5000 to 8100 keys: 68 -> 81 us), a third stage gave
-// nothing.  Many rows with much to do go to attn_span_tc.cu.
+// nothing, and with a step's scores a step ahead of its softmax took 70 -> 82.  Many rows with much to do go to attn_span_tc.cu.
 //
 // The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and a
 // last launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
@@ -920,11 +920,13 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
-// Rows of a KV head, and operations (4 D rows keys, by the sizes of the call), from which the own keys / a prefix go to the 5th-generation tensor
-// cores.  Own keys, 32/8 heads, there / on mma.sync: 128 tokens of head_dim 128 over a window of 1024 (2.2e9) 31.3 / 29.6 us, 256 tokens (4.3e9)
-// 31.8 / 31.2, 128 tokens over 4096 (8.5e9) 34 / 45.  A prefix of 1024, 32/8 heads: 64 sequences of head_dim 128 (1.1e9) 38 / 37, 128 of
-// head_dim 64 (1.1e9) 38 / 40, 128 of head_dim 128 (2.2e9) 47 / 73.
-constexpr int TC_TILE = 128, TC_PREFIX_ROWS = 32;           // rows of a tile; fewer rows leave most of it empty
+// Operations (4 D rows keys, by the sizes of the call) from which more than 16 rows of a KV head go to the 5th-generation tensor cores, own keys / a prefix.
+// There / on mma.sync, cold caches, 32/8 heads, window 4096: 16 tokens of 4 sequences, head_dim 128 (4.3e9) 41.0 / 38.9 us; 32 tokens of 4, head_dim 64
+// (4.3e9) 34.8 / 39.1; 8 tokens of 16 (8.6e9) 76.5 / 84.0; 5 tokens of 32 (1.1e10) 117 / 141; 80 tokens behind 6000 (1.1e10) 34.7 / 44.8.  A prefix of
+// 4096: 16 sequences (1.1e9) 38.9 / 36.9, 32 (2.1e9) 49.1 / 53.0; of 32768: 8 sequences, 32 rows (4.3e9) 59.4 / 63.5; 64 sequences over 4096 beside 1000 own
+// keys (4.3e9) 77 / 70, since there the own keys go in the same launch on mma.sync, 128 (8.6e9) 121 / 140.  Not the scored form: threads that have a row
+// each store its scores piecemeal (16 tokens of 4 sequences 82 / 67).
+constexpr int TC_TILE = 128, TC_PREFIX_ROWS = 32;           // rows of a tile; rows from which a prefix may go there
 constexpr double TC_WORK = 5e9, TC_PREFIX_WORK = 1.5e9;
 static double work_of(int D, int64_t rows, int64_t items, int64_t keys) { return 4.0 * D * static_cast<double>(rows) * static_cast<double>(items) * static_cast<double>(keys); }
 // One launch of clusters, or the stream kernel and the join: as long as a CTA has 16 steps at most and all CTAs run at once.  Captured in a graph,

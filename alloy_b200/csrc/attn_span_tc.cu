@@ -1,22 +1,24 @@
 // Attention of many query rows over spans of an fp16 cache on the 5th-generation tensor cores (head_dim 64 and 128): the chunks of a
 // prompt under a window, and a large batch's rows over a shared prefix.  attn_span.cu has the rest, and joins partial results.
 //
-// What bounds it: a tile of 256 rows x 128 keys takes 2048 clocks of the tensor pipe at head_dim 128 (S and P V), and its 32768
-// exponentials 2048 clocks of the SM's sixteen a clock; neither is reached, since scores, exponentials and P V of a row wait for one
-// another (about 1100 clocks from P to the next scores in the softmax's hands).  So a CTA works on two groups of 128 rows, and a group on
-// two half tiles: while a group's softmax has the one, the tensor pipe has the other one's products and the other group's.
+// What bounds it: 128 rows x 64 keys take 512 clocks of the tensor pipe at head_dim 128 (S and P V), and their 8192 exponentials 512 clocks of
+// the SM's sixteen a clock; neither is reached in a short call, since scores, exponentials and P V of a row wait for one another (about 1100 clocks from P to
+// the next scores in the softmax's hands, and as many for the softmax).  So an SM has two CTAs, and a CTA two tiles of scores: while the softmax
+// has one, the tensor pipe has the other one's products and the other CTA's.  In calls one after another for a second the 1000 W limit is the bound:
+// the SM clock falls from 1.9 to 1.65 GHz.
 //
-// * Q (two groups), K and V tiles of 128 keys in shared memory, 128-byte swizzle, K and V in two stages by TMA.  Tiles that are not 128 rows
+// * Q (128 rows), K and V tiles of 64 keys in shared memory, 128-byte swizzle, K and V in two stages by TMA.  Tiles that are not 64 rows
 //   in one piece (the first rows, the end of a sequence) come in by cp.async, places past the last key zero-filled: what a cache holds there
 //   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.
-// * Scores (two buffers of 64 keys a group) and output accumulators in tensor memory, which they fill.  A thread has a row's 64 scores; P
-//   (fp16, rounded once) overwrites them, 32 keys at a time, and is read from there as the A operand.  (One buffer of 128 keys a group and two
-//   threads a row, which have to agree on the maximum: 172 us where this takes 147.)
-// * Which half tiles every row of a warp sees is worked out once, not per tile (10 us of the same call).
+// * Two buffers of scores and the output accumulators in tensor memory, half of it a CTA.  A thread has a row's 64 scores; P
+//   (fp16, rounded once) overwrites them, 32 keys at a time, and is read from there as the A operand.
+// * Which tiles every row of a warp sees is worked out once, not per tile (2048 tokens behind 6000 under a window of 4096: 172 -> 162 us).
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
-// Measured, 32/8 heads, head_dim 128: 2048 tokens behind 6000 under a window of 4096 in 148 us (930 TFLOP/s of the products that the rows see,
-// 1020 of those that 256 tiles of 35 x 128 keys take; 1.73 rounds of tiles cost two); 64 sequences of 64/8 heads over a prefix of 32768 in
-// 73 us (940 TFLOP/s).
+// The same call with one CTA an SM, 256 rows in two groups, tiles of 128 keys: one buffer of 128 scores and two threads a row, which have to
+// agree on the maximum, 155 us; two buffers of 64 and a thread a row 147; four warps for the even tiles of keys and four for the odd ones 163.
+// This takes 136 (1010 TFLOP/s of the products that the rows see; 512 tiles are 1.73 rounds); 64 sequences of 64/8 heads over a prefix of 32768
+// take 71 (970 TFLOP/s), both 32/8 heads or more and head_dim 128.  At head_dim 64 the softmax is the bound: 132 us for the first call with everything
+// around it, where head_dim 128 takes 150.
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
 #include <cuda.h>
 
