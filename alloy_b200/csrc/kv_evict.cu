@@ -2,10 +2,10 @@
 // of those between, the ones of the largest weight stay (ties: the lower position), in their order, at the front of a cache -- another one
 // or the same.
 //
-// Two launches.  evict_select_kernel, a CTA per (sequence, KV head): the weight that the last row to stay has is found digit by digit
+// evict_select_kernel, a CTA per (sequence, KV head): the weight that the last row to stay has is found digit by digit
 // (a histogram of eleven, eleven and ten bits of the weights in an order-preserving integer form), then the positions above it, and as many
 // of those equal to it as are wanted, are written in order.  evict_copy_kernel moves the rows.  Bound: HBM, two rows read and written a
-// kept position.
+// kept position: 128 items of 4096 kept rows of 3000 to 16384 take 96 us, 5.5 TB/s.  Few items go in one launch (evict_one_kernel).
 //
 // In place a row only moves towards the front: a CTA owns a slice of columns of one (sequence, KV head) and walks the positions in order,
 // all of a batch read before any of it is written, so no row is overwritten before it is read.
@@ -17,6 +17,8 @@ namespace ev {
 static __device__ int g_evict_status = 0;    // sticky: 1 once a length was out of range
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int BINS = 2 * THREADS;                // eleven bits
+constexpr int SMS = 148, SHARE_MOST = 6 * 1024;  // most rows of a CTA that selects and copies: 24 KB of shared memory
+constexpr int64_t ONE_ROWS = 150000;             // kept rows in all up to which one launch does both
 
 struct Params {
     const __half *k, *v;                     // (B, KV_H, S, D)
@@ -26,7 +28,8 @@ struct Params {
     __half *k_out, *v_out;                   // (B, KV_H, S_out, D)
     float* w_out;
     int32_t *kept, *new_len;                 // (B, KV_H, keep), (B,)
-    int B, KV_H, S, S_out, keep, sinks, recent;
+    int B, KV_H, D, S, S_out, keep, sinks, recent;
+    int share;                               // of evict_one_kernel: rows of a CTA
 };
 
 __device__ __forceinline__ int length_of(const Params& P, int b, bool tell) {
@@ -71,23 +74,24 @@ __device__ __forceinline__ void take_digit(int* hist, int* warp_sum, int* found,
     left = found[1];
 }
 
+constexpr int runs_of(int R) { return R > 0 ? R * WARPS : WARPS; }
+template <int R>
+struct SelectShared {
+    int hist[BINS], warp_sum[WARPS], found[2];
+    uint32_t run_sum[runs_of(R)];            // of 32 positions (R == 0: of a warp's): how many above, and equal << 16
+    int run_equal[R > 0 ? 1 : WARPS];
+};
+// put(i, row): the i-th row that stays is `row` (-1: none), for every i below P.keep, by the threads of a CTA; sh.hist is clear.
 // R * THREADS weights at most, R of them in a thread's registers: position k * THREADS + thread.  R == 0: any number, read anew in every pass
 // (the positions of a warp then lie side by side in the last two).
-template <int R>
-__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
-    constexpr int RUNS = R > 0 ? R * WARPS : WARPS;
-    __shared__ int hist[BINS], warp_sum[WARPS], found[2];
-    __shared__ uint32_t run_sum[RUNS];                       // of 32 positions (R == 0: of a warp's): how many above, and equal << 16
-    __shared__ int run_equal[R > 0 ? 1 : WARPS];
-    const int item = blockIdx.x, b = item / P.KV_H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
-    pdl_wait();
-    pdl_launch_dependents();                                 // (what ran before is complete: a copy that needs nothing of this kernel may go on)
-    const int len = length_of(P, b, threadIdx.x == 0 && item == b * P.KV_H);
-    int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
-    if (threadIdx.x == 0 && item == b * P.KV_H) P.new_len[b] = min(len, P.keep);
+template <int R, typename Put>
+__device__ __forceinline__ void select(const Params& P, SelectShared<R>& sh, int item, int len, const Put& put) {
+    int (&hist)[BINS] = sh.hist, (&warp_sum)[WARPS] = sh.warp_sum, (&found)[2] = sh.found;
+    auto& run_sum = sh.run_sum;
+    auto& run_equal = sh.run_equal;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (len <= P.keep) {
-        for (int i = threadIdx.x; i < P.keep; i += THREADS) kept[i] = i < len ? i : -1;
+        for (int i = threadIdx.x; i < P.keep; i += THREADS) put(i, i < len ? i : -1);
         return;
     }
     // len > keep >= sinks + recent: the three parts do not meet
@@ -103,8 +107,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
 #pragma unroll
         for (int k = 0; k < R; ++k) u[k] = order_of(x[k]);
     }
-    for (int i = threadIdx.x; i < P.sinks; i += THREADS) kept[i] = i;
-    for (int i = threadIdx.x; i < P.recent; i += THREADS) kept[P.keep - P.recent + i] = last + i;
+    for (int i = threadIdx.x; i < P.sinks; i += THREADS) put(i, i);
+    for (int i = threadIdx.x; i < P.recent; i += THREADS) put(P.keep - P.recent + i, last + i);
     if (want == 0) return;
     __syncthreads();
     // the integer form of the want-th largest: `prefix` holds the digits found, `left` how many are wanted of those that share them
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
             const uint32_t is_above = __ballot_sync(0xffffffffu, u[k] > prefix), is_equal = __ballot_sync(0xffffffffu, u[k] == prefix);
             const uint32_t before = run_sum[k * WARPS + warp];
             const int a = static_cast<int>(before & 0xffffu) + __popc(is_above & below), e = static_cast<int>(before >> 16) + __popc(is_equal & below);
-            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + k * THREADS + threadIdx.x;
+            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) put(P.sinks + a + min(e, left), first + k * THREADS + static_cast<int>(threadIdx.x));
         }
     } else {
         const int run = (count + WARPS * 32 - 1) / (WARPS * 32) * 32, r0 = min(count, warp * run), r1 = min(count, r0 + run);
@@ -183,10 +187,64 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
             const uint32_t x = i < r1 ? order_of(__ldcg(w + i)) : 0u;
             const uint32_t is_above = __ballot_sync(0xffffffffu, i < r1 && x > prefix), is_equal = __ballot_sync(0xffffffffu, i < r1 && x == prefix);
             const int a = above + __popc(is_above & below), e = equal + __popc(is_equal & below);
-            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) kept[P.sinks + a + min(e, left)] = first + i;
+            if ((is_above >> lane & 1u) || ((is_equal >> lane & 1u) && e < left)) put(P.sinks + a + min(e, left), first + i);
             above += __popc(is_above);
             equal += __popc(is_equal);
         }
+    }
+}
+
+template <int R>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
+    __shared__ SelectShared<R> sh;
+    const int item = blockIdx.x, b = item / P.KV_H;
+    for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hist[i] = 0;
+    pdl_wait();
+    pdl_launch_dependents();                                 // (what ran before is complete: a copy that needs nothing of this kernel may go on)
+    const int len = length_of(P, b, threadIdx.x == 0 && item == b * P.KV_H);
+    int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
+    if (threadIdx.x == 0 && item == b * P.KV_H) P.new_len[b] = min(len, P.keep);
+    select<R>(P, sh, item, len, [&](int i, int row) { kept[i] = row; });
+}
+
+// Few items, another cache: selection and copy in one launch.  Grid (CTAs of an item, items): every CTA of an item selects for itself, on SMs that would
+// be idle, and copies its share of the rows, P.share of them, whose places it keeps in shared memory.  One launch / two, cold: 8 items of 2048 of 8000
+// rows 16.4 / 18.4 us (calls from Python 17.9 / 20.1), 2 of 500 10.3 / 12.3, 72 of 2048 40.8 / 41.0; 72 of 4096 of 16000 74.1 / 69.7, 8 of 8192 of 32000 42.9 / 38.1.
+template <int R>
+__global__ void __launch_bounds__(THREADS) evict_one_kernel(const Params P) {
+    pdl_launch_dependents();
+    extern __shared__ int32_t list[];
+    __shared__ SelectShared<R> sh;
+    const int item = blockIdx.y, b = item / P.KV_H, row0 = blockIdx.x * P.share, rows = min(P.share, P.keep - row0);
+    for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hist[i] = 0;
+    pdl_wait();
+    const bool tells = threadIdx.x == 0 && blockIdx.x == 0 && item == b * P.KV_H;
+    const int len = length_of(P, b, tells);
+    if (tells) P.new_len[b] = min(len, P.keep);
+    if (rows <= 0) return;                                   // (the last CTAs of an item whose rows the others have)
+    select<R>(P, sh, item, len, [&](int i, int row) {
+        if (i >= row0 && i < row0 + rows) list[i - row0] = row;
+    });
+    __syncthreads();
+    const int64_t src = static_cast<int64_t>(item) * P.S, dst = static_cast<int64_t>(item) * P.S_out + row0;
+    const int half = P.D / 8, shift = P.D == 64 ? 4 : (P.D == 128 ? 5 : 6), pieces = 1 << shift;      // of a row of K, of both
+    constexpr int UNROLL = 4;
+    for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += THREADS * UNROLL) {
+        uint4 x[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = i0 + u * THREADS, r = i >> shift, p = i & (pieces - 1);
+            if (i < rows * pieces && list[r] >= 0) x[u] = __ldcg(reinterpret_cast<const uint4*>((p < half ? P.k : P.v) + (src + list[r]) * P.D) + (p & (half - 1)));
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int i = i0 + u * THREADS, r = i >> shift, p = i & (pieces - 1);
+            if (i < rows * pieces && list[r] >= 0) __stcg(reinterpret_cast<uint4*>((p < half ? P.k_out : P.v_out) + (dst + r) * P.D) + (p & (half - 1)), x[u]);
+        }
+    }
+    for (int i = threadIdx.x; i < rows; i += THREADS) {
+        P.kept[static_cast<int64_t>(item) * P.keep + row0 + i] = list[i];
+        if (list[i] >= 0) P.w_out[dst + i] = __ldcg(P.w + src + list[i]);
     }
 }
 
@@ -338,16 +396,24 @@ extern "C" int alloyb_kv_evict(const void* k, const void* v, const float* weight
     P.len = lengths; P.len_count = lengths_count;
     P.k_out = static_cast<__half*>(k_out); P.v_out = static_cast<__half*>(v_out); P.w_out = weights_out;
     P.kept = kept; P.new_len = new_lengths;
-    P.B = B; P.KV_H = KV_H; P.S = S; P.S_out = S_out; P.keep = keep; P.sinks = sinks; P.recent = recent;
+    P.B = B; P.KV_H = KV_H; P.D = D; P.S = S; P.S_out = S_out; P.keep = keep; P.sinks = sinks; P.recent = recent;
     cudaStream_t st = as_stream(stream);
     // as many weights in registers as a cache of S positions can ask for (16384: 22 us from shared memory); past 32 a thread: none
-    auto select = S <= 8 * ev::THREADS ? ev::evict_select_kernel<8> : S <= 16 * ev::THREADS ? ev::evict_select_kernel<16> : S <= 32 * ev::THREADS ? ev::evict_select_kernel<32> : ev::evict_select_kernel<0>;
-    cudaError_t e = launch_pdl(select, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), 0, st, P);
-    if (e == cudaSuccess) {
-        switch (D) {
-            case 64: e = ev::copy<64>(P, in_place, st); break;
-            case 128: e = ev::copy<128>(P, in_place, st); break;
-            default: e = ev::copy<256>(P, in_place, st); break;
+    const int held = S <= 8 * ev::THREADS ? 8 : S <= 16 * ev::THREADS ? 16 : S <= 32 * ev::THREADS ? 32 : 0;
+    const int sharers = static_cast<int>(ev::SMS / items);
+    P.share = sharers > 1 ? (keep + sharers - 1) / sharers : 0;
+    cudaError_t e;
+    if (!in_place && sharers > 1 && (held == 8 || held == 16) && items * keep <= ev::ONE_ROWS && P.share <= ev::SHARE_MOST) {
+        e = launch_pdl(held == 8 ? ev::evict_one_kernel<8> : ev::evict_one_kernel<16>, dim3(sharers, static_cast<unsigned>(items)), dim3(ev::THREADS), static_cast<size_t>(P.share) * 4, st, P);
+    } else {
+        auto select = held == 8 ? ev::evict_select_kernel<8> : held == 16 ? ev::evict_select_kernel<16> : held == 32 ? ev::evict_select_kernel<32> : ev::evict_select_kernel<0>;
+        e = launch_pdl(select, dim3(static_cast<unsigned>(items)), dim3(ev::THREADS), 0, st, P);
+        if (e == cudaSuccess) {
+            switch (D) {
+                case 64: e = ev::copy<64>(P, in_place, st); break;
+                case 128: e = ev::copy<128>(P, in_place, st); break;
+                default: e = ev::copy<256>(P, in_place, st); break;
+            }
         }
     }
     if (e != cudaSuccess) {

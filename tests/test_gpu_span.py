@@ -332,6 +332,34 @@ def evict_case(b, kv_h, s, s_out, d, lengths, kind="random", seed=0):
     return k, v, w
 
 
+def evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place):
+    k, v, w = evict_case(b, kv_h, s, keep, d, lengths, kind)
+    kd, vd, wd = k.to(DEV), v.to(DEV), w.to(DEV)
+    if in_place:
+        ko, vo, wo = kd, vd, wd
+    else:
+        room = keep + 3
+        ko, vo = (torch.full((b, kv_h, room, d), 7.0, dtype=torch.float16, device=DEV) for _ in range(2))
+        wo = torch.full((b, kv_h, room), 7.0, device=DEV)
+    sent, lengths = lengths, [n if 0 <= n <= s else 0 for n in lengths]                # out of range counts as 0, and is told
+    before = [t.cpu().clone() for t in (ko, vo, wo)]
+    kept, new = OPS.kv_evict(kd, vd, wd, torch.tensor(sent, dtype=torch.int32, device=DEV), ko, vo, wo, keep, sinks, recent)
+    assert new.tolist() == [min(n, keep) for n in lengths]
+    kept = kept.cpu()
+    for i in range(b):
+        for h in range(kv_h):
+            rows = R.evict(w[i, h].tolist(), lengths[i], keep, sinks, recent)
+            assert kept[i, h].tolist() == rows + [-1] * (keep - len(rows))
+            for src, was in zip((k, v, w), before):
+                was[i, h, :len(rows)] = src[i, h, rows]
+    for t, want in zip((ko, vo, wo), before):
+        ints = torch.int16 if t.dtype == torch.float16 else torch.int32
+        assert torch.equal(t.cpu().view(ints), want.view(ints))
+    if not in_place:
+        assert torch.equal(kd.cpu().view(torch.int16), k.view(torch.int16))
+    assert ops.span_status() == (0 if sent == lengths else 2)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("b,kv_h,s,d,lengths,keep,sinks,recent,kind", [
     (1, 2, 300, 128, [300], 100, 4, 20, "random"),
@@ -351,30 +379,7 @@ def evict_case(b, kv_h, s, s_out, d, lengths, kind="random", seed=0):
     (1, 1, 70000, 64, [69999], 100, 10, 20, "odd"),
 ])
 def test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place):
-    k, v, w = evict_case(b, kv_h, s, keep, d, lengths, kind)
-    kd, vd, wd = k.to(DEV), v.to(DEV), w.to(DEV)
-    if in_place:
-        ko, vo, wo = kd, vd, wd
-    else:
-        room = keep + 3
-        ko, vo = (torch.full((b, kv_h, room, d), 7.0, dtype=torch.float16, device=DEV) for _ in range(2))
-        wo = torch.full((b, kv_h, room), 7.0, device=DEV)
-    before = [t.cpu().clone() for t in (ko, vo, wo)]
-    kept, new = OPS.kv_evict(kd, vd, wd, torch.tensor(lengths, dtype=torch.int32, device=DEV), ko, vo, wo, keep, sinks, recent)
-    assert new.tolist() == [min(n, keep) for n in lengths]
-    kept = kept.cpu()
-    for i in range(b):
-        for h in range(kv_h):
-            rows = R.evict(w[i, h].tolist(), lengths[i], keep, sinks, recent)
-            assert kept[i, h].tolist() == rows + [-1] * (keep - len(rows))
-            for src, was in zip((k, v, w), before):
-                was[i, h, :len(rows)] = src[i, h, rows]
-    for t, want in zip((ko, vo, wo), before):
-        ints = torch.int16 if t.dtype == torch.float16 else torch.int32
-        assert torch.equal(t.cpu().view(ints), want.view(ints))
-    if not in_place:
-        assert torch.equal(kd.cpu().view(torch.int16), k.view(torch.int16))
-    assert ops.span_status() == 0
+    evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place)
 
 
 @pytest.mark.parametrize("b,kv_h,s,d,lengths,keep,sinks,recent", [
@@ -386,8 +391,22 @@ def test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, kind, in_place):
     (5, 4, 3000, 128, [3000, 2048, 2049, 1, 2700], 2048, 4, 1500),
 ])
 def test_evict_many_recent_rows(b, kv_h, s, d, lengths, keep, sinks, recent):
-    test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, "random", False)
-    test_evict(b, kv_h, s, d, lengths, keep, sinks, recent, "ties", False)
+    evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, "random", False)
+    evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, "ties", False)
+
+
+@pytest.mark.parametrize("b,kv_h,s,d,lengths,keep,sinks,recent,kind", [
+    (10, 8, 900, 128, [900 - 7 * i for i in range(10)], 640, 1, 320, "random"),        # more items than half the SMs: two launches
+    (80, 1, 700, 64, [9 * i for i in range(80)], 300, 140, 150, "ties"),
+    (19, 4, 400, 256, [400 - i for i in range(19)], 200, 0, 200, "odd"),
+    (37, 2, 600, 128, [600] * 36 + [0], 130, 3, 0, "odd"),                             # half of them: two CTAs an item
+    (1, 75, 9000, 64, [8999], 700, 5, 129, "equal"),
+    (1, 1, 20000, 128, [19999], 147, 4, 30, "random"),                                 # a row a CTA, and none for the last
+    (3, 1, 500, 256, [500, 3, 40], 2, 1, 1, "random"),
+])
+def test_evict_by_items(b, kv_h, s, d, lengths, keep, sinks, recent, kind):
+    evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, kind, False)
+    evict_against_definition(b, kv_h, s, d, lengths, keep, sinks, recent, kind, True)
 
 
 def test_evict_length_out_of_range():
