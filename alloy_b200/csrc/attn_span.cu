@@ -16,7 +16,8 @@
 // nothing, and with a step's scores a step ahead of its softmax took 70 -> 82.  Many rows with much to do go to attn_span_tc.cu.
 //
 // The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and a
-// last launch adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.
+// launch of its own adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.  It joins the log-sums itself, so the
+// outputs are joined beside it (4 sequences of 16 tokens over 5000 to 8100 keys: 67 -> 60 us).
 //
 // New tokens' rows: keys from `pos` on are read from new_k / new_v, by every CTA that needs them, and written to the cache by one; nobody reads
 // them there in the same launch.
@@ -757,30 +758,27 @@ __device__ __forceinline__ Parts parts_of(const Params& P, int b, int kvh, int R
     return p;
 }
 
-// Grid (CTAs for the rows, sequences * KV heads); P.merge_team warps a row, 1 or all.  The scored form keeps the rows' log-sums.
+// Steps before a sequence, of it and those before, of all.
+__device__ __forceinline__ void steps_of(const Params& P, int b, int (&steps)[3]) {
+    steps[0] = __ldcg(P.cum + b);
+    steps[1] = __ldcg(P.cum + b + 1);
+    steps[2] = __ldcg(P.cum + P.B);
+}
+// P.merge_team warps a row, 1 or all.
 template <int D, bool STREAM>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
-    pdl_launch_dependents();
+__device__ __forceinline__ void join_rows(const Params& P) {
     __shared__ float4 sm[MERGE_WARPS * D / 4];                           // a warp's sums each
     __shared__ float sm_m[MERGE_WARPS], sm_l[MERGE_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, item = blockIdx.y, rows = P.n * P.G;
     const int b = item / P.KV_H, kvh = item - b * P.KV_H;
     const int team = P.merge_team;
-    pdl_wait();
     int steps[3] = {0, 0, 0};
-    if (STREAM) {                                                        // asked for along with the position, not behind it
-        steps[0] = __ldcg(P.cum + b);
-        steps[1] = __ldcg(P.cum + b + 1);
-        steps[2] = __ldcg(P.cum + P.B);
-    }
+    if (STREAM) steps_of(P, b, steps);                                   // asked for along with the position, not behind it
     const int pos = live_pos(P, b, false);
     const int R = (blockIdx.x * MERGE_WARPS + warp) / team, w0 = warp % team;
     if (R >= rows) return;                                               // (a whole CTA's row, or a warp's: nobody waits for it)
     const Parts p = parts_of<STREAM>(P, b, kvh, R, steps);
-    if (p.stored) {
-        if (P.row_lse && w0 == 0 && lane == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = __ldcg(P.part_lse + p.own_first);
-        return;
-    }
+    if (p.stored) return;
     // one pass: the parts' log-sums and outputs are asked for several at once, the running maximum and sum follow
     constexpr int E = D / 32 < 4 ? D / 32 : 4, PER = D / 32 / E;     // elements of a lane's access, accesses
     float m = -INFINITY, l = 0.f, acc[D / 32];
@@ -818,7 +816,6 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
     const int64_t out = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
     if (team == 1) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        if (P.row_lse && lane == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = l == 0.f ? -INFINITY : m + log2f(l);
 #pragma unroll
         for (int c = 0; c < PER; ++c) {
             const int64_t at = out + (c * 32 + lane) * E;
@@ -850,51 +847,84 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Para
             x = make_float4(fmaf(f, v.x, x.x), fmaf(f, v.y, x.y), fmaf(f, v.z, x.z), fmaf(f, v.w, x.w));
         }
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        if (P.row_lse && threadIdx.x == 0) P.row_lse[static_cast<int64_t>(item) * rows + R] = sum == 0.f ? -INFINITY : top + log2f(sum);
         store4(P.out, P.q_dtype, out + threadIdx.x * 4, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
 }
 
-// The weights of the scored form, once the rows' log-sums are known: a thread adds up four keys' probabilities, of up to 16 rows all, of more
-// rows (MANY) a quarter, in a fixed order.  Grid (key chunks, sequences * KV heads).
-template <bool MANY>
-struct Weights {
-    static constexpr int THREADS = 256, GROUPS = MANY ? 4 : 1, KEYS = THREADS * 4 / GROUPS;
-};
-template <bool MANY>
-__global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
-    using W = Weights<MANY>;
+// Grid (CTAs for the rows, sequences * KV heads).  BESIDE: behind the weights' kernel, which reads the same partial results and lets this one begin
+// once they are complete; the wait, for those who follow, comes last.
+template <int D, bool STREAM, bool BESIDE>
+__global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
     pdl_launch_dependents();
-    __shared__ float4 sm[MANY ? W::THREADS : 1];
-    const int item = blockIdx.y, rows = P.n * P.G, first_key = blockIdx.x * W::KEYS, group = threadIdx.x / (W::KEYS / 4);
-    const int j0 = first_key + threadIdx.x % (W::KEYS / 4) * 4;
+    if (!BESIDE) pdl_wait();
+    join_rows<D, STREAM>(P);
+    if (BESIDE) pdl_wait();
+}
+
+// The weights of the scored form: a CTA joins the rows' log-sums from their parts, and a thread adds up four keys' probabilities, of up to 16 rows
+// (STREAM) all, of more a quarter, in a fixed order.  Grid (key chunks, sequences * KV heads).
+template <bool STREAM>
+struct Weights {
+    static constexpr int THREADS = 256, GROUPS = STREAM ? 1 : 4, KEYS = THREADS * 4 / GROUPS;
+};
+template <bool STREAM>
+__global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
+    using W = Weights<STREAM>;
+    __shared__ float4 sm[STREAM ? 1 : W::THREADS];
+    __shared__ float lse[STREAM ? 16 : W::THREADS];
+    const int item = blockIdx.y, b = item / P.KV_H, kvh = item - b * P.KV_H, rows = P.n * P.G, first_key = blockIdx.x * W::KEYS;
+    const int group = threadIdx.x / (W::KEYS / 4), j0 = first_key + threadIdx.x % (W::KEYS / 4) * 4;
     float* weights = P.weights + static_cast<int64_t>(item) * P.S;
     const float* scores = P.scores + static_cast<int64_t>(item) * rows * P.pitch + j0;
-    const float* lse = P.row_lse + static_cast<int64_t>(item) * rows;
     pdl_wait();
-    const int pos = live_pos(P, item / P.KV_H, false), len = pos + P.n;
+    pdl_launch_dependents();
+    int steps[3] = {0, 0, 0};
+    if (STREAM) steps_of(P, b, steps);
+    const int pos = live_pos(P, b, false), len = pos + P.n;
     if (pos < 0 || first_key >= len) return;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (j0 + 3 <= pos) {                                                 // every row sees the four keys
-#pragma unroll 8
-        for (int r = group; r < rows; r += W::GROUPS) {
-            const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + r * P.pitch));
-            const float x = __ldcg(lse + r);
-            sum[0] += ex2(s.x - x);
-            sum[1] += ex2(s.y - x);
-            sum[2] += ex2(s.z - x);
-            sum[3] += ex2(s.w - x);
+    // the rows from r0 on, as many as fit
+    auto join_lse = [&](int r0) {
+        const int R = r0 + threadIdx.x;
+        if (static_cast<int>(threadIdx.x) < (STREAM ? 16 : W::THREADS) && R < rows) {
+            const Parts p = parts_of<STREAM>(P, b, kvh, R, steps);
+            float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < p.own; ++i) {
+                const float x = __ldcg(P.part_lse + p.own_index(i)), top = fmaxf(m, x);
+                if (x == -INFINITY) continue;                            // (an empty part)
+                l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + ex2(x - top);
+                m = top;
+            }
+            lse[threadIdx.x] = l == 0.f ? -INFINITY : m + log2f(l);
         }
-    } else if (j0 < len) {                                               // (a key behind the row's own position may have no score)
-        for (int r = group; r < rows; r += W::GROUPS) {
-            const float x = __ldcg(lse + r);
-            const int room = min(3, pos + r / P.G - j0);
+        __syncthreads();
+    };
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r0 = 0; r0 < rows; r0 += W::THREADS) {
+        if (r0 > 0) __syncthreads();
+        join_lse(r0);
+        const int r1 = min(rows, r0 + W::THREADS);
+        if (j0 + 3 <= pos) {                                             // every row sees the four keys
+#pragma unroll 8
+            for (int r = r0 + group; r < r1; r += W::GROUPS) {
+                const float4 s = __ldcg(reinterpret_cast<const float4*>(scores + r * P.pitch));
+                const float x = lse[r - r0];
+                sum[0] += ex2(s.x - x);
+                sum[1] += ex2(s.y - x);
+                sum[2] += ex2(s.z - x);
+                sum[3] += ex2(s.w - x);
+            }
+        } else if (j0 < len) {                                           // (a key behind the row's own position may have no score)
+            for (int r = r0 + group; r < r1; r += W::GROUPS) {
+                const float x = lse[r - r0];
+                const int room = min(3, pos + r / P.G - j0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e <= room) sum[e] += ex2(__ldcg(scores + r * P.pitch + e) - x);
+                for (int e = 0; e < 4; ++e)
+                    if (e <= room) sum[e] += ex2(__ldcg(scores + r * P.pitch + e) - x);
+            }
         }
     }
-    if (!MANY) {
+    if (STREAM) {
         if (P.S % 4 == 0 && reinterpret_cast<uintptr_t>(P.weights) % 16 == 0 && j0 + 3 < pos) {
             float4* to = reinterpret_cast<float4*>(weights + j0);
             const float4 was = __ldcg(to);
@@ -946,7 +976,7 @@ struct Plan {
     int cluster, cluster_steps;          // few rows, few steps: span_cluster_kernel with this many CTAs, of this many steps at most
     bool tc, pre_tc;                     // more rows, the own keys / the prefix: span_tc_kernel, not span_rows_kernel
     int ctas, splits, tiles, pre_splits, pre_tiles;
-    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, row_lse, bytes;    // byte offsets in the workspace
+    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;    // byte offsets in the workspace
     int64_t pitch;
 };
 
@@ -1042,7 +1072,6 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     if (scored) {
         p.pitch = (static_cast<int64_t>(S) + 3) / 4 * 4;
         p.scores = take(static_cast<size_t>(items) * rows * p.pitch * 4);
-        p.row_lse = take(static_cast<size_t>(items) * rows * 4);
     }
     p.bytes = at;
     return p;
@@ -1136,17 +1165,19 @@ static int run_d(const Plan& plan, const Params& P, cudaStream_t st) {
         rc = plan.tc ? launch_span_tc(P, D, false, dim3(plan.tiles * plan.splits, P.KV_H, P.B), st)
                      : launch(span_rows_kernel<D, SCORED>, dim3(plan.tiles * plan.splits, P.KV_H, P.B), WARPS * 32, TILES, TILES, ready[2], st, P);
     if (rc != ALLOYB_OK) return rc;
-    if (!plan.stream && plan.splits == 1 && !PREFIX && !SCORED) return check_launch();       // everything is stored
-    Params M = P;
-    // a CTA a row where it has many parts, and the GPU holds all of them at once (16 sequences of 4 heads behind 4096 rows: 4 us sooner); else
-    // a warp a row (64 sequences of 8 heads: 12 us sooner)
-    const int64_t parts = plan.pre_splits + (plan.stream ? plan.ctas / items + 2 : plan.splits);
-    M.merge_team = parts > MERGE_WARPS && static_cast<int64_t>(rows) * items <= 8 * SMS ? MERGE_WARPS : 1;
-    auto merge = plan.stream ? span_merge_kernel<D, true> : span_merge_kernel<D, false>;
-    cudaError_t e = launch_pdl(merge, dim3((rows * M.merge_team + MERGE_WARPS - 1) / MERGE_WARPS, items), dim3(MERGE_WARPS * 32), 0, st, M);
-    if (e == cudaSuccess && SCORED) {
-        const int keys = plan.stream ? Weights<false>::KEYS : Weights<true>::KEYS;
-        e = launch_pdl(plan.stream ? span_weights_kernel<false> : span_weights_kernel<true>, dim3((P.S + keys - 1) / keys, items), dim3(256), 0, st, P);
+    cudaError_t e = cudaSuccess;
+    if (SCORED) {
+        const int keys = plan.stream ? Weights<true>::KEYS : Weights<false>::KEYS;
+        e = launch_pdl(plan.stream ? span_weights_kernel<true> : span_weights_kernel<false>, dim3((P.S + keys - 1) / keys, items), dim3(256), 0, st, P);
+    }
+    if (e == cudaSuccess && (plan.stream || plan.splits > 1 || PREFIX)) {                    // (else every output is stored)
+        Params M = P;
+        // a CTA a row where it has many parts, and the GPU holds all of them at once (16 sequences of 4 heads behind 4096 rows: 4 us sooner); else
+        // a warp a row (64 sequences of 8 heads: 12 us sooner)
+        const int64_t parts = plan.pre_splits + (plan.stream ? plan.ctas / items + 2 : plan.splits);
+        M.merge_team = parts > MERGE_WARPS && static_cast<int64_t>(rows) * items <= 8 * SMS ? MERGE_WARPS : 1;
+        auto merge = plan.stream ? span_merge_kernel<D, true, SCORED> : span_merge_kernel<D, false, SCORED>;
+        e = launch_pdl(merge, dim3((rows * M.merge_team + MERGE_WARPS - 1) / MERGE_WARPS, items), dim3(MERGE_WARPS * 32), 0, st, M);
     }
     if (e != cudaSuccess) {
         set_cuda_error(e);
@@ -1217,7 +1248,6 @@ static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_
     }
     if (plan.pitch) {
         P.scores = reinterpret_cast<float*>(ws + plan.scores);
-        P.row_lse = reinterpret_cast<float*>(ws + plan.row_lse);
         P.pitch = plan.pitch;
     }
     return ALLOYB_OK;

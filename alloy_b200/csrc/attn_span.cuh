@@ -45,7 +45,6 @@ struct Params {
     int merge_team;                      // warps that join a row's partial results
     float* scores;                       // [sequence, KV head][row][pitch], log2 frame, for the weights
     int64_t pitch;
-    float* row_lse;                      // [sequence, KV head][row], for the weights
     float* weights;                      // (B, KV_H, S)
 };
 
