@@ -12,13 +12,13 @@
 //   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.
 // * Two buffers of scores and the output accumulators in tensor memory, half of it a CTA.  A thread has a row's 64 scores; P
 //   (fp16, rounded once) overwrites them, 32 keys at a time, and is read from there as the A operand.
-// * Which tiles every row of a warp sees is worked out once, not per tile (2048 tokens behind 6000 under a window of 4096: 172 -> 162 us).
+// * Which tiles every row of a warp sees is worked out once, not per tile (2048 tokens behind 6000 under a window of 4096, 32/8 heads, head_dim
+//   128: 172 -> 162 us).
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
 // The same call with one CTA an SM, 256 rows in two groups, tiles of 128 keys: one buffer of 128 scores and two threads a row, which have to
 // agree on the maximum, 155 us; two buffers of 64 and a thread a row 147; four warps for the even tiles of keys and four for the odd ones 163.
-// This takes 136 (1010 TFLOP/s of the products that the rows see; 512 tiles are 1.73 rounds); 64 sequences of 64/8 heads over a prefix of 32768
-// take 71 (970 TFLOP/s), both 32/8 heads or more and head_dim 128.  At head_dim 64 the softmax is the bound: 132 us for the first call with everything
-// around it, where head_dim 128 takes 150.
+// This takes 136 (1010 TFLOP/s of the products that the rows see; 512 tiles are 1.73 rounds), and 64 sequences of 64/8 heads over a prefix of 32768
+// 71 (970 TFLOP/s).  At head_dim 64 the softmax is the bound: the first call takes 132 us with everything around it, where head_dim 128 takes 150.
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
 #include <cuda.h>
 
