@@ -21,6 +21,8 @@
 //
 // New tokens' rows: keys from `pos` on are read from new_k / new_v, by every CTA that needs them, and written to the cache by one; nobody reads
 // them there in the same launch.
+#include <atomic>
+
 #include "attn_span.cuh"
 
 namespace alloyb {
@@ -705,14 +707,14 @@ __global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) 
     if (i < pre) span_rows<D, false, true>(P, i / P.pre_splits % tiles, tiles, i % P.pre_splits, P.pre_splits, i / (P.pre_splits * tiles), 0);
     else span_stream<D, false, true>(P, i - pre, P.ctas);
 }
-// The own keys behind a prefix that the 5th-generation tensor cores have.  Nothing here reads what that kernel writes, and its CTAs let this one
-// begin only once what ran before them is complete: so these CTAs take the SMs as those leave them, and the wait, for the join's sake, comes
-// last (64 sequences of 64/8 heads over 32768 shared keys and up to 1000 of their own: 146 -> 134 us).
+// The own keys behind a prefix that the 5th-generation tensor cores have.  Nothing here reads what that kernel writes, so
+// these CTAs take the SMs as those leave them (64 sequences of 64/8 heads over 32768 shared keys and up to 1000 of their own: 146 -> 134 us).
 template <int D>
 __global__ void __launch_bounds__(WARPS * 32, D == 64 ? 3 : (D == 128 ? 2 : 1)) span_stream_prefix_kernel(const Params P) {
     pdl_launch_dependents();
+    wait_unless_begun(P);
     span_stream<D, false, true>(P, blockIdx.x, gridDim.x);
-    pdl_wait();
+    end_behind(P, blockIdx.x == 0 && threadIdx.x == 0);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- joining
@@ -851,14 +853,14 @@ __device__ __forceinline__ void join_rows(const Params& P) {
     }
 }
 
-// Grid (CTAs for the rows, sequences * KV heads).  BESIDE: behind the weights' kernel, which reads the same partial results and lets this one begin
-// once they are complete; the wait, for those who follow, comes last.
+// Grid (CTAs for the rows, sequences * KV heads).  BESIDE: behind the weights' kernel, which reads the same partial results.
 template <int D, bool STREAM, bool BESIDE>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) span_merge_kernel(const Params P) {
     pdl_launch_dependents();
-    if (!BESIDE) pdl_wait();
+    if (BESIDE) wait_unless_begun(P);
+    else pdl_wait();
     join_rows<D, STREAM>(P);
-    if (BESIDE) pdl_wait();
+    if (BESIDE) end_behind(P, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0);
 }
 
 // The weights of the scored form: a CTA joins the rows' log-sums from their parts, and a thread adds up four keys' probabilities, of up to 16 rows
@@ -877,6 +879,10 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
     float* weights = P.weights + static_cast<int64_t>(item) * P.S;
     const float* scores = P.scores + static_cast<int64_t>(item) * rows * P.pitch + j0;
     pdl_wait();
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        if (threadIdx.x == 0) tell_begun(P);
+        __syncthreads();
+    }
     pdl_launch_dependents();
     int steps[3] = {0, 0, 0};
     if (STREAM) steps_of(P, b, steps);
@@ -976,7 +982,7 @@ struct Plan {
     int cluster, cluster_steps;          // few rows, few steps: span_cluster_kernel with this many CTAs, of this many steps at most
     bool tc, pre_tc;                     // more rows, the own keys / the prefix: span_tc_kernel, not span_rows_kernel
     int ctas, splits, tiles, pre_splits, pre_tiles;
-    size_t cum, part_lse, part_o, pre_lse, pre_o, scores, bytes;    // byte offsets in the workspace
+    size_t cum, begun, part_lse, part_o, pre_lse, pre_o, scores, bytes;    // byte offsets in the workspace
     int64_t pitch;
 };
 
@@ -1061,6 +1067,7 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         return here;
     };
     p.cum = take((static_cast<size_t>(B) + 1) * 4);
+    p.begun = take(8);
     p.part_lse = take(lse_rows * 4);
     p.part_o = take(o_rows * D * 4);
     if (P > 0) {
@@ -1237,6 +1244,9 @@ static int place(Params& P, const Plan& plan, void* workspace, size_t workspace_
     if (workspace_bytes < plan.bytes) return ALLOYB_E_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     P.cum = reinterpret_cast<int*>(ws + plan.cum);
+    static std::atomic<unsigned long long> calls{0};
+    P.begun = reinterpret_cast<unsigned long long*>(ws + plan.begun);
+    P.call = ++calls * 0x9e3779b97f4a7c15ull;                            // (odd: no two calls alike, and no number that lies about)
     P.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
     P.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     P.ctas = plan.ctas; P.splits = plan.splits; P.tiles = plan.tiles; P.pre_splits = plan.pre_splits;

@@ -46,7 +46,24 @@ struct Params {
     float* scores;                       // [sequence, KV head][row][pitch], log2 frame, for the weights
     int64_t pitch;
     float* weights;                      // (B, KV_H, S)
+    unsigned long long *begun, call;     // *begun == call: what ran before this call is complete, and so is what its earlier launches wait for
 };
+
+// Launches that begin beside the launch ahead of them, whose results they do not need.  That launch tells, behind its own wait, that what ran
+// before is complete (one CTA of it, ahead of letting others begin); where nothing is told yet, as when another thread's launch came in between on the stream,
+// the launch waits first, as all others do.  Either way it waits at its end: its end is the end of what lies before it.
+__device__ __forceinline__ void tell_begun(const Params& P) {
+    *static_cast<volatile unsigned long long*>(P.begun) = P.call;
+    __threadfence();
+}
+__device__ __forceinline__ void wait_unless_begun(const Params& P) {
+    if (*static_cast<volatile unsigned long long*>(P.begun) != P.call) pdl_wait();
+    __threadfence();
+}
+__device__ __forceinline__ void end_behind(const Params& P, bool last) {
+    pdl_wait();
+    if (last) *static_cast<volatile unsigned long long*>(P.begun) = 0;       // a graph's next replay begins anew
+}
 
 // One sequence of a call: the keys its tokens tok0 .. tok1 - 1 see, as one run of `keys` places: `sink` first rows, then rows from lo on.
 struct Seq {

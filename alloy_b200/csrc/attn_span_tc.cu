@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(THREADS, 2) span_tc_kernel(const __grid_consta
     // Tensor memory behind the wait, and what follows may begin only once every CTA has its own: a CTA of the launch before or behind that
     // shares the SM could otherwise wait for the columns that this one holds while this one waits for it.
     pdl_wait();
+    if (PREFIX && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) sp::tell_begun(P);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&bars->tmem_base)), "r"(C::COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -510,8 +511,9 @@ static int launch(dim3 grid, cudaStream_t st, const Params& P) {
     a.p = P;
     if (e == cudaSuccess) {
         const int64_t rows = PREFIX ? P.P : P.S, heads = PREFIX ? P.KV_H : static_cast<int64_t>(P.B) * P.KV_H, apart = PREFIX && P.KV_H > 1 ? P.p_hs : rows * D;
-        if (!map_rows(&a.k, PREFIX ? P.pk : P.k, D, rows, heads, apart) || !map_rows(&a.v, PREFIX ? P.pv : P.v, D, rows, heads, apart))
-            e = cudaErrorInvalidValue;
+        auto map = [&] { return map_rows(&a.k, PREFIX ? P.pk : P.k, D, rows, heads, apart) && map_rows(&a.v, PREFIX ? P.pv : P.v, D, rows, heads, apart); };
+        // (a host thread's first call of the driver may find no current context, which cudaSetDevice gives it)
+        if (!map() && ((e = cudaSetDevice(dev)) != cudaSuccess || !map())) e = e != cudaSuccess ? e : cudaErrorInvalidValue;
     }
     if (e == cudaSuccess && !PREFIX && P.nk) e = launch_pdl(span_append_kernel<D>, dim3((P.n + 2048 / D - 1) / (2048 / D), P.KV_H, P.B), dim3(256), 0, st, P);
     if (e == cudaSuccess) e = launch_pdl(kern, grid, dim3(THREADS), Cfg<D>::SMEM, st, a);

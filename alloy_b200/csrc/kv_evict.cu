@@ -5,7 +5,7 @@
 // evict_select_kernel, a CTA per (sequence, KV head): the weight that the last row to stay has is found digit by digit
 // (a histogram of eleven, eleven and ten bits of the weights in an order-preserving integer form), then the positions above it, and as many
 // of those equal to it as are wanted, are written in order.  evict_copy_kernel moves the rows.  Bound: HBM, two rows read and written a
-// kept position: 128 items of 4096 kept rows of 3000 to 16384 take 96 us, 5.5 TB/s.  Few items go in one launch (evict_one_kernel).
+// kept position: 128 items of 4096 kept rows of 3000 to 16384 take 98 us, 5.4 TB/s.  Few items go in one launch (evict_one_kernel).
 //
 // In place a row only moves towards the front: a CTA owns a slice of columns of one (sequence, KV head) and walks the positions in order,
 // all of a batch read before any of it is written, so no row is overwritten before it is read.
@@ -196,11 +196,11 @@ __device__ __forceinline__ void select(const Params& P, SelectShared<R>& sh, int
 
 template <int R>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const Params P) {
+    pdl_launch_dependents();
     __shared__ SelectShared<R> sh;
     const int item = blockIdx.x, b = item / P.KV_H;
     for (int i = threadIdx.x; i < BINS; i += THREADS) sh.hist[i] = 0;
     pdl_wait();
-    pdl_launch_dependents();                                 // (what ran before is complete: a copy that needs nothing of this kernel may go on)
     const int len = length_of(P, b, threadIdx.x == 0 && item == b * P.KV_H);
     int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
     if (threadIdx.x == 0 && item == b * P.KV_H) P.new_len[b] = min(len, P.keep);
@@ -249,9 +249,6 @@ __global__ void __launch_bounds__(THREADS) evict_one_kernel(const Params P) {
 }
 
 // Another cache: every position on its own.  A warp takes UNROLL rounds of 32 pieces of 16 bytes, K's and V's of a position side by side.
-// The recent rows are known without the selection, and are copied beside it: they come first in the grid, and only CTAs with rows that the
-// selection names wait for it before they copy (128 items of 4096 kept rows, 512 of them recent, cold: 104.5 -> 102 us; with an item's blocks
-// a whole grid of items apart, 108.6).
 constexpr int COPY_THREADS = 256, UNROLL = 8;
 template <int D>
 struct CopyCfg {
@@ -261,14 +258,10 @@ template <int D>
 __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const Params P) {
     using C = CopyCfg<D>;
     pdl_launch_dependents();
-    const int items = P.B * P.KV_H, blocks = static_cast<int>(gridDim.x) / items, back = P.recent / C::ROWS, rest = blocks - back;
-    const int i = static_cast<int>(blockIdx.x) - back * items;           // the last `back` blocks of rows of every item, then the others
-    const int item = i < 0 ? static_cast<int>(blockIdx.x) / back : i / rest, row0 = (i < 0 ? rest + static_cast<int>(blockIdx.x) % back : i % rest) * C::ROWS;
-    const int len = length_of(P, item / P.KV_H, false), n = min(len, P.keep);
-    const int mid0 = len <= P.keep ? n : P.sinks, mid1 = len <= P.keep ? n : P.keep - P.recent;      // rows that the selection names
-    const bool early = row0 >= mid1 || row0 + C::ROWS <= mid0;
-    auto row_at = [&](int row, const int32_t* kept) { return row < mid0 ? row : (row < mid1 ? __ldcg(kept + row) : row + len - n); };
-    if (!early) pdl_wait();
+    const int item = blockIdx.y, row0 = blockIdx.x * C::ROWS;
+    pdl_wait();
+    const int n = min(length_of(P, item / P.KV_H, false), P.keep);
+    if (row0 >= n) return;
     const int32_t* kept = P.kept + static_cast<int64_t>(item) * P.keep;
     const int64_t src = static_cast<int64_t>(item) * P.S, dst = static_cast<int64_t>(item) * P.S_out;
     uint4 x[UNROLL];
@@ -276,7 +269,7 @@ __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const Params P
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
         const int row = row0 + (u * COPY_THREADS + threadIdx.x) / C::PIECES;
-        at[u] = row < n ? row_at(row, kept) : -1;
+        at[u] = row < n ? __ldcg(kept + row) : -1;
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -291,8 +284,7 @@ __global__ void __launch_bounds__(COPY_THREADS) evict_copy_kernel(const Params P
         if (at[u] >= 0) __stcg(reinterpret_cast<uint4*>(to + (dst + row) * D) + p % (D / 8), x[u]);
     }
     for (int i = threadIdx.x; i < C::ROWS && row0 + i < n; i += COPY_THREADS)
-        P.w_out[dst + row0 + i] = __ldcg(P.w + src + row_at(row0 + i, kept));
-    if (early) pdl_wait();                                   // this launch's end is the selection's too
+        P.w_out[dst + row0 + i] = __ldcg(P.w + src + __ldcg(kept + row0 + i));
 }
 
 // The same cache: grid (slices of 32 bytes of K's and of V's columns, and one for the weights; sequences * KV heads).
@@ -347,7 +339,7 @@ template <int D>
 static cudaError_t copy(const Params& P, bool in_place, cudaStream_t st) {
     const int items = P.B * P.KV_H;
     if (in_place) return launch_pdl(evict_move_kernel<D>, dim3(2 * (D / 16) + 1, items), dim3(COPY_THREADS), 0, st, P);
-    return launch_pdl(evict_copy_kernel<D>, dim3((P.keep + CopyCfg<D>::ROWS - 1) / CopyCfg<D>::ROWS * items), dim3(COPY_THREADS), 0, st, P);
+    return launch_pdl(evict_copy_kernel<D>, dim3((P.keep + CopyCfg<D>::ROWS - 1) / CopyCfg<D>::ROWS, items), dim3(COPY_THREADS), 0, st, P);
 }
 
 }  // namespace ev

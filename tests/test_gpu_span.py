@@ -1,6 +1,8 @@
 """Attention over a window with sinks, behind a shared prefix and with its weights kept, and eviction by those weights, against their
 definitions in 64 bits."""
 
+import threading
+
 import pytest
 import torch
 
@@ -543,6 +545,55 @@ def test_calls_in_a_row():
             for x, y in zip(a, z):
                 bits = torch.int16 if x.element_size() == 2 else torch.int32
                 assert torch.equal(x.view(bits), y.view(bits))
+
+
+def test_two_threads_on_one_stream():
+    """Launches of two threads' calls may alternate on the stream that they share; each call still gives its own bits."""
+    p = 14001
+    behind = Case(70, 8, 2, 128, 1, 32, [(i * 5) % 32 for i in range(70)], prefix=p)
+    pk, pv = behind.pk.to(DEV), behind.pv.to(DEV)
+    step = Case(40, 16, 8, 128, 1, 300, [(i * 37) % 300 for i in range(40)])
+    chunk = Case(2, 32, 8, 64, 12, 900, [700, 880])
+    weights = {c: torch.rand(c.b, c.kv_h, c.s, generator=torch.Generator().manual_seed(3)).to(DEV) for c in (step, chunk)}
+    caches = {c: [x.to(DEV) for x in (c.k, c.v)] for c in (behind, step, chunk)}
+    pos = {c: c.pos_t() for c in caches}
+    threads, rounds = 2, 60
+
+    def prefix():
+        return (OPS.attention_shared_prefix(behind.q, behind.nk, behind.nv, pos[behind], pk, pv, *caches[behind], -1.0, False),)
+
+    def scored(c):
+        w = weights[c].clone()
+        return OPS.attention_cache_scored(c.q, c.nk, c.nv, pos[c], *caches[c], w, -1.0, False), w
+
+    calls = [prefix, lambda: scored(step), lambda: scored(chunk)]
+    alone = []
+    for f in calls:
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in f()])
+        torch.cuda.synchronize()
+    got, failed, start = [[] for _ in range(threads)], [], threading.Barrier(threads)
+
+    def work(i):
+        try:
+            start.wait()
+            for n in range(rounds):
+                k = (n + i) % len(calls)
+                got[i].append((k, calls[k]()))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    pool = [threading.Thread(target=work, args=(i,)) for i in range(threads)]
+    for t in pool:
+        t.start()
+    for t in pool:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for k, results in (x for g in got for x in g):
+        for x, y in zip(alone[k], results):
+            bits = torch.int16 if x.element_size() == 2 else torch.int32
+            assert torch.equal(x.view(bits), y.view(bits))
 
 
 def test_same_bits_again_and_on_another_stream():
