@@ -147,7 +147,7 @@ __device__ __forceinline__ void span_segment(const Params& P, StreamShared& sh, 
                         if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < sq.keys)
                             put(g + 8 * rr, place0 + 8 * n + 2 * t, make_float2(s[n][2 * rr], s[n][2 * rr + 1]));
             }
-            st.template take<1, true>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
+            st.template take<1>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
         }
         __syncwarp();                                                // the slot has been read: the next request may fill it
     }
@@ -367,7 +367,7 @@ __device__ __forceinline__ void span_stream(const Params& P, int cta, int ctas) 
                         if (g + 8 * rr < rows && place0 + 8 * n + 2 * t < at.sq.keys)
                             *reinterpret_cast<float2*>(to + (g + 8 * rr) * P.pitch + 8 * n) = make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
             }
-            st.template take<1, true>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
+            st.template take<1>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
         }
         __syncwarp();                                                    // the slot has been read: the next request may fill it
         if (++at.step < at.steps && i + 1 < count) continue;
@@ -658,7 +658,7 @@ __device__ __forceinline__ void span_rows(const Params& P, int tile, int tiles, 
                         *reinterpret_cast<float2*>(P.scores + (static_cast<int64_t>(item) * rows + r_own[rr]) * P.pitch + place0 + 8 * n + 2 * t) =
                             make_float2(s[n][2 * rr], s[n][2 * rr + 1]);
         }
-        st.template take<KT / 16, false>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
+        st.template take<KT / 16>(s, k_tile + C::TILE + Rows<D>::v_lane(lane));
         __syncthreads();                                                 // the tile has been read: its stage may be refilled
     }
     copy_wait<0>();

@@ -264,7 +264,7 @@ struct Rows {
         }
     }
     // s: scores in the log2 frame, -inf where a row does not see the key (a NaN score makes the row NaN); v_at: the tile's address plus v_lane
-    template <int NK, bool FINE>
+    template <int NK>
     __device__ __forceinline__ void take(float (&s)[2 * NK][4], uint32_t v_at) {
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -299,9 +299,8 @@ struct Rows {
         }
 #pragma unroll
         for (int k2 = 0; k2 < NK; ++k2) {
-            // P enters the product as fp16, the sum l is of the unrounded weights.  FINE: as two halves, which keep 22 bits of a weight (few rows,
-            // where HBM is the bound: nothing at 4096 keys and 32 sequences, 3 to 6 % of the smallest calls); else rounded once (2^-11 of each weight at most: an output's error from it stays below half a step of an fp16
-            // output that does not cancel)
+            // P enters the product as two fp16 halves, which keep 22 bits of a weight (as in the framework's other attention: a call's accuracy does
+            // not go by how many rows it has); the sum l is of the unrounded weights
             uint32_t p[4], low[4];
 #pragma unroll
             for (int nn = 0; nn < 2; ++nn) {
@@ -311,11 +310,9 @@ struct Rows {
                 l[1] += p2 + p3;
                 p[2 * nn] = pack_h2(p0, p1);
                 p[2 * nn + 1] = pack_h2(p2, p3);
-                if (FINE) {
-                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&p[2 * nn])), b = __half22float2(*reinterpret_cast<const __half2*>(&p[2 * nn + 1]));
-                    low[2 * nn] = pack_h2(p0 - a.x, p1 - a.y);
-                    low[2 * nn + 1] = pack_h2(p2 - b.x, p3 - b.y);
-                }
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&p[2 * nn])), b = __half22float2(*reinterpret_cast<const __half2*>(&p[2 * nn + 1]));
+                low[2 * nn] = pack_h2(p0 - a.x, p1 - a.y);
+                low[2 * nn + 1] = pack_h2(p2 - b.x, p3 - b.y);
             }
 #pragma unroll
             for (int n2 = 0; n2 < D / 16; ++n2) {
@@ -323,10 +320,8 @@ struct Rows {
                 ldsm_x4_t((v_at ^ (n2 << 5)) + k2 * 16 * D * 2, b);
                 mma16816(o[2 * n2], p, b[0], b[1]);
                 mma16816(o[2 * n2 + 1], p, b[2], b[3]);
-                if (FINE) {
-                    mma16816(o[2 * n2], low, b[0], b[1]);
-                    mma16816(o[2 * n2 + 1], low, b[2], b[3]);
-                }
+                mma16816(o[2 * n2], low, b[0], b[1]);
+                mma16816(o[2 * n2 + 1], low, b[2], b[3]);
             }
         }
     }
