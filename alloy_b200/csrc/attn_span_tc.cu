@@ -1,24 +1,25 @@
 // Attention of many query rows over spans of an fp16 cache on the 5th-generation tensor cores (head_dim 64 and 128): the chunks of a
 // prompt under a window, and a large batch's rows over a shared prefix.  attn_span.cu has the rest, and joins partial results.
 //
-// What bounds it: 128 rows x 64 keys take 512 clocks of the tensor pipe at head_dim 128 (S and P V), and their 8192 exponentials 512 clocks of
-// the SM's sixteen a clock; neither is reached in a short call, since scores, exponentials and P V of a row wait for one another (about 1100 clocks from P to
-// the next scores in the softmax's hands, and as many for the softmax).  So an SM has two CTAs, and a CTA two tiles of scores: while the softmax
-// has one, the tensor pipe has the other one's products and the other CTA's.  In calls one after another for a second the 1000 W limit is the bound:
-// the SM clock falls from 1.9 to 1.65 GHz.
+// What bounds it: 128 rows x 64 keys take 768 clocks of the tensor pipe at head_dim 128 (S, and P V twice), and their 8192 exponentials 512 clocks of
+// the SM's sixteen a clock; neither is reached in a short call, since scores, exponentials and P V of a row wait for one another.  So an SM has two
+// CTAs, and a CTA two tiles of scores: while the softmax has one, the tensor pipe has the other one's products and the other CTA's.  In calls one
+// after another for a second the 1000 W limit is the bound.
 //
 // * Q (128 rows), K and V tiles of 64 keys in shared memory, 128-byte swizzle, K and V in two stages by TMA.  Tiles that are not 64 rows
 //   in one piece (the first rows, the end of a sequence) come in by cp.async, places past the last key zero-filled: what a cache holds there
 //   is nobody's business.  K is a K-major operand, V an MN-major one, so neither is transposed.
-// * Two buffers of scores and the output accumulators in tensor memory, half of it a CTA.  A thread has a row's 64 scores; P
-//   (fp16, rounded once) overwrites them, 32 keys at a time, and is read from there as the A operand.
+// * Two buffers of scores and the output accumulators in tensor memory, half of it a CTA.  A thread has a row's 64 scores; P, as two
+//   fp16 halves (22 bits of a weight, as in the framework's other attention), overwrites them, 32 keys at a time: the high halves take the first 32
+//   columns, the low ones the others, and both are read from there as A operands.
 // * Which tiles every row of a warp sees is worked out once, not per tile (2048 tokens behind 6000 under a window of 4096, 32/8 heads, head_dim
 //   128: 172 -> 162 us).
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
-// The same call with one CTA an SM, 256 rows in two groups, tiles of 128 keys: one buffer of 128 scores and two threads a row, which have to
-// agree on the maximum, 155 us; two buffers of 64 and a thread a row 147; four warps for the even tiles of keys and four for the odd ones 163.
-// This takes 136 (1010 TFLOP/s of the products that the rows see; 512 tiles are 1.73 rounds), and 64 sequences of 64/8 heads over a prefix of 32768
-// 71 (970 TFLOP/s).  At head_dim 64 the softmax is the bound: the first call takes 132 us with everything around it, where head_dim 128 takes 150.
+// Two CTAs of 128 rows, a thread a row, two buffers of 64 scores; measured while P was one half: 136 us for the kernel of that call, where one CTA an
+// SM of 256 rows took 147 to 155, and four warps for the even tiles of keys and four for the odd ones 163.  With both halves of P the call takes 182 us
+// cold (152 with one half; 742 TFLOP/s of the products that the rows see), 64 sequences of 64/8 heads over a prefix of 32768 with own keys and join
+// 141 (124); at head_dim 64 160 and 113.  P in pieces of 16 keys on its way to tensor memory keeps the softmax within 128 registers (head_dim 64,
+// the first call: 164 -> 160 us).
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.
 #include <cuda.h>
 
@@ -132,6 +133,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
         "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -277,7 +283,9 @@ __global__ void __launch_bounds__(THREADS, 2) span_tc_kernel(const __grid_consta
                             fence_after();
                             if (!ok) break;
                         }
-                        umma_ts(tmem + 2 * KT, tmem + h * KT + kk * 8, v_desc + ((s * TILE + kk * 2048) >> 4), umma_idesc(D, true), j > 0 || kk > 0, lead);
+                        const uint64_t vd = v_desc + ((s * TILE + kk * 2048) >> 4);
+                        umma_ts(tmem + 2 * KT, tmem + h * KT + kk * 8, vd, umma_idesc(D, true), j > 0 || kk > 0, lead);
+                        umma_ts(tmem + 2 * KT, tmem + h * KT + KT / 2 + kk * 8, vd, umma_idesc(D, true), 1, lead);
                     }
                     if (!ok) break;
                     umma_commit(&bars->v_empty[s], lead);
@@ -400,22 +408,27 @@ __global__ void __launch_bounds__(THREADS, 2) span_tc_kernel(const __grid_consta
             const uint64_t scale2 = f2(scale, scale), sub2 = f2(sub, sub);
             uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) {
-                uint32_t p[16];
+            for (int c = 0; c < KT / 16; ++c) {
+                uint32_t p[8], low[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 8; ++e) {
                     float x0, x1;
-                    unf2(f2_fma(f2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), scale2, sub2), x0, x1);
+                    unf2(f2_fma(f2(s[c * 16 + 2 * e], s[c * 16 + 2 * e + 1]), scale2, sub2), x0, x1);
                     x0 = ex2(x0);
                     x1 = ex2(x1);
                     sum[e & 1] = f2_add(sum[e & 1], f2(x0, x1));
                     p[e] = pack_h2(x0, x1);
+                    const float2 high = __half22float2(*reinterpret_cast<const __half2*>(&p[e]));
+                    low[e] = pack_h2(x0 - high.x, x1 - high.y);
                 }
-                tmem_st16(buf + c * 16, p);
-                wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(c == 0 ? &bars->p_half[j & 1] : &bars->p_full[j & 1]);
+                tmem_st8(buf + c * 8, p);
+                tmem_st8(buf + KT / 2 + c * 8, low);
+                if (c % 2 == 1) {                                             // 32 keys at a time
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(c == 1 ? &bars->p_half[j & 1] : &bars->p_full[j & 1]);
+                }
             }
             float a0, a1, b0, b1;
             unf2(sum[0], a0, a1);

@@ -348,8 +348,8 @@ int alloyb_attn_static_status(int32_t* status_out, void* stream);
  * output is zeros, its cache is left alone.  So is one whose rows do not fit (pos + n_tokens > S_max), which also sets bit 0 of
  * alloyb_span_status.  new_k / new_v (both or neither): the tokens' rows, fp16 (B, KV_H, n_tokens, D) with strides in elements
  * (multiples of 8, 16-byte aligned); they are stored at rows pos + i.  NULL: the cache holds them already.
- * scale <= 0 selects 1/sqrt(D).  Scores, softmax and sums are fp32, the probabilities enter P V as fp16; bf16 queries keep all
- * their bits.  What rows hold that no token of a sequence sees does not matter (a NaN or an infinity in a row that one token of a
+ * scale <= 0 selects 1/sqrt(D).  Scores, softmax and sums are fp32, the probabilities enter P V as two fp16 halves (22 bits),
+ * so an infinity in a V row that a token sees may come out as a NaN; bf16 queries keep all their bits.  What rows hold that no token of a sequence sees does not matter (a NaN or an infinity in a row that one token of a
  * chunk sees may reach the chunk's other tokens).  At most 1024 sequences, B * KV_H <= 65535.
  * workspace: alloyb_attn_span_workspace_bytes(the same sizes) bytes, 256-byte aligned, undefined before and
  * after: it needs no clearing and must not be shared by calls that may overlap.  window 0 = none; prefix_len and scored

@@ -11,6 +11,11 @@ from tests.test_gpu_span import DEV, OPS, Case
 pytestmark = pytest.mark.gpu
 
 
+def work(c, keys):
+    """Operations of a call's products, by its sizes."""
+    return 4 * c.d * c.h * c.n * c.b * keys
+
+
 class Cancelling(Case):
     """Scores are single products, exact in fp32 but for the scale's rounding.  Keys come in pairs of nearly equal scores and opposite values, so that
     the outputs are small beside what is added up and show each probability's own rounding."""
@@ -101,3 +106,31 @@ def test_scored_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, dtype):
     ref, _, mag, _ = R.attention(c.q64, k64, v64, pos, scale=1.0)
     check_fine(out, ref, mag, dtype)
 
+
+# from 5e9 operations of more than 16 rows a KV head on: the 5th-generation tensor cores, with head_dim 64 and 128
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,window,sinks,dtype", [
+    (1, 8, 1, 128, 700, 6000, [5100], 4000, 129, torch.float16),
+    (4, 24, 2, 64, 500, 5000, [4000, -1, 0, 777], 3500, 5, torch.bfloat16),
+    (1, 64, 8, 128, 30, 20000, [19000], 16000, 64, torch.float16),                 # few tiles: the keys are split
+])
+def test_long_window_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, window, sinks, dtype):
+    c = Cancelling(b, h, kv_h, d, n, s, pos, dtype, spread=8.0)
+    assert work(c, min(s, window + sinks + n)) >= 5e9
+    k, v, k64, v64 = c.caches(True)
+    out = OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), k, v, window, sinks, 1.0)
+    ref, mag = R.attention_wide(c.q64.to(DEV) * d ** 0.5, k64.to(DEV), v64.to(DEV), pos, window=window, sinks=sinks)
+    check_fine(out, ref.cpu(), mag.cpu(), dtype)
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,p,dtype", [
+    (70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], 14001, torch.float16),
+    (33, 32, 2, 64, 2, 24, [i % 23 - 1 for i in range(33)], 8100, torch.bfloat16),
+    (2, 32, 1, 128, 100, 900, [800, -1], 5000, torch.float16),
+])
+def test_long_prefix_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, p, dtype):
+    c = Cancelling(b, h, kv_h, d, n, s, pos, dtype, prefix=p, spread=8.0)
+    assert work(c, p) >= 1.5e9
+    k, v, k64, v64 = c.caches(True)
+    out = OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), c.pk.to(DEV), c.pv.to(DEV), k, v, 1.0)
+    ref, mag = R.attention_wide(c.q64.to(DEV) * d ** 0.5, k64.to(DEV), v64.to(DEV), pos, prefix=(c.pk.double().to(DEV), c.pv.double().to(DEV)))
+    check_fine(out, ref.cpu(), mag.cpu(), dtype)
