@@ -52,13 +52,13 @@ struct Params {
 // Launches that begin beside the launch ahead of them, whose results they do not need.  That launch tells, behind its own wait, that what ran
 // before is complete (one CTA of it, ahead of letting others begin); where nothing is told yet, as when another thread's launch came in between on the stream,
 // the launch waits first, as all others do.  Either way it waits at its end: its end is the end of what lies before it.
-__device__ __forceinline__ void tell_begun(const Params& P) {
-    *static_cast<volatile unsigned long long*>(P.begun) = P.call;
-    __threadfence();
+__device__ __forceinline__ void tell_begun(const Params& P) {                 // (a release: what the wait made visible to this thread goes ahead of the word)
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(P.begun), "l"(P.call) : "memory");
 }
 __device__ __forceinline__ void wait_unless_begun(const Params& P) {
-    if (*static_cast<volatile unsigned long long*>(P.begun) != P.call) pdl_wait();
-    __threadfence();
+    unsigned long long told;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(told) : "l"(P.begun) : "memory");
+    if (told != P.call) pdl_wait();
 }
 __device__ __forceinline__ void end_behind(const Params& P, bool last) {
     pdl_wait();

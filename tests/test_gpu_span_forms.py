@@ -134,3 +134,76 @@ def test_long_prefix_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, p, dtype)
     out = OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), c.pk.to(DEV), c.pv.to(DEV), k, v, 1.0)
     ref, mag = R.attention_wide(c.q64.to(DEV) * d ** 0.5, k64.to(DEV), v64.to(DEV), pos, prefix=(c.pk.double().to(DEV), c.pv.double().to(DEV)))
     check_fine(out, ref.cpu(), mag.cpu(), dtype)
+
+
+def replayed(*ways):
+    """Each way: a change of the inputs and a call.  Captured once, replayed with other data each time, against the same call made directly; two graphs take turns."""
+    graphs = []
+    for change, call in ways:
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for turn in range(4):
+        for change, _ in ways:
+            change(turn)
+        for graph, _ in graphs + graphs[:1]:                          # (the first once more: a replay right behind another's launches)
+            graph.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in out] for _, out in graphs]
+        for (_, call), mine in zip(ways, got):
+            torch.cuda.synchronize()
+            for x, y in zip(mine, call()):
+                bits = torch.int16 if x.element_size() == 2 else torch.int32
+                assert torch.equal(x.view(bits), y.view(bits)), turn
+    assert _lib.load().alloyb_device_error(1) == 0 and ops.span_status() == 0
+
+
+def moving(c, seed):
+    """A change of q, of the new rows and of the positions in place."""
+    at = c.pos_t()
+
+    def change(turn):
+        g = torch.Generator().manual_seed(seed * 100 + turn)
+        c.q.copy_(torch.randn(c.q.shape, generator=g))
+        c.nk.copy_(torch.randn(c.nk.shape, generator=g))
+        c.nv.copy_(torch.randn(c.nv.shape, generator=g))
+        new = torch.randint(-1, c.s - c.n + 1, (c.b,), generator=g)
+        at.copy_(new.int() if turn else torch.tensor(c.pos, dtype=torch.int32).expand(c.b))
+    return at, change
+
+
+def scored_way(c, seed):
+    at, change = moving(c, seed)
+    k, v = c.k.to(DEV), c.v.to(DEV)
+    w0 = torch.rand(c.b, c.kv_h, c.s, generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+    def call():
+        w = w0.clone()
+        return OPS.attention_cache_scored(c.q, c.nk, c.nv, at, k, v, w), w, k, v
+    return change, call
+
+
+def test_replays_of_launches_that_begin_beside_one_another():
+    """Large prefixes with few own keys, and scored calls: launches that skip their wait when the one ahead has told that it may, in graphs."""
+    c = Case(70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], prefix=14001)
+    assert work(c, 14001) >= 1.5e9
+    pk, pv, k, v = (t.to(DEV) for t in (c.pk, c.pv, c.k, c.v))
+    at, change = moving(c, 1)
+    behind = change, lambda: (OPS.attention_shared_prefix(c.q, c.nk, c.nv, at, pk, pv, k, v), k, v)
+    replayed(behind, scored_way(Case(40, 16, 8, 128, 1, 300, [(i * 37) % 300 for i in range(40)]), 2))
+    replayed(scored_way(Case(2, 32, 8, 64, 12, 900, [700, 880]), 3), scored_way(Case(1, 16, 2, 128, 5, 9000, [8000]), 4))
+
+
+def test_replays_of_large_chunks():
+    """Tensor maps are made when a call is captured; what they lead to changes from replay to replay."""
+    ways = []
+    for seed, (b, h, kv_h, d, n, s, pos) in enumerate([(1, 8, 1, 128, 700, 6000, [5100]), (4, 24, 2, 64, 500, 5000, [4000, -1, 0, 777])]):
+        c = Case(b, h, kv_h, d, n, s, pos)
+        assert work(c, min(s, 4000 + 129 + n)) >= 5e9
+        at, change = moving(c, seed + 9)
+        k, v = c.k.to(DEV), c.v.to(DEV)
+        ways.append((change, lambda c=c, at=at, k=k, v=v: (OPS.attention_cache_window(c.q, c.nk, c.nv, at, k, v, 4000, 129), k, v)))
+    replayed(*ways)
