@@ -369,20 +369,28 @@ extern "C" int alloyb_kv_evict(const void* k, const void* v, const float* weight
     if (items > 65535) return ALLOYB_E_LIMIT;
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
         return ALLOYB_E_ALIGN;
-    // every output either is its input or lies apart from all three
-    const uintptr_t in[3] = {reinterpret_cast<uintptr_t>(k), reinterpret_cast<uintptr_t>(v), reinterpret_cast<uintptr_t>(weights)};
-    const uintptr_t out[3] = {reinterpret_cast<uintptr_t>(k_out), reinterpret_cast<uintptr_t>(v_out), reinterpret_cast<uintptr_t>(weights_out)};
-    const int64_t row[3] = {D * 2, D * 2, 4};
+    // k_out, v_out and weights_out each are their input or lie apart from every input; no output overlaps another, and kept and new_lengths none of the
+    // inputs (the CTAs of a sequence read its length while one of them writes the new one)
+    struct Span {
+        const void* at;
+        int64_t bytes;
+    };
+    const int64_t row = D * 2, rows_in = items * S, rows_out = items * S_out;
+    const Span in[4] = {{k, rows_in * row}, {v, rows_in * row}, {weights, rows_in * 4}, {lengths, static_cast<int64_t>(lengths_count) * 4}};
+    const Span out[5] = {{k_out, rows_out * row}, {v_out, rows_out * row}, {weights_out, rows_out * 4}, {kept, items * keep * 4}, {new_lengths, static_cast<int64_t>(B) * 4}};
+    auto meet = [](const Span& x, const Span& y) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x.at), b = reinterpret_cast<uintptr_t>(y.at);
+        return a < b + y.bytes && b < a + x.bytes;
+    };
     bool in_place = false;
-    for (int o = 0; o < 3; ++o)
-        for (int i = 0; i < 3; ++i) {
-            if (o == i && out[o] == in[i] && S_out == S) {
-                in_place = true;
-                continue;
-            }
-            const uintptr_t out_end = out[o] + items * S_out * row[o], in_end = in[i] + items * S * row[i];
-            if (out[o] < in_end && in[i] < out_end) return ALLOYB_E_SHAPE;
+    for (int o = 0; o < 5; ++o) {
+        for (int i = 0; i < 4; ++i) {
+            if (o == i && o < 3 && out[o].at == in[i].at && S_out == S) in_place = true;
+            else if (meet(out[o], in[i])) return ALLOYB_E_SHAPE;
         }
+        for (int i = 0; i < o; ++i)
+            if (meet(out[o], out[i])) return ALLOYB_E_SHAPE;
+    }
     ev::Params P;
     P.k = static_cast<const __half*>(k); P.v = static_cast<const __half*>(v); P.w = weights;
     P.len = lengths; P.len_count = lengths_count;

@@ -383,9 +383,9 @@ int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t q_head_str
 /* Of each (sequence, KV head)'s rows [0, lengths[b]) keeps min(lengths[b], keep): the first `sinks`, the last `recent`, and of
  * those between the ones of the largest weight (ties: the lowest row; NaN below everything; sinks + recent <= keep).  They go, in
  * their order, to rows [0, min(lengths[b], keep)) of k_out / v_out / weights_out -- (B, KV_H, S_out, D) and
- * (B, KV_H, S_out) dense, keep <= S_out; rows behind them are left alone.  Each output may be its input itself (S_out == S); otherwise
- * it must not overlap an input.  kept: int32 (B, KV_H, keep), the rows they came from, -1 behind the last; new_lengths: int32
- * (B,).  lengths: int32 device (lengths_count,), 1 = shared.  A length outside [0, S] counts as 0 and sets bit 1 of
+ * (B, KV_H, S_out) dense, keep <= S_out; rows behind them are left alone.  Each of the three may be its input itself (S_out == S);
+ * otherwise no output may overlap an input or another output (ALLOYB_E_SHAPE), new_lengths not `lengths` either.
+ * kept: int32 (B, KV_H, keep), the rows they came from, -1 behind the last; new_lengths: int32 (B,).  lengths: int32 device (lengths_count,), 1 = shared.  A length outside [0, S] counts as 0 and sets bit 1 of
  * alloyb_span_status. */
 int alloyb_kv_evict(const void* k, const void* v, const float* weights, const int32_t* lengths, int lengths_count,
                     void* k_out, void* v_out, float* weights_out, int32_t* kept, int32_t* new_lengths, int B, int KV_H,

@@ -109,3 +109,20 @@ def test_the_definitions_themselves():
         assert torch.allclose(a[0], b[0]) and torch.allclose(a[2], b[1]) and torch.allclose(a[1], grown)
     assert R.evict([5, 1, 3, 3, 2, 9, 0, 0], 8, 5, 1, 1) == [0, 2, 3, 5, 7]
     assert R.evict([1.0, float("nan"), 0.0, 1.0], 4, 3, 0, 0) == [0, 2, 3]
+
+
+@pytest.mark.parametrize("change", [
+    dict(new=3), dict(new=3, new_off=4), dict(new=0), dict(new=2), dict(new=4), dict(new=7), dict(kept=3), dict(kept=1), dict(kept=6), dict(kept=6, kept_off=96),
+    dict(ko=5, ko_off=512), dict(vo=4, vo_off=16), dict(wo=4), dict(wo=5, wo_off=1024),
+])
+def test_evict_outputs_lie_apart(change):
+    """The sequence's CTAs read its length while one of them writes the new one, and copies know no order among outputs."""
+    mb = 1 << 20
+    # places 0 .. 8, megabytes apart: k, v, weights, lengths, k_out, v_out, weights_out, kept, new_lengths
+
+    def evict(ko=4, vo=5, wo=6, kept=7, new=8, ko_off=0, vo_off=0, wo_off=0, kept_off=0, new_off=0, b=2):
+        at = lambda i, off=0: (i + 1) * mb + off  # noqa: E731
+        return _lib.load().alloyb_kv_evict(at(0), at(1), at(2), at(3), 2, at(ko, ko_off), at(vo, vo_off), at(wo, wo_off), at(kept, kept_off), at(new, new_off), b, 2,
+                                           64, 100, 50, 50, 0, 0, None)
+    assert evict(b=3) == E_SHAPE                                               # (two lengths for three sequences: the call is refused before a launch)
+    assert evict(**change) == E_SHAPE
