@@ -420,7 +420,7 @@ __device__ __forceinline__ void span_stream(const Params& P, int cta, int ctas) 
                 if (c0 + d == 0) P.part_lse[slot * 16 + r] = l == 0.f ? -INFINITY : top + log2f(l) - P_BIAS_LOG2;
                 if (all && !PREFIX) {
                     const int tok = r / P.G, hg = r - tok * P.G;
-                    store4(P.out, P.q_dtype, ((static_cast<int64_t>(at.b) * P.n + tok) * P.H + at.kvh * P.G + hg) * D + c0 + d, acc.x, acc.y, acc.z, acc.w);
+                    store4(P.out, P.q_dtype, ((static_cast<int64_t>(at.b) * P.n_all + tok) * P.H + at.kvh * P.G + hg) * D + c0 + d, acc.x, acc.y, acc.z, acc.w);
                 } else {
                     *reinterpret_cast<float4*>(P.part_o + (slot * 16 + r) * D + c0 + d) = acc;
                 }
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(WARPS * 32) span_cluster_kernel(const Params P
         }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         const int tok = r / P.G, hg = r - tok * P.G;
-        store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        store4(P.out, P.q_dtype, ((static_cast<int64_t>(b) * P.n_all + tok) * P.H + kvh * P.G + hg) * D + d, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
     if (SCORED) {
         if (threadIdx.x < rows) {
@@ -675,7 +675,7 @@ __device__ __forceinline__ void span_rows(const Params& P, int tile, int tiles, 
         if (t == 0 && (!direct || SCORED)) pl[slot * 64 + r] = st.l[rr] == 0.f ? -INFINITY : st.m[rr] + log2f(st.l[rr]) - P_BIAS_LOG2;
         if (direct) {
             const int tok = r_own[rr] / P.G, hg = r_own[rr] - tok * P.G;
-            const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+            const int64_t at = ((static_cast<int64_t>(b) * P.n_all + tok) * P.H + kvh * P.G + hg) * D;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) {
                 const float x = st.o[i][2 * rr] * inv, y = st.o[i][2 * rr + 1] * inv;
@@ -815,7 +815,7 @@ __device__ __forceinline__ void join_rows(const Params& P) {
         }
     }
     const int tok = R / P.G, hg = R - tok * P.G;
-    const int64_t out = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+    const int64_t out = ((static_cast<int64_t>(b) * P.n_all + tok) * P.H + kvh * P.G + hg) * D;
     if (team == 1) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
@@ -1084,6 +1084,17 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
     return p;
 }
 
+// The scored form keeps its scores, 4 bytes a query row and cache row, until their rows' sums are known.  Calls with more than this much of them
+// run as several, of as many tokens as fit each: the weights of a token's own row are set by its part and added to by those behind it, as in calls
+// one after another.  A token at a time there is nothing left to divide: B * H * S * 4 bytes, G / D of what the cache has.
+constexpr int64_t SCORES_MOST = int64_t(1) << 30;
+static int scored_tokens(int B, int H, int n, int S) {
+    const int64_t token = static_cast<int64_t>(B) * H * ((static_cast<int64_t>(S) + 3) / 4 * 4) * 4;
+    if (n <= 1 || token * n <= SCORES_MOST) return n;
+    const int64_t fit = token < SCORES_MOST ? SCORES_MOST / token : 1, parts = (n + fit - 1) / fit;
+    return static_cast<int>((n + parts - 1) / parts);
+}
+
 // A kernel with more dynamic shared memory than the default, once per device.
 template <typename K>
 static int allow_smem(K kern, int bytes, bool (&done)[64]) {
@@ -1233,7 +1244,7 @@ static int fill(Params& P, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_
     P.nk = static_cast<const __half*>(nk); P.nv = static_cast<const __half*>(nv);
     P.n_bs = n_bs; P.n_hs = n_hs; P.n_ts = n_ts;
     P.pos = pos; P.pos_count = pos_count; P.out = out;
-    P.B = B; P.H = H; P.KV_H = KV_H; P.G = H / KV_H; P.n = n;
+    P.B = B; P.H = H; P.KV_H = KV_H; P.G = H / KV_H; P.n = P.n_all = n;
     P.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * 1.4426950408889634f;
     return ALLOYB_OK;
 }
@@ -1275,7 +1286,11 @@ using namespace alloyb;
 extern "C" size_t alloyb_attn_span_workspace_bytes(int B, int H, int KV_H, int D, int n_tokens, int S_max, int window, int sinks, int prefix_len,
                                                    int scored) {
     if (sp::sizes_ok(B, H, KV_H, D, n_tokens, S_max) != ALLOYB_OK || window < 0 || sinks < 0 || prefix_len < 0) return 0;
-    return sp::plan_of(B, H, KV_H, D, n_tokens, S_max, window, sinks, prefix_len, scored != 0).bytes;
+    if (!scored) return sp::plan_of(B, H, KV_H, D, n_tokens, S_max, window, sinks, prefix_len, false).bytes;
+    const int part = sp::scored_tokens(B, H, n_tokens, S_max), rest = part > 0 ? n_tokens % part : 0;
+    const size_t most = sp::plan_of(B, H, KV_H, D, part, S_max, window, sinks, prefix_len, true).bytes;
+    const size_t last = sp::plan_of(B, H, KV_H, D, rest, S_max, window, sinks, prefix_len, true).bytes;
+    return most > last ? most : last;
 }
 
 extern "C" int alloyb_attn_window(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype, void* k, void* v,
@@ -1331,10 +1346,28 @@ extern "C" int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t
     if (!weights) return ALLOYB_E_NULL;
     if (reinterpret_cast<uintptr_t>(weights) % 4) return ALLOYB_E_ALIGN;
     P.weights = weights;
-    const sp::Plan plan = sp::plan_of(B, H, KV_H, D, n_tokens, S_max, 0, 0, 0, true);
-    rc = sp::place(P, plan, workspace, workspace_bytes);
-    if (rc != ALLOYB_OK || n_tokens == 0) return rc;
-    return sp::run<true, false>(plan, P, D, as_stream(stream));
+    const int part = sp::scored_tokens(B, H, n_tokens, S_max);
+    sp::Plan whole = {};                                                     // (checked ahead of the first part's launches)
+    whole.bytes = alloyb_attn_span_workspace_bytes(B, H, KV_H, D, n_tokens, S_max, 0, 0, 0, 1);
+    sp::Params probe = P;
+    rc = sp::place(probe, whole, workspace, workspace_bytes);
+    if (rc != ALLOYB_OK) return rc;
+    for (int tok0 = 0; tok0 < n_tokens; tok0 += part) {
+        sp::Params p = P;
+        p.tok0 = tok0;
+        p.n = n_tokens - tok0 < part ? n_tokens - tok0 : part;
+        p.q = static_cast<const char*>(q) + tok0 * P.q_ts * 2;
+        p.out = static_cast<char*>(out) + static_cast<int64_t>(tok0) * H * D * 2;
+        if (new_k) {
+            p.nk += tok0 * P.n_ts;
+            p.nv += tok0 * P.n_ts;
+        }
+        const sp::Plan plan = sp::plan_of(B, H, KV_H, D, p.n, S_max, 0, 0, 0, true);
+        rc = sp::place(p, plan, workspace, workspace_bytes);
+        if (rc == ALLOYB_OK) rc = sp::run<true, false>(plan, p, D, as_stream(stream));
+        if (rc != ALLOYB_OK) return rc;
+    }
+    return ALLOYB_OK;
 }
 
 extern "C" int alloyb_span_status(int32_t* status_out, int clear) {

@@ -27,8 +27,9 @@ struct Params {
     int64_t n_bs, n_hs, n_ts;
     const int32_t* pos;
     int pos_count;
-    void* out;                           // (B, n, H, D)
+    void* out;                           // (B, n_all, H, D)
     int B, H, KV_H, G, n;
+    int n_all, tok0;                     // the call's tokens, of which these launches have n from tok0 on (q, nk and out begin at tok0)
     int window, sinks;                   // window 0: every position up to the row's own
     float scale_log2;
     const __half *pk, *pv;               // shared prefix (KV_H, P, D)
@@ -65,7 +66,7 @@ __device__ __forceinline__ void end_behind(const Params& P, bool last) {
     if (last) *static_cast<volatile unsigned long long*>(P.begun) = 0;       // a graph's next replay begins anew
 }
 
-// One sequence of a call: the keys its tokens tok0 .. tok1 - 1 see, as one run of `keys` places: `sink` first rows, then rows from lo on.
+// One sequence of a call (pos: the row of the launch's first token): the keys its tokens tok0 .. tok1 - 1 see, as one run of `keys` places: `sink` first rows, then rows from lo on.
 struct Seq {
     int pos, lo, sink, keys;
     __device__ __forceinline__ int row_of(int place) const { return place < sink ? place : lo + place - sink; }
@@ -73,11 +74,11 @@ struct Seq {
 __device__ __forceinline__ int live_pos(const Params& P, int b, bool tell) {
     const int pos = __ldcg(P.pos + (P.pos_count == 1 ? 0 : b));
     if (pos < 0) return -1;                                  // a sequence without tokens in this call
-    if (pos > P.S - P.n) {
+    if (pos > P.S - P.n_all) {
         if (tell) atomicOr(&g_span_status, SPAN_POS_RANGE);
         return -1;
     }
-    return pos;
+    return pos + P.tok0;
 }
 __device__ __forceinline__ Seq seq_at(const Params& P, int pos, int tok0, int tok1) {
     Seq s = {pos, 0, 0, 0};

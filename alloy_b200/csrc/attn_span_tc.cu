@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 2) span_tc_kernel(const __grid_consta
         if (row_live && !direct)
             (PREFIX ? P.pre_lse : P.part_lse)[slot * ROWS + r] = l_run == 0.f ? -INFINITY : m_run + log2f(l_run) - sp::P_BIAS_LOG2;
         float* po = (PREFIX ? P.pre_o : P.part_o) + (slot * ROWS + r) * D;
-        const int64_t at = ((static_cast<int64_t>(b) * P.n + tok) * P.H + kvh * P.G + hg) * D;
+        const int64_t at = ((static_cast<int64_t>(b) * P.n_all + tok) * P.H + kvh * P.G + hg) * D;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
             float o[32];

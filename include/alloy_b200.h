@@ -374,7 +374,8 @@ int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, int64_t q_h
 /* Causal attention over the cache that keeps its weights: weights[b, kvh, j] (fp32, (B, KV_H, S_max) dense) grows by the sum over the
  * KV head's query heads and the call's tokens of the probability that each gives row j.  The entries of the tokens' own rows are
  * set instead: what stood there belonged to a row that is gone.  Entries behind them are left alone.  The sums are taken in a fixed
- * order. */
+ * order.  The workspace holds scores, 4 bytes a query row and row of the cache's S_max: calls whose scores would take more than 1 GiB run as several of
+ * fewer tokens (at least one, B * H * S_max * 4 bytes), so it grows with n_tokens up to that only. */
 int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype,
                        void* k, void* v, const void* new_k, const void* new_v, int64_t new_batch_stride,
                        int64_t new_head_stride, int64_t new_tok_stride, const int32_t* pos, int pos_count, float* weights,

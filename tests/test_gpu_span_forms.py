@@ -207,3 +207,32 @@ def test_replays_of_large_chunks():
         k, v = c.k.to(DEV), c.v.to(DEV)
         ways.append((change, lambda c=c, at=at, k=k, v=v: (OPS.attention_cache_window(c.q, c.nk, c.nv, at, k, v, 4000, 129), k, v)))
     replayed(*ways)
+
+
+# calls whose scores take more than 1 GiB, which run in parts
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,dtype,write", [
+    (2, 64, 4, 128, 301, 8192, [7000, 0], torch.float16, True),                    # 4 MiB a token: parts of 151 and 150
+    (2, 128, 1, 64, 5, 262143, [262138, 100], torch.bfloat16, False),              # 256 MiB a token: parts of 3 and 2
+    (5, 64, 1, 64, 7, 200000, [199993, -1, 199994, 3, 70000], torch.float16, True),    # an idle sequence, one whose last token does not fit
+])
+def test_scored_in_parts(b, h, kv_h, d, n, s, pos, dtype, write):
+    parts = -(-b * h * n * s * 4 // (1 << 30))
+    assert parts > 1 and _lib.load().alloyb_attn_span_workspace_bytes(b, h, kv_h, d, n, s, 0, 0, 0, 1) < 3 << 29
+    c = Case(b, h, kv_h, d, n, s, pos, dtype)
+    k, v, k64, v64 = c.caches(write)
+    k0 = k.clone()
+    w = torch.rand(b, kv_h, s, generator=torch.Generator().manual_seed(1)).to(DEV)
+    before, add = w.double(), torch.zeros(b, kv_h, s, dtype=torch.float64, device=DEV)
+    for i in range(b):
+        if c.place(i) is not None:
+            w[i, :, c.place(i):c.place(i) + n] = float("nan")
+            before[i, :, c.place(i):c.place(i) + n] = 0.0
+    out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w, -1.0, write)
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, weights=add)
+    got = out.double()
+    assert ((got - ref).abs() <= R.out_bound(ref, mag, dtype)).all()
+    big = float((c.q64.abs().amax() * c.k.abs().amax()) * d ** 0.5)
+    # a rounding of the sum a part on top of the probabilities' errors
+    assert ((w.double() - before - add).abs() <= R.weight_bound(add, big, d) + (before + add) * parts * 2.0 ** -23).all()
+    c.check_written(k0, k, c.nk64, write)
+    assert ops.span_status() == (1 if any(p + n > s for p in pos) else 0)

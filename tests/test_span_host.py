@@ -126,3 +126,18 @@ def test_evict_outputs_lie_apart(change):
                                            64, 100, 50, 50, 0, 0, None)
     assert evict(b=3) == E_SHAPE                                               # (two lengths for three sequences: the call is refused before a launch)
     assert evict(**change) == E_SHAPE
+
+
+def test_scored_workspace_is_bounded():
+    """A prompt-sized scored call asks for no more than its parts of 1 GiB of scores (and what is joined), one token for what one token needs."""
+    size = _lib.load().alloyb_attn_span_workspace_bytes
+    gib = 1 << 30
+    for n in (64, 2048, 4096, 32768):
+        assert size(1, 32, 8, 128, n, 131072, 0, 0, 0, 1) < 1.5 * gib
+    assert size(1, 32, 8, 128, 32, 1 << 18, 0, 0, 0, 1) >= gib                 # 32 MiB a token: a call of 32 is one part
+    token = size(16, 64, 8, 64, 1, 1 << 20, 0, 0, 0, 1)
+    assert token >= 4 * gib and size(16, 64, 8, 64, 5, 1 << 20, 0, 0, 0, 1) < token + gib // 4
+    for n in (1, 33, 4096):
+        need = size(1, 32, 8, 128, n, 131072, 0, 0, 0, 1)
+        assert _lib.load().alloyb_attn_scored(OK, 64, 64, 64, _lib.F16, OK, OK, None, None, 0, 0, 0, OK, 1, OK, OK, 1, 32, 8, 128, n, 131072, -1.0, OK,
+                                              need - 1, None) == E_WORKSPACE
