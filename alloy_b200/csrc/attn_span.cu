@@ -898,7 +898,7 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
             for (int i = 0; i < p.own; ++i) {
                 const float x = __ldcg(P.part_lse + p.own_index(i)), top = fmaxf(m, x);
                 if (x == -INFINITY) continue;                            // (an empty part)
-                l = (m == -INFINITY ? 0.f : l * ex2(m - top)) + ex2(x - top);
+                l = l * (m == -INFINITY ? 0.f : ex2(m - top)) + ex2(x - top);    // (a NaN stays one)
                 m = top;
             }
             lse[threadIdx.x] = l == 0.f ? -INFINITY : m + log2f(l);

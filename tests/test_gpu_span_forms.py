@@ -236,3 +236,22 @@ def test_scored_in_parts(b, h, kv_h, d, n, s, pos, dtype, write):
     assert ((w.double() - before - add).abs() <= R.weight_bound(add, big, d) + (before + add) * parts * 2.0 ** -23).all()
     c.check_written(k0, k, c.nk64, write)
     assert ops.span_status() == (1 if any(p + n > s for p in pos) else 0)
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos", [
+    (2, 8, 2, 128, 1, 300, [290, 100]),                                            # clusters
+    (40, 16, 8, 128, 1, 300, [299 - i for i in range(40)]),                        # streamed
+    (1, 8, 1, 128, 1, 33000, [32000]),
+    (1, 16, 2, 128, 5, 9000, [8000]),                                              # row tiles, several parts
+    (2, 8, 2, 64, 40, 300, [200, 7]),
+])
+@pytest.mark.parametrize("at", [0, 5])
+def test_scored_of_rows_that_are_not_numbers(b, h, kv_h, d, n, s, pos, at):
+    """A NaN in a key makes every weight of the rows that see it a NaN, wherever among the keys it lies; sequence 0's first KV head has one."""
+    c = Case(b, h, kv_h, d, n, s, pos)
+    c.k[0, 0, at, 3] = float("nan")
+    k, v, _, _ = c.caches(True)
+    w = torch.zeros(b, kv_h, s, device=DEV)
+    out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w)
+    assert out[0, :h // kv_h].isnan().all() and w[0, 0, :pos[0] + n].isnan().all() and not w[0, 0, pos[0] + n:].any()
+    assert not out[0, h // kv_h:].isnan().any() and not w[0, 1:].isnan().any() and not w[1:].isnan().any() and not out[1:].isnan().any()
