@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(WARPS * 32) span_cluster_kernel(const Params P
                 const float m = peer_f32(cta_m + threadIdx.x, k), lk = peer_f32(cta_l + threadIdx.x, k);
                 l += m == -INFINITY && lk == 0.f ? 0.f : lk * ex2(m - top);
             }
-            lse[threadIdx.x] = top + log2f(l) - P_BIAS_LOG2;
+            lse[threadIdx.x] = l == 0.f ? INFINITY : top + log2f(l) - P_BIAS_LOG2;      // (a row whose scores are all -inf adds nothing)
         }
         __syncthreads();
         float* w = P.weights + static_cast<int64_t>(item) * P.S;
@@ -901,7 +901,7 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
                 l = l * (m == -INFINITY ? 0.f : ex2(m - top)) + ex2(x - top);    // (a NaN stays one)
                 m = top;
             }
-            lse[threadIdx.x] = l == 0.f ? -INFINITY : m + log2f(l);
+            lse[threadIdx.x] = l == 0.f ? INFINITY : m + log2f(l);       // (a row whose scores are all -inf adds nothing)
         }
         __syncthreads();
     };

@@ -255,3 +255,26 @@ def test_scored_of_rows_that_are_not_numbers(b, h, kv_h, d, n, s, pos, at):
     out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w)
     assert out[0, :h // kv_h].isnan().all() and w[0, 0, :pos[0] + n].isnan().all() and not w[0, 0, pos[0] + n:].any()
     assert not out[0, h // kv_h:].isnan().any() and not w[0, 1:].isnan().any() and not w[1:].isnan().any() and not out[1:].isnan().any()
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,pos", [
+    (2, 8, 2, 128, 1, 300, [290, 0]),
+    (40, 16, 8, 128, 1, 300, [299 - i for i in range(40)]),
+    (1, 8, 1, 128, 1, 33000, [32000]),
+    (1, 16, 2, 128, 5, 9000, [8000]),
+    (2, 8, 2, 64, 40, 300, [200, 7]),
+])
+def test_scored_of_rows_that_see_nothing(b, h, kv_h, d, n, s, pos):
+    """Every score of sequence 0's first KV head is -inf: nothing is attended to, the outputs are zeros and the weights do not grow."""
+    c = Case(b, h, kv_h, d, n, s, pos)
+    c.k[0, 0, :, 0] = float("-inf")
+    c.nk64[0, 0, :, 0] = float("-inf")
+    c.nk[0, 0, :, 0] = float("-inf")
+    c.q[0, :h // kv_h, :, 0] = 1.0
+    k, v, _, _ = c.caches(True)
+    w = torch.rand(b, kv_h, s, generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = w[0, 0].clone()
+    want[pos[0]:pos[0] + n] = 0.0
+    out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w)
+    assert not out[0, :h // kv_h].any() and torch.equal(w[0, 0], want)
+    assert not w.isnan().any() and not out.isnan().any() and (kv_h == 1 or out[0, h // kv_h:].any())
