@@ -956,14 +956,18 @@ __global__ void __launch_bounds__(256) span_weights_kernel(const Params P) {
 // ---------------------------------------------------------------------------------------------------------------- host
 constexpr int SMS = 148;
 
-// Operations (4 D rows keys, by the sizes of the call) from which more than 16 rows of a KV head go to the 5th-generation tensor cores, own keys / a prefix.
-// There / on mma.sync, cold caches, 32/8 heads, window 4096: 16 tokens of 4 sequences, head_dim 128 (4.3e9) 41.0 / 38.9 us; 32 tokens of 4, head_dim 64
-// (4.3e9) 34.8 / 39.1; 8 tokens of 16 (8.6e9) 76.5 / 84.0; 5 tokens of 32 (1.1e10) 117 / 141; 80 tokens behind 6000 (1.1e10) 34.7 / 44.8.  A prefix of
-// 4096: 16 sequences (1.1e9) 38.9 / 36.9, 32 (2.1e9) 49.1 / 53.0; of 32768: 8 sequences, 32 rows (4.3e9) 59.4 / 63.5; 64 sequences over 4096 beside 1000 own
-// keys (4.3e9) 77 / 70, since there the own keys go in the same launch on mma.sync, 128 (8.6e9) 121 / 140.  Not the scored form: threads that have a row
-// each store its scores piecemeal (16 tokens of 4 sequences 82 / 67).
+// More than 16 rows of a KV head go to the 5th-generation tensor cores from this many operations (4 D rows keys, by the sizes of the call) on.  mma.sync /
+// there, cold caches, 32/8 heads, window 4096: head_dim 128, 5 tokens of 32 sequences (1.1e10) 186 / 120 us, 8 of 8 (4.3e9) 64 / 53, 16 of 4 (4.3e9) 43.0 / 41.0, 40
+// of 1 (2.7e9) 36.8 / 34.8, 32 of 1 (2.2e9) 34.8 / 34.8; 64, 32 of 4 (4.3e9) 43.2 / 34.8, 8 of 16 under a window of 2048 (2.2e9) 45 / 41, 16 of 4 (2.2e9) 30.7 /
+// 32.8.  Not the scored form: threads that have a row each store its scores piecemeal.
+// A prefix whose sequences have such chunks goes there by the same rule (16 tokens of 4 over 8192 rows: 72 / 53).  With few rows each, the prefix there has a launch
+// of its own ahead of the own keys, where mma.sync has both in one, so it takes more, counted in pairs of a row and a key, from 32 rows in all on.
+// mma.sync / there, 32/8 heads, head_dim 128: 16 sequences over 16384 (8.4e6 pairs) 43 / 49 us, over 32768 (1.7e7) 59 / 64, over 65536 (3.4e7) 94 / 86; 8 over 65536 (1.7e7)
+// 88 / 82; 32 over 8192 (8.4e6) beside up to 2000 own keys 82 / 84, over 16384 (1.7e7) 70 / 60; 64 beside 1000 own keys over 4096 (8.4e6) 81 / 86, over 8192 (1.7e7) 94 / 93;
+// 128 over 4096 (1.7e7) beside 100 own keys 121 / 62, beside 1000 128 / 113; head_dim 64, 32 over 8192 (8.4e6) 41 / 39, 64 over 6000 (1.2e7) beside 1000 55 / 65, 128 over
+// 4096 (1.7e7) beside 1000 86 / 85.
 constexpr int TC_TILE = 128, TC_PREFIX_ROWS = 32;           // rows of a tile; rows from which a prefix may go there
-constexpr double TC_WORK = 5e9, TC_PREFIX_WORK = 1.5e9;
+constexpr double TC_WORK = 2e9, TC_PREFIX_PAIRS = 1.3e7;
 static double work_of(int D, int64_t rows, int64_t items, int64_t keys) { return 4.0 * D * static_cast<double>(rows) * static_cast<double>(items) * static_cast<double>(keys); }
 // One launch of clusters, or the stream kernel and the join: as long as a CTA has 16 steps at most and all CTAs run at once.  Captured in a graph,
 // 32/8 heads, clusters / stream: head_dim 128, one sequence of 4000 keys 10.3 / 11.3 us, 4 of 2000 10.1 / 14.2, 16 of 1000 13.9 / 18.7, 32 of 1000
@@ -1043,7 +1047,8 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
         o_rows = P > 0 || p.splits > 1 ? lse_rows : 0;
     }
     if (P > 0) {
-        p.pre_tc = D <= 128 && rows * B >= TC_PREFIX_ROWS && work_of(D, rows, items, P) >= TC_PREFIX_WORK;
+        p.pre_tc = D <= 128 && rows * B >= TC_PREFIX_ROWS &&
+                   (p.stream ? static_cast<double>(rows) * static_cast<double>(items) * P >= TC_PREFIX_PAIRS : work_of(D, rows, items, P) >= TC_WORK);
         const int kt = D == 256 ? 32 : 64, tr = p.pre_tc ? TC_TILE : 64;
         p.pre_tiles = static_cast<int>((rows * B + tr - 1) / tr);
         const int64_t tiles = static_cast<int64_t>(p.pre_tiles) * KV_H, steps = (P + kt - 1) / kt;

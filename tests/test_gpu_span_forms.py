@@ -11,9 +11,12 @@ from tests.test_gpu_span import DEV, OPS, Case
 pytestmark = pytest.mark.gpu
 
 
-def work(c, keys):
-    """Operations of a call's products, by its sizes."""
-    return 4 * c.d * c.h * c.n * c.b * keys
+def tensor_cores(c, keys, prefix=False):
+    """Whether a call's sizes send its own keys, or the prefix's, to the 5th-generation tensor cores."""
+    rows, pairs = c.n * c.h // c.kv_h, c.h * c.n * c.b * keys
+    if prefix and rows <= 16:
+        return c.d <= 128 and rows * c.b >= 32 and pairs >= 1.3e7
+    return c.d <= 128 and (rows > 16 or prefix and rows * c.b >= 32) and 4 * c.d * pairs >= 2e9
 
 
 class Cancelling(Case):
@@ -107,7 +110,8 @@ def test_scored_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, dtype):
     check_fine(out, ref, mag, dtype)
 
 
-# from 5e9 operations of more than 16 rows a KV head on: the 5th-generation tensor cores, with head_dim 64 and 128
+# from 2e9 operations of more than 16 rows a KV head on (a prefix with fewer each: 1.3e7 pairs of a row and a key): the 5th-generation tensor cores, with
+# head_dim 64 and 128
 @pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,window,sinks,dtype", [
     (1, 8, 1, 128, 700, 6000, [5100], 4000, 129, torch.float16),
     (4, 24, 2, 64, 500, 5000, [4000, -1, 0, 777], 3500, 5, torch.bfloat16),
@@ -115,7 +119,7 @@ def test_scored_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, dtype):
 ])
 def test_long_window_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, window, sinks, dtype):
     c = Cancelling(b, h, kv_h, d, n, s, pos, dtype, spread=8.0)
-    assert work(c, min(s, window + sinks + n)) >= 5e9
+    assert tensor_cores(c, min(s, window + sinks + n))
     k, v, k64, v64 = c.caches(True)
     out = OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), k, v, window, sinks, 1.0)
     ref, mag = R.attention_wide(c.q64.to(DEV) * d ** 0.5, k64.to(DEV), v64.to(DEV), pos, window=window, sinks=sinks)
@@ -123,13 +127,13 @@ def test_long_window_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, window, s
 
 
 @pytest.mark.parametrize("b,h,kv_h,d,n,s,pos,p,dtype", [
-    (70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], 14001, torch.float16),
+    (70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], 24001, torch.float16),
     (33, 32, 2, 64, 2, 24, [i % 23 - 1 for i in range(33)], 8100, torch.bfloat16),
     (2, 32, 1, 128, 100, 900, [800, -1], 5000, torch.float16),
 ])
 def test_long_prefix_keeps_the_probabilities(b, h, kv_h, d, n, s, pos, p, dtype):
     c = Cancelling(b, h, kv_h, d, n, s, pos, dtype, prefix=p, spread=8.0)
-    assert work(c, p) >= 1.5e9
+    assert tensor_cores(c, p, True)
     k, v, k64, v64 = c.caches(True)
     out = OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), c.pk.to(DEV), c.pv.to(DEV), k, v, 1.0)
     ref, mag = R.attention_wide(c.q64.to(DEV) * d ** 0.5, k64.to(DEV), v64.to(DEV), pos, prefix=(c.pk.double().to(DEV), c.pv.double().to(DEV)))
@@ -188,8 +192,8 @@ def scored_way(c, seed):
 
 def test_replays_of_launches_that_begin_beside_one_another():
     """Large prefixes with few own keys, and scored calls: launches that skip their wait when the one ahead has told that it may, in graphs."""
-    c = Case(70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], prefix=14001)
-    assert work(c, 14001) >= 1.5e9
+    c = Case(70, 8, 2, 128, 1, 32, [i % 32 for i in range(70)], prefix=24001)
+    assert tensor_cores(c, 24001, True)
     pk, pv, k, v = (t.to(DEV) for t in (c.pk, c.pv, c.k, c.v))
     at, change = moving(c, 1)
     behind = change, lambda: (OPS.attention_shared_prefix(c.q, c.nk, c.nv, at, pk, pv, k, v), k, v)
@@ -202,7 +206,7 @@ def test_replays_of_large_chunks():
     ways = []
     for seed, (b, h, kv_h, d, n, s, pos) in enumerate([(1, 8, 1, 128, 700, 6000, [5100]), (4, 24, 2, 64, 500, 5000, [4000, -1, 0, 777])]):
         c = Case(b, h, kv_h, d, n, s, pos)
-        assert work(c, min(s, 4000 + 129 + n)) >= 5e9
+        assert tensor_cores(c, min(s, 4000 + 129 + n))
         at, change = moving(c, seed + 9)
         k, v = c.k.to(DEV), c.v.to(DEV)
         ways.append((change, lambda c=c, at=at, k=k, v=v: (OPS.attention_cache_window(c.q, c.nk, c.nv, at, k, v, 4000, 129), k, v)))
