@@ -1,5 +1,7 @@
 """The forms of the attention ops over spans of an fp16 cache give the same accuracy: each against the definition in 64 bits."""
 
+import threading
+
 import pytest
 import torch
 
@@ -282,3 +284,120 @@ def test_scored_of_rows_that_see_nothing(b, h, kv_h, d, n, s, pos):
     out = OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), k, v, w)
     assert not out[0, :h // kv_h].any() and torch.equal(w[0, 0], want)
     assert not w.isnan().any() and not out.isnan().any() and (kv_h == 1 or out[0, h // kv_h:].any())
+
+
+def check_wide(c, out, k64, v64, pos, dtype, **kw):
+    ref, mag = R.attention_wide(c.q64.to(DEV), k64.to(DEV), v64.to(DEV), pos, **kw)
+    over = (out.double() - ref).abs() - R.out_bound(ref, mag, dtype)
+    assert _lib.load().alloyb_device_error(1) == 0 and torch.isfinite(out).all() and float(over.max()) <= 0, float(over.max())
+
+
+# the fewest rows that go to tiles of 128: one tile, mostly or nearly empty, full, and one row more
+@pytest.mark.parametrize("b,h,kv_h,d,n,s,window,sinks,dtype,write", [
+    (16, 68, 4, 128, 1, 3700, 9999, 0, torch.float16, True),                       # 17 rows
+    (32, 32, 8, 128, 5, 820, 700, 100, torch.bfloat16, False),                     # 20
+    (24, 12, 4, 64, 11, 2600, 2500, 70, torch.float16, True),                      # 33
+    (6, 8, 8, 128, 127, 800, 600, 3, torch.float16, True),                         # 127
+    (8, 32, 4, 64, 16, 2000, 1990, 0, torch.bfloat16, False),                      # 128
+    (8, 6, 2, 128, 43, 2000, 1900, 65, torch.float16, True),                       # 129
+])
+def test_window_of_few_rows_on_tensor_cores(b, h, kv_h, d, n, s, window, sinks, dtype, write):
+    pos = [(i * 977) % (s - n + 1) if i % 5 != 3 else -1 for i in range(b - 1)] + [s - n]
+    c = Case(b, h, kv_h, d, n, s, pos, dtype)
+    assert tensor_cores(c, min(s, window + sinks + n))
+    k, v, k64, v64 = c.caches(write, window, sinks)
+    k0, v0 = k.clone(), v.clone()
+    out = OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), k, v, window, sinks, -1.0, write)
+    check_wide(c, out, k64, v64, pos, dtype, window=window, sinks=sinks)
+    c.check_written(k0, k, c.nk64, write)
+    c.check_written(v0, v, c.nv64, write)
+
+
+@pytest.mark.parametrize("b,h,kv_h,d,n,p,dtype,write", [
+    (8, 32, 8, 128, 1, 51001, torch.float16, True),                                # 32 rows in all
+    (11, 12, 4, 64, 1, 99000, torch.bfloat16, False),                              # 33
+    (127, 8, 8, 128, 1, 12801, torch.float16, True),                               # 127
+    (32, 8, 2, 64, 1, 50790, torch.float16, False),                                # 128
+    (43, 6, 2, 128, 1, 50400, torch.bfloat16, True),                               # 129
+    (1, 36, 2, 128, 2, 55000, torch.float16, True),                                # 36 rows of one sequence
+    (70, 8, 2, 128, 1, 24001, torch.float16, True),                                # 280
+    (40, 64, 8, 128, 1, 5123, torch.float16, True),                                # 320
+])
+def test_prefix_of_few_rows_on_tensor_cores(b, h, kv_h, d, n, p, dtype, write):
+    s = 150
+    pos = [(i * 37) % (s - n + 1) if i % 6 != 4 else -1 for i in range(b)]
+    c = Case(b, h, kv_h, d, n, s, pos, dtype, prefix=p)
+    assert tensor_cores(c, p, True)
+    k, v, k64, v64 = c.caches(write)
+    k0 = k.clone()
+    store = [torch.full((kv_h, p + 8, d), float("nan"), dtype=torch.float16, device=DEV) for _ in range(2)]
+    for t, src in zip(store, (c.pk, c.pv)):
+        t[:, :p] = src.to(DEV)
+    out = OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), store[0][:, :p], store[1][:, :p], k, v, -1.0, write)
+    check_wide(c, out, k64, v64, pos, dtype, prefix=(c.pk.double().to(DEV), c.pv.double().to(DEV)))
+    c.check_written(k0, k, c.nk64, write)
+
+
+def prefix_and_scored():
+    """Calls whose second launch may begin beside the first, and what each gives alone."""
+    p = 24001
+    c = Case(70, 8, 2, 128, 1, 32, [(i * 5) % 32 for i in range(70)], prefix=p)
+    assert tensor_cores(c, p, True)
+    step, chunk = Case(40, 16, 8, 128, 1, 300, [(i * 37) % 300 for i in range(40)]), Case(2, 32, 8, 64, 12, 900, [700, 880])
+    data = {x: (x.pos_t(), x.k.to(DEV), x.v.to(DEV)) for x in (c, step, chunk)}
+    pk, pv = c.pk.to(DEV), c.pv.to(DEV)
+
+    def prefix():
+        at, k, v = data[c]
+        return OPS.attention_shared_prefix(c.q, c.nk, c.nv, at, pk, pv, kc := k.clone(), vc := v.clone()), kc, vc
+
+    def scored(x):
+        at, k, v = data[x]
+        w = torch.ones(x.b, x.kv_h, x.s, device=DEV)
+        return OPS.attention_cache_scored(x.q, x.nk, x.nv, at, kc := k.clone(), vc := v.clone(), w), kc, vc, w
+
+    calls = [prefix, lambda: scored(step), prefix, lambda: scored(chunk)]
+    alone = []
+    for f in calls:
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in f()])
+        torch.cuda.synchronize()
+    return calls, alone
+
+
+def same_bits(alone, got):
+    for x, y in zip(alone, got):
+        bits = torch.int16 if x.element_size() == 2 else torch.int32
+        assert torch.equal(x.view(bits), y.view(bits))
+
+
+def test_large_prefixes_in_a_row():
+    calls, alone = prefix_and_scored()
+    rounds = [[f() for f in calls] for _ in range(4)]
+    torch.cuda.synchronize()
+    for got in rounds:
+        for a, z in zip(alone, got):
+            same_bits(a, z)
+
+
+def test_large_prefixes_of_two_threads_on_one_stream():
+    calls, alone = prefix_and_scored()
+    got, failed, start = [[], []], [], threading.Barrier(2)
+
+    def turns(i):
+        try:
+            start.wait()
+            for n in range(60):
+                got[i].append(((n + i) % len(calls), calls[(n + i) % len(calls)]()))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    pool = [threading.Thread(target=turns, args=(i,)) for i in range(2)]
+    for t in pool:
+        t.start()
+    for t in pool:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for n, results in got[0] + got[1]:
+        same_bits(alone[n], results)
