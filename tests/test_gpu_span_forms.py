@@ -401,3 +401,35 @@ def test_large_prefixes_of_two_threads_on_one_stream():
     assert not failed
     for n, results in got[0] + got[1]:
         same_bits(alone[n], results)
+
+
+def test_conversation_in_a_bounded_cache():
+    """Steps and evictions in place, sequences that sit calls out among them: every new row is among the next eviction's, the last ones stay, and an
+    idle sequence keeps its rows."""
+    b, h, kv_h, d, s, keep, sinks, recent = 3, 8, 2, 64, 64, 40, 4, 8
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.zeros(b, kv_h, s, d, dtype=torch.float16, device=DEV) for _ in range(2))
+    w = torch.zeros(b, kv_h, s, device=DEV)
+    held = torch.zeros(b, dtype=torch.int32, device=DEV)
+    for step, n in enumerate([30, 20, 1, 1, 17, 1]):
+        idle = torch.tensor([step % 3 == 1, False, step == 2], device=DEV)
+        q, nk, nv = (torch.randn(b, n, x, d, generator=g).half().to(DEV).transpose(1, 2) for x in (h, kv_h, kv_h))
+        pos = torch.where(idle, -1, held)
+        out = OPS.attention_cache_scored(q, nk, nv, pos, k, v, w)
+        ref, _, mag, _ = R.attention(q.double().cpu(), k.double().cpu(), v.double().cpu(), pos.tolist())
+        assert ((out.double().cpu() - ref).abs() <= R.out_bound(ref, mag, torch.float16)).all()
+        before = k.clone()
+        held = torch.where(idle, held, held + n)
+        kept, left = OPS.kv_evict(k, v, w, held, k, v, w, keep, sinks, recent)
+        for i in range(b):
+            rows, new = held[i].item(), left[i].item()
+            assert new == min(rows, keep)
+            if idle[i]:
+                assert kept[i, :, :new].tolist() == [list(range(new))] * kv_h
+            else:
+                last = min(n, recent, rows)
+                assert kept[i, :, new - last:new].tolist() == [list(range(rows - last, rows))] * kv_h
+                assert torch.equal(k[i, :, new - last:new], nk[i, :, n - last:])
+            assert torch.equal(k[i, :, :new], torch.gather(before[i], 1, kept[i, :, :new].long()[..., None].expand(-1, -1, d)))
+        held = left
+    assert ops.span_status() == 0
