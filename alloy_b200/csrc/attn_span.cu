@@ -12,12 +12,13 @@
 //
 // More rows (chunks, and all the batch's rows over a shared prefix; span_rows_kernel).  Bound: mma.sync.  A CTA owns 64 (token, head) rows,
 // a warp 16 of them, and tiles of 64 keys (32 at head_dim 256) that its warps share; the keys are split where the tiles alone leave SMs
-// empty.  Tiles of 32 keys and three CTAs an SM were slower (4 x 16 tokens looking back over 5000 to 8100 keys: 68 -> 81 us), a third stage gave
-// nothing, and with a step's scores a step ahead of its softmax took 70 -> 82.  Many rows with much to do go to attn_span_tc.cu.
+// empty.  4 x 16 scored tokens looking back over 5000 to 8100 keys: 53 us of the call's 67, 48 % of the tensor pipe.  While P was one fp16 half, tiles of
+// 32 keys and three CTAs an SM were slower (the call 68 -> 81 us), a third stage gave nothing, and with a step's scores a step ahead of its softmax it
+// took 70 -> 82.  Many rows with much to do go to attn_span_tc.cu.
 //
 // The weights (scored form): the scores are left in the workspace (4 bytes a row and key beside the 4 D that a key's K and V cost) and a
 // launch of its own adds up exp2(score - the row's log-sum) over a KV head's rows, which needs no second read of K.  It joins the log-sums itself, so the
-// outputs are joined beside it (4 sequences of 16 tokens over 5000 to 8100 keys: 67 -> 60 us).
+// outputs are joined beside it (the call above, with one half of P: 67 -> 60 us).
 //
 // New tokens' rows: keys from `pos` on are read from new_k / new_v, by every CTA that needs them, and written to the cache by one; nobody reads
 // them there in the same launch.
@@ -1095,8 +1096,9 @@ static Plan plan_of(int B, int H, int KV_H, int D, int n, int S, int window, int
 constexpr int64_t SCORES_MOST = int64_t(1) << 30;
 static int scored_tokens(int B, int H, int n, int S) {
     const int64_t token = static_cast<int64_t>(B) * H * ((static_cast<int64_t>(S) + 3) / 4 * 4) * 4;
-    if (n <= 1 || token * n <= SCORES_MOST) return n;
-    const int64_t fit = token < SCORES_MOST ? SCORES_MOST / token : 1, parts = (n + fit - 1) / fit;
+    const int64_t fit = token < SCORES_MOST ? SCORES_MOST / token : 1;
+    if (n <= fit) return n;
+    const int64_t parts = (n + fit - 1) / fit;
     return static_cast<int>((n + parts - 1) / parts);
 }
 

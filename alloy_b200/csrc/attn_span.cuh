@@ -7,7 +7,7 @@ namespace sp {
 
 constexpr float P_BIAS_LOG2 = 6.0f;      // probabilities enter P * V times 64: fp16 keeps 11 bits of one down to 2^-20 of the row's largest
 constexpr float RESCALE_LOG2 = 8.0f;     // accumulators follow a row's maximum in steps of this (P then stays below 2^14)
-constexpr int MAX_BATCH = 1024;          // sequences per call: their step counts are summed in shared memory
+constexpr int MAX_BATCH = 1024;          // sequences per call: every warp of the stream kernel walks all their positions, 32 a round and twice, before it begins
 constexpr int STEP = 64;                 // keys that a CTA takes at a time
 constexpr int WARPS = 4;
 

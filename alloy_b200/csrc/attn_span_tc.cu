@@ -2,7 +2,7 @@
 // prompt under a window, and a large batch's rows over a shared prefix.  attn_span.cu has the rest, and joins partial results.
 //
 // What bounds it: 128 rows x 64 keys take 768 clocks of the tensor pipe at head_dim 128 (S, and P V twice), and their 8192 exponentials 512 clocks of
-// the SM's sixteen a clock; neither is reached in a short call, since scores, exponentials and P V of a row wait for one another.  So an SM has two
+// the SM's sixteen a clock; neither is reached in a short call (66 % of the tensor pipe), since scores, exponentials and P V of a row wait for one another.  So an SM has two
 // CTAs, and a CTA two tiles of scores: while the softmax has one, the tensor pipe has the other one's products and the other CTA's.  In calls one
 // after another for a second the 1000 W limit is the bound.
 //
@@ -16,8 +16,8 @@
 //   128: 172 -> 162 us).
 // * The output is rescaled only when a row's maximum grows by more than 2^8; the stale maximum cancels in the normalisation.
 // Two CTAs of 128 rows, a thread a row, two buffers of 64 scores; measured while P was one half: 136 us for the kernel of that call, where one CTA an
-// SM of 256 rows took 147 to 155, and four warps for the even tiles of keys and four for the odd ones 163.  With both halves of P the call takes 182 us
-// cold (152 with one half; 742 TFLOP/s of the products that the rows see), 64 sequences of 64/8 heads over a prefix of 32768 with own keys and join
+// SM of 256 rows took 147 to 155, and four warps for the even tiles of keys and four for the odd ones 163.  With both halves of P the call takes 183 us
+// cold (152 with one half; 750 TFLOP/s of the operations that the rows ask for), 64 sequences of 64/8 heads over a prefix of 32768 with own keys and join
 // 141 (124); at head_dim 64 160 and 113.  P in pieces of 16 keys on its way to tensor memory keeps the softmax within 128 registers (head_dim 64,
 // the first call: 164 -> 160 us).
 // Every wait is bounded: on a time-out the sticky error word is set, tensor memory is freed and the CTA returns.

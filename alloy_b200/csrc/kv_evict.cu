@@ -8,7 +8,7 @@
 // kept position: 128 items of 4096 kept rows of 3000 to 16384 take 98 us, 5.4 TB/s.  Few items go in one launch (evict_one_kernel).
 //
 // In place a row only moves towards the front: a CTA owns a slice of columns of one (sequence, KV head) and walks the positions in order,
-// all of a batch read before any of it is written, so no row is overwritten before it is read.
+// all of a batch read before any of it is written, so no row is overwritten before it is read: the same 128 items 133 us.
 #include "common.cuh"
 
 namespace alloyb {

@@ -349,8 +349,9 @@ int alloyb_attn_static_status(int32_t* status_out, void* stream);
  * alloyb_span_status.  new_k / new_v (both or neither): the tokens' rows, fp16 (B, KV_H, n_tokens, D) with strides in elements
  * (multiples of 8, 16-byte aligned); they are stored at rows pos + i.  NULL: the cache holds them already.
  * scale <= 0 selects 1/sqrt(D).  Scores, softmax and sums are fp32, the probabilities enter P V as two fp16 halves (22 bits),
- * so an infinity in a V row that a token sees may come out as a NaN; bf16 queries keep all their bits.  What rows hold that no token of a sequence sees does not matter (a NaN or an infinity in a row that one token of a
- * chunk sees may reach the chunk's other tokens).  At most 1024 sequences, B * KV_H <= 65535.
+ * so an infinity in a V row that a token sees may come out as a NaN; bf16 queries keep all their bits.  What rows hold that no
+ * token of a sequence sees does not matter (a NaN or an infinity in a row that one token of a chunk sees may reach the chunk's
+ * other tokens).  At most 1024 sequences, B * KV_H <= 65535, B * n_tokens * H / KV_H <= 2^28.
  * workspace: alloyb_attn_span_workspace_bytes(the same sizes) bytes, 256-byte aligned, undefined before and
  * after: it needs no clearing and must not be shared by calls that may overlap.  window 0 = none; prefix_len and scored
  * as in the call.  0 where the call needs none (workspace may be NULL then), and for sizes that the calls refuse. */
@@ -374,8 +375,8 @@ int alloyb_attn_shared_prefix(const void* q, int64_t q_batch_stride, int64_t q_h
 /* Causal attention over the cache that keeps its weights: weights[b, kvh, j] (fp32, (B, KV_H, S_max) dense) grows by the sum over the
  * KV head's query heads and the call's tokens of the probability that each gives row j.  The entries of the tokens' own rows are
  * set instead: what stood there belonged to a row that is gone.  Entries behind them are left alone.  The sums are taken in a fixed
- * order.  The workspace holds scores, 4 bytes a query row and row of the cache's S_max: calls whose scores would take more than 1 GiB run as several of
- * fewer tokens (at least one, B * H * S_max * 4 bytes), so it grows with n_tokens up to that only. */
+ * order.  The workspace holds scores, 4 bytes a query row and row of S_max: calls whose scores would take more than 1 GiB run
+ * as several of fewer tokens (at least one, B * H * S_max * 4 bytes), so it grows with n_tokens up to that only. */
 int alloyb_attn_scored(const void* q, int64_t q_batch_stride, int64_t q_head_stride, int64_t q_tok_stride, int q_dtype,
                        void* k, void* v, const void* new_k, const void* new_v, int64_t new_batch_stride,
                        int64_t new_head_stride, int64_t new_tok_stride, const int32_t* pos, int pos_count, float* weights,
