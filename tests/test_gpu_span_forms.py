@@ -433,3 +433,58 @@ def test_conversation_in_a_bounded_cache():
             assert torch.equal(k[i, :, :new], torch.gather(before[i], 1, kept[i, :, :new].long()[..., None].expand(-1, -1, d)))
         held = left
     assert ops.span_status() == 0
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_caches_of_more_sequences_than_the_call(n):
+    """The call has the cache's first sequences; the others' rows and weights are left alone."""
+    b, h, kv_h, d, s, p = 2, 8, 2, 128, 200, 70
+    c = Case(b, h, kv_h, d, n, s, [150, 3], prefix=p)
+    wide = [torch.full((b + 2, kv_h, s, d), float("nan"), dtype=torch.float16, device=DEV) for _ in range(2)]
+    w = torch.full((b + 2, kv_h, s), 7.0, device=DEV)
+    k, v, k64, v64 = c.caches(True)
+    for call, kw in (
+        (lambda kk, vv: OPS.attention_cache_window(c.q, c.nk, c.nv, c.pos_t(), kk, vv, 50, 3), dict(window=50, sinks=3)),
+        (lambda kk, vv: OPS.attention_shared_prefix(c.q, c.nk, c.nv, c.pos_t(), c.pk.to(DEV), c.pv.to(DEV), kk, vv), dict(prefix=(c.pk.double(), c.pv.double()))),
+        (lambda kk, vv: OPS.attention_cache_scored(c.q, c.nk, c.nv, c.pos_t(), kk, vv, w), dict()),
+    ):
+        for t, src in zip(wide, (k, v)):
+            t[:b] = src
+        out = call(*wide)
+        ref, _, mag, _ = R.attention(c.q64, k64, v64, c.pos, **kw)
+        assert ((out.double().cpu() - ref).abs() <= R.out_bound(ref, mag, torch.float16)).all()
+        c.check_written(k, wide[0][:b], c.nk64, True)
+        assert wide[0][b:].isnan().all() and wide[1][b:].isnan().all()
+    assert (w[b:] == 7.0).all() and not (w[:b] == 7.0).all()
+
+
+def test_eviction_in_place_replayed():
+    """A graph of an eviction in place gives what the call gives, on other weights and lengths each time."""
+    b, kv_h, s, d, keep = 3, 2, 900, 64, 200
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.zeros(b, kv_h, s, d, dtype=torch.float16, device=DEV) for _ in range(2))
+    w, lengths = torch.zeros(b, kv_h, s, device=DEV), torch.full((b,), s, dtype=torch.int32, device=DEV)
+
+    def call():
+        return OPS.kv_evict(k, v, w, lengths, k, v, w, keep, 4, 50)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, new = call()
+    for turn in range(3):
+        data = [torch.randn(b, kv_h, s, d, generator=g).half(), torch.randn(b, kv_h, s, d, generator=g).half(), torch.rand(b, kv_h, s, generator=g)]
+        lengths.copy_(torch.randint(0, s + 1, (b,), generator=g).int())
+        got = []
+        for run in (lambda: (graph.replay(), (kept, new))[1], call):
+            for t, x in zip((k, v, w), data):
+                t.copy_(x)
+            out = run()
+            torch.cuda.synchronize()
+            got.append([t.clone() for t in (*out, k, v, w)])
+        for x, y in zip(*got):
+            assert torch.equal(x, y)
+        for i in range(b):
+            rows = R.evict(data[2][i, 0].tolist(), lengths[i].item(), keep, 4, 50)
+            assert got[0][0][i, 0].tolist() == rows + [-1] * (keep - len(rows)) and torch.equal(got[0][2][i, 0, :len(rows)].cpu(), data[0][i, 0, rows])
+    assert ops.span_status() == 0
